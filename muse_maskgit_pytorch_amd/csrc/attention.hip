@@ -457,7 +457,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         // (the weights are rounded to bf16 for the PV MFMA, so the hardware exp2, ~1e-6 relative, is exact enough)
         const float mc = -m * c1;
-        // packed fp32 (v_pk_fma_f32 / v_pk_add_f32): this kernel is bound by VALU issue, not by the MFMA pipe
+        // two-element vectors (the build takes no packed fp32 instructions, see build.py): this kernel is bound by VALU issue, not by the MFMA pipe
         const f32x2_t c1v = {c1, c1}, mcv = {mc, mc};
         f32x2_t ps2 = {0.f, 0.f};
 #pragma unroll

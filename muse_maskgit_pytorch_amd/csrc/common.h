@@ -80,9 +80,8 @@ __device__ __forceinline__ float gelu_phi(float x) {
 __device__ __forceinline__ float geglu_f(float x, float gate) {
     return gate * (x * gelu_phi(x));
 }
-// TWO values at once on the packed fp32 instructions (v_pk_mul_f32 / v_pk_fma_f32 / v_pk_add_f32: two lanes' worth of arithmetic per instruction at the full VALU
-// rate): the same IEEE operations in the same order as gelu_phi / geglu_f on each element -- bit-identical results, ~10 instead of 17 instructions per value
-// (the FF w1 epilogue of gemm_wide.hip evaluates 64 per lane and tile)
+// TWO values at once, written on two-element vectors: the same IEEE operations in the same order as gelu_phi / geglu_f on each element -- bit-identical results
+// (the FF w1 epilogue of gemm_wide.hip evaluates 64 per lane and tile).  The build takes no packed fp32 instructions, so each operation is two scalar ones.
 typedef float mm_f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ mm_f32x2_t gelu_phi2(mm_f32x2_t x) {
     const mm_f32x2_t one = {1.f, 1.f};
@@ -311,8 +310,8 @@ __device__ __forceinline__ uint32_t fs_interleave16(uint32_t even, uint32_t odd)
 // exp(x - ml) as v_exp_f32((x - ml) * log2 e): the subtraction first -- exact near the maximum, so the largest value contributes exactly 1 (an FMA
 // form x * log2 e - ml * log2 e rounds the product of the MAGNITUDES: 2e-6 off at |ml| ~ 40, enough to push a dominant token's 1 - p below 0)
 __device__ __forceinline__ float fs_exp(float x, float ml) { return __builtin_amdgcn_exp2f((x - ml) * 1.4426950408889634f); }
-// g(a) = (e0 + e1) + (e2 + e3) of one accumulator fragment with the subtraction and the scaling as PACKED fp32 operations (v_pk_add_f32 / v_pk_mul_f32: two
-// values per instruction at the full VALU rate) -- the same IEEE operations on the same operands in the same order as four fs_exp calls, bit-identical
+// g(a) = (e0 + e1) + (e2 + e3) of one accumulator fragment on two-element vectors -- the same IEEE operations on the same operands in the same order as four
+// fs_exp calls, bit-identical
 typedef float fs_f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float fs_exp_sum4(float x0, float x1, float x2, float x3, float ml) {
     const fs_f32x2_t m2 = {ml, ml}, l2 = {1.4426950408889634f, 1.4426950408889634f};
