@@ -267,6 +267,81 @@ int mm_qk_norm_bwd(mm_stream_t stream, const void* x, int64_t ldx, const float* 
                    const float* dy_f32, const float* scale, int64_t rows, int heads_per_row, void* dx, int64_t lddx,
                    float* dx_f32, float* dscale_part);
 
+/* ---- packed rows: documents (images of several sizes, with or without their text) one behind another in one row of tokens.  Added to ABI 9: new entry points only. */
+
+#define MM_DT_BF16 0
+#define MM_DT_F16 1
+#define MM_DT_F32 2
+
+/* Which keys a query row sees, as one interval per row: out int32 [B][n][2] = (lo, hi), keys lo <= k < hi of a key row of j keys.  Document doc owns the query rows
+ * cu_q[doc] <= i < cu_q[doc + 1] and the keys cu_k[doc] <= k < cu_k[doc + 1] (int32 [docs + 1], not decreasing; q_sb / k_sb / p_sb: batch strides in elements, 0 = one
+ * table for all rows; bounds outside [0, j] are clamped).  causal != 0: query i of lq sees the first i + 1 + lk - lq of its document's lk keys, and at least the first
+ * prefix[doc] of them (optional int32 [docs]).  Rows of no document see nothing: (0, 0). */
+int mm_attention_spans(mm_stream_t stream, const int32_t* cu_q, int64_t q_sb, const int32_t* cu_k, int64_t k_sb, const int32_t* prefix, int64_t p_sb,
+                       int B, int docs, int n, int j, int causal, int32_t* out);
+
+/* Rotary positions over 1 .. 4 axes on the heads of q and of k in one launch.  The first 2 P elements of a head (P = sum of the sections) are P pairs -- elements
+ * (p, P + p), or (2p, 2p + 1) with interleaved -- and pair p of section a turns by positions[..][a] * freqs[p] radians (fp64 freqs; the angle is formed in 64 bits);
+ * the rest passes.  normalize != 0: y = x / max(|x|, 1e-12) * scale in front of the turn (mmp.py:151-153).  positions int32 [B][n][axes] (pos_sb 0: one [n][axes]
+ * for all rows).  x: element strides (batch, head, token), head elements contiguous, heads == 0: absent.  out: contiguous [B][n][heads][dim].  dim even, <= 128;
+ * up to 256 where rows are 16-byte aligned and, without interleaved, P % 8 == 0 and (dim - 2 P) % 16 == 0 (then 16-byte accesses).
+ * mm_rotary_axes_bwd: dy -> out = gradient of x; with normalize x is read again and dscales fp32 [2][dim] = gradients of (q.scale, k.scale); ws:
+ * mm_rotary_axes_bwd_workspace_bytes(desc) bytes (0 without normalize).  Deterministic. */
+typedef struct {
+    const void* x;
+    const void* dy;
+    void* out;
+    const float* scale;
+    int64_t x_stride[3];
+    int64_t dy_stride[3];
+    int32_t heads;
+    int32_t reserved;
+} mm_rotary_side;
+typedef struct {
+    mm_rotary_side q, k;
+    const int32_t* positions;
+    int64_t pos_sb;
+    const double* freqs;
+    int32_t sections[4];
+    int32_t axes, batch, n, dim, dtype, interleaved, normalize, reserved;
+} mm_rotary;
+int mm_rotary_axes(mm_stream_t stream, const mm_rotary* desc);
+size_t mm_rotary_axes_bwd_workspace_bytes(const mm_rotary* desc);
+int mm_rotary_axes_bwd(mm_stream_t stream, const mm_rotary* desc, float* dscales, void* ws, size_t ws_bytes);
+
+/* Attention of packed rows: for the keys that query i sees (spans, and key_mask uint8 [B][nk], 1 = keep; both optional)
+ *     s = cap(scale q.k) - sum_a slopes[h][a] |positions_q[i][a] - positions_k[key][a]|,   cap(s) = softcap tanh(s / softcap) for softcap > 0,
+ *     out = softmax(s) v,   lse = log sum exp(s).   A row that sees nothing: out 0, lse -inf.
+ * q [B][Hq][nq][dim], k / v [B][Hk][nk][dim], Hk a divisor of Hq (query head h reads key head h / (Hq / Hk)); bf16 or fp16; dim 32, 64 or 128; element strides
+ * (batch, head, token), multiples of 8, head elements contiguous, 16-byte aligned; token strides of k and v at least dim.  slopes fp32 [Hq][axes], axes 0 .. 3,
+ * positions int32 [B][n][axes] (batch stride 0: one for all rows), |position| < 2^30.  lse fp32 [B][Hq][nq] (optional in the forward).  scale > 0.
+ * Few queries over many keys: the keys are split over workgroups, partial results in ws (mm_span_attention_workspace_bytes, may be 0) joined in a fixed order.
+ * What a row does not see never reaches it, infinities and NaN included.
+ * mm_span_attention_bwd (bf16): from q, k, v, out, lse and dout (strided like out) the gradients dq / dk / dv (bf16, own strides) and, with slopes, dslopes fp32
+ * [Hq][axes] (optional).  Rows whose lse is -inf contribute nothing.  Deterministic: no atomics; key gradients are summed over the heads that share a key head. */
+typedef struct {
+    const void* q; const void* k; const void* v;
+    void* out;
+    float* lse;
+    const int32_t* spans; int64_t spans_sb;          /* [B or 1][nq][2] */
+    const uint8_t* key_mask; int64_t key_mask_sb;
+    const float* slopes;
+    const int32_t* positions_q; int64_t positions_q_sb;
+    const int32_t* positions_k; int64_t positions_k_sb;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+    int32_t batch, heads_q, heads_k, nq, nk, dim, axes, dtype;
+    float scale, softcap;
+    /* backward only */
+    const void* dout;
+    void* dq; void* dk; void* dv;
+    float* dslopes;
+    int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} mm_span_attn;
+size_t mm_span_attention_workspace_bytes(const mm_span_attn* desc);
+int mm_span_attention(mm_stream_t stream, const mm_span_attn* desc, void* ws, size_t ws_bytes);
+size_t mm_span_attention_bwd_workspace_bytes(const mm_span_attn* desc);
+int mm_span_attention_bwd(mm_stream_t stream, const mm_span_attn* desc, void* ws, size_t ws_bytes);
+
 /* The uniforms MM_NOISE_PHILOX draws for rows [row_offset, row_offset + rows) at `step`: out fp32 [rows][V]. */
 int mm_philox_uniform(mm_stream_t stream, uint64_t seed, uint64_t row_offset, uint32_t step, int rows, int V,
                       float* out);

@@ -75,6 +75,27 @@ class VaeDesc(C.Structure):
                 ('alpha', c_f32), ('reserved', C.c_int32)]
 
 
+MM_DT_BF16, MM_DT_F16, MM_DT_F32 = 0, 1, 2
+
+
+class RotarySide(C.Structure):
+    _fields_ = [(n, c_vp) for n in ('x', 'dy', 'out', 'scale')] + [('x_stride', c_i64 * 3), ('dy_stride', c_i64 * 3), ('heads', C.c_int32), ('reserved', C.c_int32)]
+
+
+class Rotary(C.Structure):
+    _fields_ = [('q', RotarySide), ('k', RotarySide), ('positions', c_vp), ('pos_sb', c_i64), ('freqs', c_vp), ('sections', C.c_int32 * 4)] + \
+               [(n, C.c_int32) for n in ('axes', 'batch', 'n', 'dim', 'dtype', 'interleaved', 'normalize', 'reserved')]
+
+
+class SpanAttn(C.Structure):
+    _fields_ = [(n, c_vp) for n in ('q', 'k', 'v', 'out', 'lse')] + \
+               [('spans', c_vp), ('spans_sb', c_i64), ('key_mask', c_vp), ('key_mask_sb', c_i64), ('slopes', c_vp),
+                ('positions_q', c_vp), ('positions_q_sb', c_i64), ('positions_k', c_vp), ('positions_k_sb', c_i64)] + \
+               [(n, c_i64 * 3) for n in ('q_stride', 'k_stride', 'v_stride', 'out_stride')] + \
+               [(n, C.c_int32) for n in ('batch', 'heads_q', 'heads_k', 'nq', 'nk', 'dim', 'axes', 'dtype')] + [('scale', c_f32), ('softcap', c_f32)] + \
+               [(n, c_vp) for n in ('dout', 'dq', 'dk', 'dv', 'dslopes')] + [(n, c_i64 * 3) for n in ('dout_stride', 'dq_stride', 'dk_stride', 'dv_stride')]
+
+
 class GenerateParams(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ('batch', 'n', 'timesteps', 'k_keep', 'noise_kind', 'nc', 'L', 'flags')] + \
                [('cond_scale', c_f32), ('pad0', c_f32), ('seed', c_u64), ('row_offset', c_u64),
@@ -135,6 +156,14 @@ SIGNATURES = {
     'mm_scatter_rows_bf16': (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_vp]),
     'mm_sum_parts_bf16': (c_int, [c_vp, c_vp, c_int, c_i64, c_vp]),
     'mm_attention_bwd': (c_int, [c_vp] + [c_vp, c_i64, c_i64, c_i64] * 8 + [c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_f32]),
+    'mm_attention_spans': (c_int, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_int, c_int, c_int, c_int, c_int, c_vp]),
+    'mm_rotary_axes': (c_int, [c_vp, C.POINTER(Rotary)]),
+    'mm_rotary_axes_bwd_workspace_bytes': (c_sz, [C.POINTER(Rotary)]),
+    'mm_rotary_axes_bwd': (c_int, [c_vp, C.POINTER(Rotary), c_vp, c_vp, c_sz]),
+    'mm_span_attention_workspace_bytes': (c_sz, [C.POINTER(SpanAttn)]),
+    'mm_span_attention': (c_int, [c_vp, C.POINTER(SpanAttn), c_vp, c_sz]),
+    'mm_span_attention_bwd_workspace_bytes': (c_sz, [C.POINTER(SpanAttn)]),
+    'mm_span_attention_bwd': (c_int, [c_vp, C.POINTER(SpanAttn), c_vp, c_sz]),
     'mm_qk_norm_bwd_blocks': (c_i64, [c_i64]),
     'mm_qk_norm_bwd': (c_int, [c_vp, c_vp, c_i64, c_vp, c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_vp]),
     'mm_train_step_workspace_bytes': (c_sz, [C.POINTER(TrainDesc), c_int, c_int, c_int, c_int]),

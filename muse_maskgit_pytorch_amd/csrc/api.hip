@@ -466,6 +466,140 @@ int mm_attention_bwd(mm_stream_t stream, const void* q, int64_t q_sb, int64_t q_
                            q_scale, k_scale, null_k, null_v, scale);
 }
 
+int mm_attention_spans(mm_stream_t stream, const int32_t* cu_q, int64_t q_sb, const int32_t* cu_k, int64_t k_sb, const int32_t* prefix, int64_t p_sb,
+                       int B, int docs, int n, int j, int causal, int32_t* out) {
+    if (B < 0 || n < 0 || j < 0 || docs < 0 || B > 65535) return mm_set_error(MM_ERR_SHAPE, "attention_spans: sizes (batch <= 65535)");
+    if (B == 0 || n == 0) return MM_OK;
+    CHK_PTR(cu_q, "cu_q"); CHK_PTR(cu_k, "cu_k"); CHK_PTR(out, "out");
+    if (((uintptr_t)out) & 7) return mm_set_error(MM_ERR_ALIGN, "attention_spans: out must be 8-byte aligned");
+    return k_attention_spans((hipStream_t)stream, cu_q, q_sb, cu_k, k_sb, prefix, p_sb, B, docs, n, j, causal, out);
+}
+
+static int rotary_check(const mm_rotary* r, bool bwd) {
+    if (!r) return mm_set_error(MM_ERR_SHAPE, "rotary: desc is NULL");
+    if (r->dtype != MM_DT_BF16 && r->dtype != MM_DT_F16 && r->dtype != MM_DT_F32) return mm_set_error(MM_ERR_DTYPE, "rotary: bf16, fp16 or fp32");
+    if (r->axes < 1 || r->axes > 4) return mm_set_error(MM_ERR_SHAPE, "rotary: 1 to 4 axes");
+    long P = 0;
+    for (int a = 0; a < r->axes; ++a) {
+        if (r->sections[a] < 0 || r->sections[a] > 128) return mm_set_error(MM_ERR_SHAPE, "rotary: a section is 0 .. 128 pairs");
+        P += r->sections[a];
+    }
+    if (r->batch < 0 || r->n < 0 || r->q.heads < 0 || r->k.heads < 0 || r->q.heads > 4096 || r->k.heads > 4096) return mm_set_error(MM_ERR_SHAPE, "rotary: sizes");
+    if (r->dim < 2 || r->dim > 256 || r->dim % 2 || 2 * P > r->dim) return mm_set_error(MM_ERR_SHAPE, "rotary: dim even, at most 256, at least twice the sum of the sections");
+    if (r->batch == 0 || r->n == 0 || r->q.heads + r->k.heads == 0) return MM_OK;
+    CHK_PTR(r->positions, "rotary: positions");
+    if (P > 0) CHK_PTR(r->freqs, "rotary: freqs");
+    for (int w = 0; w < 2; ++w) {
+        const mm_rotary_side* t = w ? &r->k : &r->q;
+        if (t->heads == 0) continue;
+        CHK_PTR(t->out, "rotary: out");
+        if (!bwd || r->normalize) CHK_PTR(t->x, "rotary: x");
+        if (bwd) CHK_PTR(t->dy, "rotary: dy");
+        if (r->normalize) CHK_PTR(t->scale, "rotary: scale");
+    }
+    return MM_OK;
+}
+static int rotary_run(mm_stream_t stream, const mm_rotary* desc, bool bwd, float* ws, float* dscales) {
+    if (desc->dim > 128 && k_rotary_parts(desc) < 0) return mm_set_error(MM_ERR_UNSUPPORTED, "rotary: dim above 128 needs 16-byte aligned rows, and without interleaved sections that add up to a multiple of 8 with a rest of whole 16 elements");
+    return k_rotary((hipStream_t)stream, desc, bwd, ws, dscales);
+}
+int mm_rotary_axes(mm_stream_t stream, const mm_rotary* desc) {
+    const int rc = rotary_check(desc, false);
+    if (rc) return rc;
+    return rotary_run(stream, desc, false, nullptr, nullptr);
+}
+size_t mm_rotary_axes_bwd_workspace_bytes(const mm_rotary* desc) {
+    if (rotary_check(desc, true) || !desc->normalize) return 0;
+    const long parts = k_rotary_parts(desc);
+    return parts > 0 ? (size_t)parts * 2 * desc->dim * sizeof(float) : 0;
+}
+int mm_rotary_axes_bwd(mm_stream_t stream, const mm_rotary* desc, float* dscales, void* ws, size_t ws_bytes) {
+    const int rc = rotary_check(desc, true);
+    if (rc) return rc;
+    if (desc->normalize) {
+        CHK_PTR(dscales, "rotary: dscales");
+        const size_t need = mm_rotary_axes_bwd_workspace_bytes(desc);
+        if (need && (!ws || ws_bytes < need)) return mm_set_error(MM_ERR_WORKSPACE, "rotary: workspace too small (mm_rotary_axes_bwd_workspace_bytes)");
+    }
+    return rotary_run(stream, desc, true, (float*)ws, dscales);
+}
+
+// strides of a 16-bit operand that is read in 16-byte pieces (tok >= 0: the token stride is at least that); dimensions of one element have no stride to check
+static int span_operand(const void* ptr, const int64_t* st, const int* n, int tok, const char* name) {
+    static thread_local char msg[160];
+    if (!ptr) { snprintf(msg, sizeof(msg), "span attention: %s is NULL", name); return mm_set_error(MM_ERR_SHAPE, msg); }
+    if (((uintptr_t)ptr) & 15) { snprintf(msg, sizeof(msg), "span attention: %s must be 16-byte aligned", name); return mm_set_error(MM_ERR_ALIGN, msg); }
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] <= 1) continue;
+        if (st[i] < 0 || st[i] % 8) { snprintf(msg, sizeof(msg), "span attention: strides of %s must be multiples of 8 elements, not negative", name); return mm_set_error(MM_ERR_ALIGN, msg); }
+    }
+    if (n[2] > 1 && (st[2] < tok || st[2] > (1 << 22))) { snprintf(msg, sizeof(msg), "span attention: token stride of %s at least the width and at most 2^22 elements", name); return mm_set_error(MM_ERR_SHAPE, msg); }
+    return MM_OK;
+}
+static int span_check(const mm_span_attn* a, bool bwd) {
+    if (!a) return mm_set_error(MM_ERR_SHAPE, "span attention: desc is NULL");
+    if (bwd ? a->dtype != MM_DT_BF16 : (a->dtype != MM_DT_BF16 && a->dtype != MM_DT_F16))
+        return mm_set_error(MM_ERR_DTYPE, bwd ? "span attention: the backward takes bf16" : "span attention: bf16 or fp16");
+    if (a->dim != 32 && a->dim != 64 && a->dim != 128) return mm_set_error(MM_ERR_UNSUPPORTED, "span attention: dim 32, 64 or 128");
+    if (a->batch < 0 || a->nq < 0 || a->nk < 0 || a->heads_q < 1 || a->heads_k < 1 || a->heads_q % a->heads_k || a->heads_q > 1024)
+        return mm_set_error(MM_ERR_SHAPE, "span attention: sizes (heads_k divides heads_q, at most 1024 heads)");
+    if (a->batch > (1 << 20) || a->nq > (1 << 28) || a->nk > (1 << 28) || (int64_t)a->batch * a->heads_q * ((a->nq + 31) / 32 + 1) > (1 << 28) ||
+        (int64_t)a->batch * a->heads_q * ((a->nk + 31) / 32 + 1) > (1 << 28))
+        return mm_set_error(MM_ERR_SHAPE, "span attention: too many rows for one call");
+    if (!(a->scale > 0.f) || a->scale > 1e30f) return mm_set_error(MM_ERR_SHAPE, "span attention: scale must be positive");
+    if (!(a->softcap >= 0.f) || a->softcap > 1e30f) return mm_set_error(MM_ERR_SHAPE, "span attention: softcap must be 0 (none) or positive");
+    if (a->axes < 0 || a->axes > 3 || (a->slopes && a->axes == 0)) return mm_set_error(MM_ERR_SHAPE, "span attention: 1 to 3 axes for the distance bias");
+    if (a->slopes && (!a->positions_q || !a->positions_k)) return mm_set_error(MM_ERR_SHAPE, "span attention: slopes need positions of queries and keys");
+    if (a->spans && (((uintptr_t)a->spans) & 7)) return mm_set_error(MM_ERR_ALIGN, "span attention: spans must be 8-byte aligned");
+    if (a->spans && a->spans_sb % 2) return mm_set_error(MM_ERR_ALIGN, "span attention: spans batch stride must be even");
+    if (a->batch == 0) return MM_OK;
+    const int nq[3] = {a->batch, a->heads_q, a->nq}, nk[3] = {a->batch, a->heads_k, a->nk};
+    int rc = MM_OK;
+    if (a->nq > 0) {
+        if ((rc = span_operand(a->q, a->q_stride, nq, 0, "q"))) return rc;
+        if ((rc = span_operand(a->out, a->out_stride, nq, 1, "out"))) return rc;
+    }
+    if (a->nk > 0) {
+        if ((rc = span_operand(a->k, a->k_stride, nk, a->dim, "k"))) return rc;
+        if ((rc = span_operand(a->v, a->v_stride, nk, a->dim, "v"))) return rc;
+    }
+    if (!bwd) return MM_OK;
+    if (a->nq > 0) {
+        CHK_PTR(a->lse, "span attention: lse");
+        if ((rc = span_operand(a->dout, a->dout_stride, nq, 0, "dout"))) return rc;
+        if ((rc = span_operand(a->dq, a->dq_stride, nq, 1, "dq"))) return rc;
+    }
+    if (a->nk > 0) {
+        if ((rc = span_operand(a->dk, a->dk_stride, nk, 1, "dk"))) return rc;
+        if ((rc = span_operand(a->dv, a->dv_stride, nk, 1, "dv"))) return rc;
+    }
+    return MM_OK;
+}
+size_t mm_span_attention_workspace_bytes(const mm_span_attn* desc) {
+    if (span_check(desc, false) || desc->batch == 0 || desc->nq == 0) return 0;
+    return k_span_attn_workspace_bytes(desc);
+}
+int mm_span_attention(mm_stream_t stream, const mm_span_attn* desc, void* ws, size_t ws_bytes) {
+    const int rc = span_check(desc, false);
+    if (rc || desc->batch == 0 || desc->nq == 0) return rc;
+    const size_t need = k_span_attn_workspace_bytes(desc);
+    if (need && (!ws || ws_bytes < need)) return mm_set_error(MM_ERR_WORKSPACE, "span attention: workspace too small (mm_span_attention_workspace_bytes)");
+    if (need && (((uintptr_t)ws) & 15)) return mm_set_error(MM_ERR_ALIGN, "span attention: workspace must be 16-byte aligned");
+    return k_span_attn((hipStream_t)stream, desc, ws);
+}
+size_t mm_span_attention_bwd_workspace_bytes(const mm_span_attn* desc) {
+    if (span_check(desc, true) || desc->batch == 0) return 0;
+    return k_span_attn_bwd_workspace_bytes(desc);
+}
+int mm_span_attention_bwd(mm_stream_t stream, const mm_span_attn* desc, void* ws, size_t ws_bytes) {
+    const int rc = span_check(desc, true);
+    if (rc || desc->batch == 0) return rc;
+    const size_t need = k_span_attn_bwd_workspace_bytes(desc);
+    if (need && (!ws || ws_bytes < need)) return mm_set_error(MM_ERR_WORKSPACE, "span attention: workspace too small (mm_span_attention_bwd_workspace_bytes)");
+    if (need && (((uintptr_t)ws) & 15)) return mm_set_error(MM_ERR_ALIGN, "span attention: workspace must be 16-byte aligned");
+    return k_span_attn_bwd((hipStream_t)stream, desc, ws);
+}
+
 int64_t mm_qk_norm_bwd_blocks(int64_t nvec) { return k_qk_norm_bwd_blocks(nvec); }
 
 int mm_qk_norm_bwd(mm_stream_t stream, const void* x, int64_t ldx, const float* x_f32, int H, const void* dy, int64_t lddy,

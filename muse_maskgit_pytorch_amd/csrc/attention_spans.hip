@@ -1,0 +1,563 @@
+// Attention of packed rows, forward:   out_i = sum over the keys lo_i <= key < hi_i of softmax(s)_key v_key,   s = cap(scale q.k) - sum_a slope_a |pos_q - pos_k|
+// One pass over the keys with a running maximum and sum per query.  S^T = K Q^T puts a query into a lane's column (common layout in span_attn.h): its scores, maximum,
+// sum and the rescaling of its output stay in that lane (and its partner in the other half wave), P needs no LDS, O^T = V^T P^T.
+//   span_attn_wide   : 128 queries of one head (4 waves x 32), key tiles of 64 shared by the waves, double-buffered by LDS-DMA.  A wave passes over tiles that none of
+//                      its rows sees; tiles that all of its rows see whole take no mask.
+//   span_attn_narrow : few rows (a new position over a cache, one image): 32 rows = (heads that share a key head) x queries; the four waves take every fourth 32-key tile
+//                      each, on their own, and are joined through LDS; longer key ranges are split over workgroups as well and joined by span_attn_join in split order.
+// What a row does not see never reaches it: rows behind the workgroup's key range are not read (zeros), rows that the key mask hides are cleared in LDS, and a row whose
+// output is not finite although its sum is -- another row's infinity or NaN met its zero weight in the matrix instruction -- is computed again from its own keys alone.
+#include <string.h>
+
+#include "span_attn.h"
+
+namespace {
+
+constexpr int WQ = 128, KT = 64;
+
+// sum over this row's visible keys in [k0, k1) of exp2(s - m) v, by one wave: lane = key for the scores, lane = element for the sum
+template <int D, bool F16, int AX>
+__device__ __forceinline__ void row_again(const SpanArgs& p, int b, int h, int i, int k0, int k1, float m, int lane, float (&o)[2]) {
+    const uint16_t* q = p.q + b * p.q_s[0] + h * p.q_s[1] + (long)i * p.q_s[2];
+    const int hk = h / (p.Hq / p.Hk);
+    const uint16_t* kb = p.k + b * p.k_s[0] + hk * p.k_s[1];
+    const uint16_t* vb = p.v + b * p.v_s[0] + hk * p.v_s[1];
+    o[0] = o[1] = 0.f;
+#pragma nounroll
+    for (int t0 = k0; t0 < k1; t0 += 64) {
+        const int key = t0 + lane;
+        float w = 0.f, unused;
+        if (key < k1 && (!p.kmask || p.kmask[b * p.km_sb + key])) w = __builtin_amdgcn_exp2f(pair_score<D, F16, AX>(p, q, kb + (long)key * p.k_s[2], b, h, i, key, &unused) - m);
+#pragma nounroll
+        for (int e = 0; e < min(64, k1 - t0); ++e) {
+            const float we = __shfl(w, e, 64);
+            if (p.kmask && !p.kmask[b * p.km_sb + t0 + e]) continue;
+            const uint16_t* v = vb + (long)(t0 + e) * p.v_s[2];
+            if (lane < D) o[0] = __builtin_fmaf(we, to_f32<F16>(v[lane]), o[0]);
+            if (D > 64) o[1] = __builtin_fmaf(we, to_f32<F16>(v[lane + 64]), o[1]);
+        }
+    }
+}
+
+// scores of NS 32-key blocks of one tile (raw products in) -> log2 units with cap, bias and mask; returns the lane's largest
+template <int AX, int NS>
+__device__ __forceinline__ float scores(f32x16_t (&s)[NS], float cap, float c1, float c2, const int (&pq)[AX ? AX : 1], const float (&sl)[AX ? AX : 1], const int* pk, int half,
+                                        bool masked, unsigned long long bits) {
+    if (cap > 0.f) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[n][r] = span_tanh(s[n][r], c1) * c2;
+    } else {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[n][r] *= c1;
+    }
+    if constexpr (AX > 0) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                int4 kp[AX];
+#pragma unroll
+                for (int a = 0; a < AX; ++a) kp[a] = *reinterpret_cast<const int4*>(pk + a * NS * 32 + n * 32 + g * 8 + half * 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int a = 0; a < AX; ++a) {
+                        const int kv = e == 0 ? kp[a].x : (e == 1 ? kp[a].y : (e == 2 ? kp[a].z : kp[a].w));
+                        s[n][g * 4 + e] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - kv)), s[n][g * 4 + e]);
+                    }
+            }
+    }
+    if (masked) {
+        bits >>= 4 * half;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            const uint32_t w = (uint32_t)(bits >> (32 * n));
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!(w & (1u << (8 * (r >> 2) + (r & 3))))) s[n][r] = -INFINITY;
+        }
+    }
+    float m = s[0][0];
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, s[n][r]);
+    return m;
+}
+
+// one tile into the running state (m: same in both halves; l: this half's part)
+template <int D, bool F16, int NS>
+__device__ __forceinline__ void soften(f32x16_t (&s)[NS], float tmax, float& m, float& l, f32x16_t (&o)[D / 32], u32x4_t (&pf)[2 * NS]) {
+    tmax = both_halves_max(tmax);
+    // the maximum moves only when some row's grows by more than 2^8: P stays below 2^8, exact enough in 16 bits, and most tiles rescale nothing
+    if (__any(tmax > m + 8.f)) {
+        const float mn = fmaxf(m, tmax), f = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[c][r] *= f;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - m);
+            sum += s[n][r];
+        }
+        // rounding of P to 16 bits: the products with V need it; the sum takes the unrounded values
+        pf[2 * n] = pack_slots<F16>(s[n], 0);
+        pf[2 * n + 1] = pack_slots<F16>(s[n], 1);
+    }
+    l += sum;
+}
+
+template <int D, bool F16, int AX>
+__global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
+    typedef Tile<D, KT> T;
+    extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
+    constexpr int POS = AX * KT * 4, STAGE = 2 * T::BYTES + POS;
+    int* red = reinterpret_cast<int*>(smem + 2 * STAGE);
+    const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+    // workgroups go to the 8 XCDs in turn: each XCD takes a contiguous part of (row, head, tile), so a head's keys are read into one L2; the last tiles of a head
+    // first (in ordered documents they see the most)
+    const int tiles = (p.nq + WQ - 1) / WQ, total = p.B * p.Hq * tiles, per = (total + 7) / 8;
+    const int item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || item >= total) return;
+    const int tile = tiles - 1 - item % tiles, h = (item / tiles) % p.Hq, b = item / tiles / p.Hq, hk = h / (p.Hq / p.Hk);
+    const int i = tile * WQ + w * 32 + (lane & 31);
+    const bool ok = i < p.nq;
+
+    int lo = 0, hi = 0;
+    if (ok) {
+        hi = p.nk;
+        if (p.spans) {
+            const int2 sp = reinterpret_cast<const int2*>(p.spans + b * p.spans_sb)[i];
+            lo = max(sp.x, 0); hi = min(sp.y, p.nk);
+        }
+        if (lo >= hi) lo = hi = 0;
+    }
+    int h0 = hi > lo ? lo : INT32_MAX, h1 = hi;
+    for (int o = 16; o > 0; o >>= 1) { h0 = min(h0, __shfl_xor(h0, o, 64)); h1 = max(h1, __shfl_xor(h1, o, 64)); }
+    if (lane == 0) { red[w] = h0; red[4 + w] = h1; }
+    u32x4_t qf[D / 16];
+    {
+        const uint16_t* qp = p.q + b * p.q_s[0] + h * p.q_s[1] + (long)(ok ? i : 0) * p.q_s[2] + half * 8;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) qf[c] = *reinterpret_cast<const u32x4_t*>(qp + c * 16);
+    }
+    float sl[AX ? AX : 1]; int pq[AX ? AX : 1];
+#pragma unroll
+    for (int a = 0; a < AX; ++a) {
+        sl[a] = p.slopes[h * AX + a] * SPAN_LOG2E;
+        pq[a] = ok ? p.pos_q[b * p.pq_sb + (long)i * AX + a] : 0;
+    }
+    __syncthreads();
+    const int k0 = __builtin_amdgcn_readfirstlane(min(min(red[0], red[1]), min(red[2], red[3])));
+    const int k1 = __builtin_amdgcn_readfirstlane(max(max(red[4], red[5]), max(red[6], red[7])));
+    const int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
+
+    const uint16_t* kp = p.k + b * p.k_s[0] + hk * p.k_s[1];
+    const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1];
+    const uint8_t* km = p.kmask ? p.kmask + b * p.km_sb : nullptr;
+    const int* pkp = AX ? p.pos_k + b * p.pk_sb : nullptr;
+    const bool capped = p.cap > 0.f;
+    const float c1 = capped ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E, c2 = p.cap * SPAN_LOG2E;
+
+#define SPAN_ISSUE(it_)                                                                                                \
+    {                                                                                                                  \
+        const int t0_ = k0 + (it_) * KT;                                                                               \
+        unsigned char* st_ = smem + ((it_) & 1) * STAGE;                                                               \
+        T::template fill<4>(st_, kp + (long)t0_ * p.k_s[2], min(KT, k1 - t0_), (int)p.k_s[2], w, lane);                \
+        T::template fill<4>(st_ + T::BYTES, vp + (long)t0_ * p.v_s[2], min(KT, k1 - t0_), (int)p.v_s[2], w, lane);     \
+    }
+#define SPAN_POS_LOAD(it_) \
+    if constexpr (AX > 0) { if (t < KT * AX) { const int key_ = k0 + (it_) * KT + t / AX; posv = key_ < k1 ? pkp[(long)key_ * AX + t % AX] : 0; } }
+#define SPAN_POS_STORE(it_) \
+    if constexpr (AX > 0) { if (t < KT * AX) reinterpret_cast<int*>(smem + ((it_) & 1) * STAGE + 2 * T::BYTES)[(t % AX) * KT + t / AX] = posv; }
+
+    float m = SPAN_LOW, l = 0.f;
+    f32x16_t o[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[c][r] = 0.f;
+    int posv = 0;
+    if (nt > 0) {
+        SPAN_ISSUE(0);
+        SPAN_POS_LOAD(0);
+        SPAN_POS_STORE(0);
+    }
+    for (int it = 0; it < nt; ++it) {
+        const int t0 = k0 + it * KT;
+        unsigned char* Ks = smem + (it & 1) * STAGE;
+        unsigned char* Vs = Ks + T::BYTES;
+        unsigned long long keep = ~0ull;
+        if (km) keep = __ballot(t0 + lane < k1 && km[t0 + lane]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();      // this tile has landed for every wave, and every wave is done with the other stage
+        if (it + 1 < nt) { SPAN_ISSUE(it + 1); SPAN_POS_LOAD(it + 1); }
+        if (keep != ~0ull) {
+            T::clear_rows(Vs, keep, t, 256);
+            __syncthreads();
+        }
+        if (__any(lo < t0 + KT && hi > t0)) {
+            f32x16_t s[2];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                s[0] = mfma32<F16>(T::rows(Ks, c, 0, lane), qf[c], s[0]);
+                s[1] = mfma32<F16>(T::rows(Ks, c, 1, lane), qf[c], s[1]);
+            }
+            const bool masked = keep != ~0ull || !__all(lo <= t0 && hi >= t0 + KT);
+            const float tmax = scores<AX, 2>(s, p.cap, c1, c2, pq, sl, reinterpret_cast<const int*>(Ks + 2 * T::BYTES), half, masked, masked ? bit_range(lo - t0, hi - t0) & keep : 0ull);
+            u32x4_t pf[4];
+            soften<D, F16, 2>(s, tmax, m, l, o, pf);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) o[c] = mfma32<F16>(T::cols(Vs, ks, c, lane), pf[ks], o[c]);
+        }
+        if (it + 1 < nt) SPAN_POS_STORE(it + 1);
+    }
+#undef SPAN_ISSUE
+#undef SPAN_POS_LOAD
+#undef SPAN_POS_STORE
+
+    l = both_halves_sum(l);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    if (p.lse && ok && half == 0) p.lse[((long)b * p.Hq + h) * p.nq + i] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * SPAN_LN2 : (l == 0.f ? -INFINITY : l);
+    float bad = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(o[c][r], 0.f, bad);
+    bad = both_halves_sum(bad);
+    const bool redo = ok && bad != 0.f && l * 0.f == 0.f;      // (bad is 0 or NaN; NaN != 0)
+    if (ok && !redo) {
+        const float f = l != l ? l : inv;
+        uint16_t* op = p.out + b * p.o_s[0] + h * p.o_s[1] + (long)i * p.o_s[2] + half * 4;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<uint2*>(op + c * 32 + g * 8) = make_uint2(pack2<F16>(o[c][4 * g] * f, o[c][4 * g + 1] * f), pack2<F16>(o[c][4 * g + 2] * f, o[c][4 * g + 3] * f));
+    }
+    unsigned long long todo = __ballot(redo) & 0xFFFFFFFFull;
+#pragma nounroll
+    while (todo) {
+        const int r = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int ri = tile * WQ + w * 32 + r;
+        float ro[2];
+        row_again<D, F16, AX>(p, b, h, ri, __shfl(lo, r, 64), __shfl(hi, r, 64), __shfl(m, r, 64), lane, ro);
+        const float rinv = __shfl(inv, r, 64);
+        uint16_t* op = p.out + b * p.o_s[0] + h * p.o_s[1] + (long)ri * p.o_s[2];
+        if (lane < D) op[lane] = (uint16_t)pack2<F16>(ro[0] * rinv, 0.f);
+        if (D > 64) op[lane + 64] = (uint16_t)pack2<F16>(ro[1] * rinv, 0.f);
+    }
+}
+
+template <int D, bool F16, int AX>
+__global__ __launch_bounds__(256) void span_attn_narrow(const SpanArgs p) {
+    typedef Tile<D, 32> T;
+    constexpr int POS = AX * 32 * 4, STAGE = 2 * T::BYTES + POS, OS = D + 4;      // OS: row of the joined output in floats
+    extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
+    float* ml = reinterpret_cast<float*>(smem + (8 * STAGE > 4 * 32 * OS * 4 ? 8 * STAGE : 4 * 32 * OS * 4));      // [4][32][2]
+    float* os = reinterpret_cast<float*>(smem);                                                                     // [4][32][OS], over the tiles
+    const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int group = p.Hq / p.Hk, rows = group * p.nq;
+    const int rt = blockIdx.x % p.row_tiles, hk = (blockIdx.x / p.row_tiles) % p.Hk, b = blockIdx.x / p.row_tiles / p.Hk, split = blockIdx.y;
+    const int row = rt * 32 + (lane & 31);
+    const bool ok = row < rows;
+    const int h = hk * group + (ok ? row / p.nq : 0), i = ok ? row % p.nq : 0;
+    int lo = 0, hi = 0;
+    if (ok) {
+        hi = p.nk;
+        if (p.spans) {
+            const int2 sp = reinterpret_cast<const int2*>(p.spans + b * p.spans_sb)[i];
+            lo = max(sp.x, 0); hi = min(sp.y, p.nk);
+        }
+        if (lo >= hi) lo = hi = 0;
+    }
+    int k0 = hi > lo ? lo : INT32_MAX, k1 = hi;
+    for (int o = 16; o > 0; o >>= 1) { k0 = min(k0, __shfl_xor(k0, o, 64)); k1 = max(k1, __shfl_xor(k1, o, 64)); }
+    k0 = __builtin_amdgcn_readfirstlane(k0); k1 = __builtin_amdgcn_readfirstlane(k1);
+    if (k1 > k0) {      // this split's keys: whole rounds of the four waves
+        const int chunk = ((k1 - k0 + p.splits - 1) / p.splits + 127) / 128 * 128;
+        k0 = (int)min((long)k0 + (long)split * chunk, (long)k1);
+        k1 = (int)min((long)k0 + chunk, (long)k1);
+    } else k0 = k1 = 0;
+    const int nt = (k1 - k0 + 31) / 32;      // tiles of 32; this wave takes w, w + 4, ...
+
+    u32x4_t qf[D / 16];
+    {
+        const uint16_t* qp = p.q + b * p.q_s[0] + h * p.q_s[1] + (long)i * p.q_s[2] + half * 8;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) qf[c] = *reinterpret_cast<const u32x4_t*>(qp + c * 16);
+    }
+    float sl[AX ? AX : 1]; int pq[AX ? AX : 1];
+#pragma unroll
+    for (int a = 0; a < AX; ++a) {
+        sl[a] = p.slopes[h * AX + a] * SPAN_LOG2E;
+        pq[a] = p.pos_q[b * p.pq_sb + (long)i * AX + a];
+    }
+    const uint16_t* kp = p.k + b * p.k_s[0] + hk * p.k_s[1];
+    const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1];
+    const uint8_t* km = p.kmask ? p.kmask + b * p.km_sb : nullptr;
+    const int* pkp = AX ? p.pos_k + b * p.pk_sb : nullptr;
+    const bool capped = p.cap > 0.f;
+    const float c1 = capped ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E, c2 = p.cap * SPAN_LOG2E;
+    unsigned char* mine = smem + w * 2 * STAGE;
+
+    float m = SPAN_LOW, l = 0.f;
+    f32x16_t o[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[c][r] = 0.f;
+#define SPAN_ISSUE(tt_, st_)                                                                                           \
+    {                                                                                                                  \
+        const int t0_ = k0 + (tt_) * 32;                                                                               \
+        unsigned char* sp_ = mine + (st_) * STAGE;                                                                     \
+        T::template fill<1>(sp_, kp + (long)t0_ * p.k_s[2], min(32, k1 - t0_), (int)p.k_s[2], 0, lane);                \
+        T::template fill<1>(sp_ + T::BYTES, vp + (long)t0_ * p.v_s[2], min(32, k1 - t0_), (int)p.v_s[2], 0, lane);     \
+    }
+    int st = 0;
+    if (w < nt) SPAN_ISSUE(w, 0);
+    for (int tt = w; tt < nt; tt += 4, st ^= 1) {
+        const int t0 = k0 + tt * 32;
+        unsigned char* Ks = mine + st * STAGE;
+        unsigned char* Vs = Ks + T::BYTES;
+        int* pks = reinterpret_cast<int*>(Ks + 2 * T::BYTES);
+        if constexpr (AX > 0) {
+            if (lane < 32) {
+#pragma unroll
+                for (int a = 0; a < AX; ++a) pks[a * 32 + lane] = t0 + lane < k1 ? pkp[(long)(t0 + lane) * AX + a] : 0;
+            }
+        }
+        uint32_t keep = 0xFFFFFFFFu;
+        if (km) keep = (uint32_t)__ballot(lane < 32 && t0 + lane < k1 && km[t0 + lane]);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // (the wave's own tile: no barrier)
+        if (tt + 4 < nt) SPAN_ISSUE(tt + 4, st ^ 1);
+        if (keep != 0xFFFFFFFFu) T::clear_rows(Vs, keep, lane, 64);
+        __builtin_amdgcn_wave_barrier();
+        f32x16_t s[1];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) s[0] = mfma32<F16>(T::rows(Ks, c, 0, lane), qf[c], s[0]);
+        const bool masked = keep != 0xFFFFFFFFu || !__all(lo <= t0 && hi >= t0 + 32);
+        const float tmax = scores<AX, 1>(s, p.cap, c1, c2, pq, sl, pks, half, masked, masked ? bit_range(lo - t0, hi - t0) & (unsigned long long)keep : 0ull);
+        u32x4_t pf[2];
+        soften<D, F16, 1>(s, tmax, m, l, o, pf);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) o[c] = mfma32<F16>(T::cols(Vs, ks, c, lane), pf[ks], o[c]);
+    }
+#undef SPAN_ISSUE
+    // ---- join the four waves: common maximum, then the sums in wave order
+    l = both_halves_sum(l);
+    if (half == 0) { ml[(w * 32 + lane) * 2] = m; ml[(w * 32 + lane) * 2 + 1] = l; }
+    __syncthreads();      // (also: every wave is done with its tiles)
+    {
+        const int r = lane & 31;
+        const float M = fmaxf(fmaxf(ml[r * 2], ml[(32 + r) * 2]), fmaxf(ml[(64 + r) * 2], ml[(96 + r) * 2]));
+        const float f = __builtin_amdgcn_exp2f(m - M);
+        float* dst = os + (w * 32 + r) * OS + half * 4;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) *reinterpret_cast<float4*>(dst + c * 32 + g * 8) = make_float4(o[c][4 * g] * f, o[c][4 * g + 1] * f, o[c][4 * g + 2] * f, o[c][4 * g + 3] * f);
+    }
+    __syncthreads();
+    // thread t: row t >> 3 of the tile, every 8th group of 4 elements
+    const int r = t >> 3, rr = rt * 32 + r;
+    float M = SPAN_LOW, L = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) M = fmaxf(M, ml[(x * 32 + r) * 2]);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) L += ml[(x * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(x * 32 + r) * 2] - M);
+    float4 v[D / 32];
+    float bad = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+        v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const float4 y = *reinterpret_cast<const float4*>(os + (x * 32 + r) * OS + (c * 8 + (t & 7)) * 4);
+            v[c].x += y.x; v[c].y += y.y; v[c].z += y.z; v[c].w += y.w;
+        }
+        bad += (v[c].x + v[c].y + v[c].z + v[c].w) * 0.f;
+    }
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) bad += __shfl_xor(bad, x, 64);
+    const bool live = rr < rows, redo = live && bad != 0.f && L * 0.f == 0.f;
+    const int rh = hk * group + (live ? rr / p.nq : 0), ri = live ? rr % p.nq : 0;
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+    const long prow = (((long)b * p.Hk + hk) * p.row_tiles + rt) * 32 + r, prows = (long)p.B * p.Hk * p.row_tiles * 32;
+    if (live && p.splits == 1) {
+        uint16_t* op = p.out + b * p.o_s[0] + rh * p.o_s[1] + (long)ri * p.o_s[2];
+        if (!redo)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+                *reinterpret_cast<uint2*>(op + (c * 8 + (t & 7)) * 4) = make_uint2(pack2<F16>(v[c].x * inv, v[c].y * inv), pack2<F16>(v[c].z * inv, v[c].w * inv));
+        if (p.lse && (t & 7) == 0) p.lse[((long)b * p.Hq + rh) * p.nq + ri] = L > 0.f ? (M + __builtin_amdgcn_logf(L)) * SPAN_LN2 : (L == 0.f ? -INFINITY : L);
+    } else if (live) {
+        float* po = p.part_o + (split * prows + prow) * D;
+        if (!redo)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) *reinterpret_cast<float4*>(po + (c * 8 + (t & 7)) * 4) = v[c];
+        if ((t & 7) == 0) { p.part_ml[(split * prows + prow) * 2] = M; p.part_ml[(split * prows + prow) * 2 + 1] = L; }
+    }
+    unsigned long long todo = __ballot(redo && (t & 7) == 0);
+#pragma nounroll
+    while (todo) {
+        const int src = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int xr = rt * 32 + w * 8 + (src >> 3), xh = hk * group + xr / p.nq, xi = xr % p.nq;
+        int xlo = 0, xhi = p.nk;
+        if (p.spans) {
+            const int2 sp = reinterpret_cast<const int2*>(p.spans + b * p.spans_sb)[xi];
+            xlo = max(sp.x, 0); xhi = min(sp.y, p.nk);
+        }
+        float ro[2];
+        row_again<D, F16, AX>(p, b, xh, xi, max(xlo, k0), min(xhi, k1), __shfl(M, src, 64), lane, ro);
+        const float rinv = __shfl(inv, src, 64);
+        if (p.splits == 1) {
+            uint16_t* op = p.out + b * p.o_s[0] + xh * p.o_s[1] + (long)xi * p.o_s[2];
+            if (lane < D) op[lane] = (uint16_t)pack2<F16>(ro[0] * rinv, 0.f);
+            if (D > 64) op[lane + 64] = (uint16_t)pack2<F16>(ro[1] * rinv, 0.f);
+        } else {
+            float* po = p.part_o + (split * prows + (((long)b * p.Hk + hk) * p.row_tiles + rt) * 32 + w * 8 + (src >> 3)) * D;
+            if (lane < D) po[lane] = ro[0];
+            if (D > 64) po[lane + 64] = ro[1];
+        }
+    }
+}
+
+// joins the splits of a row in split order: D / 4 threads a row
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void span_attn_join(const SpanArgs p) {
+    constexpr int TPR = D / 4;
+    const long rows = (long)p.B * p.Hk * p.row_tiles * 32;
+    const long r = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int c = threadIdx.x % TPR;
+    if (r >= rows) return;
+    const int group = p.Hq / p.Hk;
+    const int in_head = (int)(r % (p.row_tiles * 32));
+    if (in_head >= group * p.nq) return;
+    const int hk = (int)(r / (p.row_tiles * 32)) % p.Hk, b = (int)(r / (p.row_tiles * 32) / p.Hk);
+    const int h = hk * group + in_head / p.nq, i = in_head % p.nq;
+    float M = SPAN_LOW;
+    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[(s * rows + r) * 2]);
+    float L = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+        const float f = __builtin_amdgcn_exp2f(p.part_ml[(s * rows + r) * 2] - M);
+        L = __builtin_fmaf(p.part_ml[(s * rows + r) * 2 + 1], f, L);
+        const float4 y = *reinterpret_cast<const float4*>(p.part_o + (s * rows + r) * D + c * 4);
+        v.x = __builtin_fmaf(y.x, f, v.x); v.y = __builtin_fmaf(y.y, f, v.y); v.z = __builtin_fmaf(y.z, f, v.z); v.w = __builtin_fmaf(y.w, f, v.w);
+    }
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+    *reinterpret_cast<uint2*>(p.out + b * p.o_s[0] + h * p.o_s[1] + (long)i * p.o_s[2] + c * 4) =
+        make_uint2(pack2<F16>(v.x * inv, v.y * inv), pack2<F16>(v.z * inv, v.w * inv));
+    if (p.lse && c == 0) p.lse[((long)b * p.Hq + h) * p.nq + i] = L > 0.f ? (M + __builtin_amdgcn_logf(L)) * SPAN_LN2 : (L == 0.f ? -INFINITY : L);
+}
+
+struct SpanPlan { bool narrow; int row_tiles, splits; };
+
+// The narrow form where the wide grid would leave CUs without a workgroup (< 256 of them).  There: 2 workgroups' worth of splits per CU, at least 256 keys each
+// (two tiles a wave).
+SpanPlan span_plan(const mm_span_attn* a) {
+    SpanPlan r;
+    const long wide = (long)a->batch * a->heads_q * ((a->nq + WQ - 1) / WQ);
+    const long rows = (long)(a->heads_q / a->heads_k) * a->nq;
+    r.row_tiles = (int)((rows + 31) / 32);
+    r.narrow = wide < 256;
+    const long wgs = (long)a->batch * a->heads_k * r.row_tiles;
+    long s = (512 + wgs - 1) / wgs;
+    const long most = (a->nk + 255) / 256;
+    r.splits = r.narrow ? (int)(s < 1 ? 1 : (s > most ? (most < 1 ? 1 : most) : s)) : 1;
+    return r;
+}
+
+template <int D, bool F16, int AX>
+int launch_fwd(hipStream_t s, const SpanArgs& a, const SpanPlan& pl) {
+    hipError_t e;
+    if (!pl.narrow) {
+        constexpr int sm = 2 * (2 * Tile<D, KT>::BYTES + AX * KT * 4) + 64;
+        e = hipFuncSetAttribute(reinterpret_cast<const void*>(span_attn_wide<D, F16, AX>), hipFuncAttributeMaxDynamicSharedMemorySize, sm);
+        if (e != hipSuccess) return mm_set_hip_error(e, "span_attn_wide LDS");
+        const int tiles = (a.nq + WQ - 1) / WQ;
+        const long total = (long)a.B * a.Hq * tiles, per = (total + 7) / 8;
+        hipLaunchKernelGGL((span_attn_wide<D, F16, AX>), dim3((unsigned)(per * 8)), dim3(256), sm, s, a);
+        return mm_check_launch("span_attn_wide");
+    }
+    constexpr int st = 8 * (2 * Tile<D, 32>::BYTES + AX * 32 * 4), jo = 4 * 32 * (D + 4) * 4;
+    constexpr int sm = (st > jo ? st : jo) + 4 * 32 * 2 * 4;
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(span_attn_narrow<D, F16, AX>), hipFuncAttributeMaxDynamicSharedMemorySize, sm);
+    if (e != hipSuccess) return mm_set_hip_error(e, "span_attn_narrow LDS");
+    hipLaunchKernelGGL((span_attn_narrow<D, F16, AX>), dim3((unsigned)(a.B * a.Hk * pl.row_tiles), pl.splits), dim3(256), sm, s, a);
+    int rc = mm_check_launch("span_attn_narrow");
+    if (rc || pl.splits == 1) return rc;
+    const long rows = (long)a.B * a.Hk * pl.row_tiles * 32, blocks = (rows + 256 / (D / 4) - 1) / (256 / (D / 4));
+    hipLaunchKernelGGL((span_attn_join<D, F16>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    return mm_check_launch("span_attn_join");
+}
+
+template <int D, bool F16>
+int launch_axes(hipStream_t s, const SpanArgs& a, const SpanPlan& pl) {
+    switch (a.axes) {
+        case 0: return launch_fwd<D, F16, 0>(s, a, pl);
+        case 1: return launch_fwd<D, F16, 1>(s, a, pl);
+        case 2: return launch_fwd<D, F16, 2>(s, a, pl);
+        default: return launch_fwd<D, F16, 3>(s, a, pl);
+    }
+}
+
+}  // namespace
+
+void span_args(const mm_span_attn* a, SpanArgs& p) {
+    memset(&p, 0, sizeof(p));
+    p.q = (const uint16_t*)a->q; p.k = (const uint16_t*)a->k; p.v = (const uint16_t*)a->v; p.out = (uint16_t*)a->out; p.lse = a->lse;
+    p.spans = a->spans; p.spans_sb = a->spans_sb; p.kmask = a->key_mask; p.km_sb = a->key_mask_sb;
+    p.slopes = a->slopes; p.pos_q = a->positions_q; p.pq_sb = a->positions_q_sb; p.pos_k = a->positions_k; p.pk_sb = a->positions_k_sb;
+    for (int i = 0; i < 3; ++i) {
+        p.q_s[i] = a->q_stride[i]; p.k_s[i] = a->k_stride[i]; p.v_s[i] = a->v_stride[i]; p.o_s[i] = a->out_stride[i];
+        p.do_s[i] = a->dout_stride[i]; p.dq_s[i] = a->dq_stride[i]; p.dk_s[i] = a->dk_stride[i]; p.dv_s[i] = a->dv_stride[i];
+    }
+    if (a->nk == 1) p.k_s[2] = p.v_s[2] = a->dim;      // (one key: its stride says nothing)
+    p.B = a->batch; p.Hq = a->heads_q; p.Hk = a->heads_k; p.nq = a->nq; p.nk = a->nk; p.axes = a->slopes ? a->axes : 0;
+    p.scale = a->scale; p.cap = a->softcap;
+    p.dout = (const uint16_t*)a->dout; p.dq = (uint16_t*)a->dq; p.dk = (uint16_t*)a->dk; p.dv = (uint16_t*)a->dv;
+}
+
+size_t k_span_attn_workspace_bytes(const mm_span_attn* a) {
+    const SpanPlan pl = span_plan(a);
+    if (pl.splits == 1) return 0;
+    return (size_t)pl.splits * a->batch * a->heads_k * pl.row_tiles * 32 * (a->dim + 2) * sizeof(float);
+}
+
+int k_span_attn(hipStream_t s, const mm_span_attn* a, void* ws) {
+    SpanArgs p;
+    span_args(a, p);
+    const SpanPlan pl = span_plan(a);
+    p.splits = pl.splits; p.row_tiles = pl.row_tiles;
+    p.part_o = (float*)ws;
+    p.part_ml = p.part_o ? p.part_o + (size_t)pl.splits * a->batch * a->heads_k * pl.row_tiles * 32 * a->dim : nullptr;
+    const bool f16 = a->dtype == MM_DT_F16;
+    if (a->dim == 32) return f16 ? launch_axes<32, true>(s, p, pl) : launch_axes<32, false>(s, p, pl);
+    if (a->dim == 64) return f16 ? launch_axes<64, true>(s, p, pl) : launch_axes<64, false>(s, p, pl);
+    return f16 ? launch_axes<128, true>(s, p, pl) : launch_axes<128, false>(s, p, pl);
+}

@@ -245,6 +245,18 @@ int k_gemm_tn_splits(int rows, int N, int K);
 bool k_gemm_tn_prefer(int rows, int N, int K, long lda, long ldb);      // the training step's rule: this kernel instead of transposed copies + the NT GEMM
 int k_gemm_tn(hipStream_t s, const bf16_t* A, long lda, const bf16_t* B, long ldb, int rows, int N, int K, int splits, float* out_or_slabs);
 
+// rotary.hip: key spans of packed rows, rotary positions over several axes
+int k_attention_spans(hipStream_t s, const int32_t* cu_q, long q_sb, const int32_t* cu_k, long k_sb, const int32_t* prefix, long p_sb, int B, int docs, int n, int j,
+                      int causal, int32_t* out);
+long k_rotary_parts(const mm_rotary* r);
+int k_rotary(hipStream_t s, const mm_rotary* r, bool bwd, float* ws, float* dscales);
+
+// attention_spans.hip / attention_spans_bwd.hip: attention of packed rows (spans, score cap, distance bias)
+size_t k_span_attn_workspace_bytes(const mm_span_attn* a);
+int k_span_attn(hipStream_t s, const mm_span_attn* a, void* ws);
+size_t k_span_attn_bwd_workspace_bytes(const mm_span_attn* a);
+int k_span_attn_bwd(hipStream_t s, const mm_span_attn* a, void* ws);
+
 // train.hip / attention_bwd.hip: backward operators
 int k_transpose_bf16(hipStream_t s, const bf16_t* in, long rows, long cols, long ldi, bf16_t* out, long ldo, int zero_pad64 = 0);   // zero_pad64: also write zeros up to rows rounded to 64 (needs ldo >= that)
 int k_colsum(hipStream_t s, const float* part, int nparts, long D, float* out);

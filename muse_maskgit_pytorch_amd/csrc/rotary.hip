@@ -1,0 +1,334 @@
+// Positions and masks of packed rows (documents = images of several sizes, with or without their text, one behind another):
+//   attention_spans : per query row the interval [lo, hi) of keys it sees, from document bounds, causal order and prefix lengths
+//   rotary_axes     : rotary positions over up to four axes (time / height / width ...), with or without l2norm * scale in front (mmp.py:151-153), and the gradient
+#include <string.h>
+
+#include "common.h"
+#include "muse_hip_internal.h"
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------ spans
+// Row i belongs to the last document with cu_q[doc] <= i (empty documents are passed over); rows in front of the first or behind the last document see nothing.
+// One thread per row, the bounds in LDS (a binary search is log2(docs) DEPENDENT reads: 64 cycles each there, an L2 round trip each from memory).  Bounded by
+// latency: 310 rows and 131000 rows take about the same time.
+constexpr int SPAN_LDS_DOCS = 4096;
+
+__global__ __launch_bounds__(256) void attention_spans_kernel(const int32_t* __restrict__ cu_q, long q_sb, const int32_t* __restrict__ cu_k, long k_sb,
+                                                              const int32_t* __restrict__ prefix, long p_sb, int docs, int n, int j, int causal, int2* __restrict__ out) {
+    __shared__ int32_t cu[SPAN_LDS_DOCS + 1];
+    const int b = blockIdx.y;
+    const int32_t* cq = cu_q + b * q_sb;
+    const int32_t* ck = cu_k + b * k_sb;
+    const bool in_lds = docs <= SPAN_LDS_DOCS;
+    if (in_lds) {
+        for (int t = threadIdx.x; t <= docs; t += 256) cu[t] = cq[t];
+        __syncthreads();
+    }
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    int a = 0, e = docs + 1;      // number of bounds <= i
+    while (a < e) {
+        const int m = (a + e) >> 1;
+        const int v = in_lds ? cu[m] : cq[m];
+        if (v <= i) a = m + 1;
+        else e = m;
+    }
+    int2 r = make_int2(0, 0);
+    const int doc = a - 1;
+    if (doc >= 0 && doc < docs) {
+        const int q0 = cq[doc], q1 = cq[doc + 1];
+        const int k0 = min(max(ck[doc], 0), j), k1 = min(max(ck[doc + 1], k0), j);
+        const int lk = k1 - k0;
+        int seen = lk;
+        if (causal) {
+            seen = i - q0 + 1 + lk - (q1 - q0);      // the last row of a document sees all of its keys
+            if (prefix) seen = max(seen, prefix[b * p_sb + doc]);
+            seen = min(max(seen, 0), lk);
+        }
+        r = make_int2(k0, k0 + seen);
+    }
+    out[(long)b * n + i] = r;
+}
+
+// ------------------------------------------------------------------------------------------------ rotary positions
+// Pair p of a head (p < P = sum of the sections) belongs to axis a(p) and turns by the angle  pos_a * freq_p:   a' = a cos - b sin,  b' = a sin + b cos,  with
+// (a, b) = elements (p, P + p), or (2p, 2p + 1) interleaved; elements from 2P on pass.  The gradient turns back.  The angle is formed in 64 bits and reduced to one
+// turn there (far positions: an fp32 product is 0.03 rad off at position 10^6), then sin / cos in fp32.
+// HBM-bound: one read + one write of every element (the backward with the norm reads two).  A token's angles serve all of its heads: a group of G lanes owns a
+// token, lane u of it VEC pairs, and walks over the heads of q and of k.  With few tokens the heads are split over blockIdx.y instead (angles computed again there).
+struct RotT {      // one of q / k
+    const void* x; long x_sb, x_sh, x_sn;      // forward: the input; backward: the forward's input (NORM only)
+    const void* dy; long d_sb, d_sh, d_sn;     // backward: the gradient of the output
+    void* out;                                 // [B][n][H][d] contiguous
+    const float* scale;                        // fp32 [d]
+    int H;
+};
+struct RotArgs {
+    RotT t[2];
+    const int32_t* pos; long pos_sb; int A;
+    const double* freq;
+    int P, c1, c2, c3;                         // axis of pair p = (p >= c1) + (p >= c2) + (p >= c3)
+    int B, n, d, G, interleaved, heads_per_block;
+    float* part;                               // backward with the norm: [gridDim.x * gridDim.y][2][d]
+};
+
+template <typename T> __device__ __forceinline__ float rot_ld(T v);
+template <> __device__ __forceinline__ float rot_ld<float>(float v) { return v; }
+template <> __device__ __forceinline__ float rot_ld<_Float16>(_Float16 v) { return (float)v; }
+template <> __device__ __forceinline__ float rot_ld<__bf16>(__bf16 v) { return (float)v; }
+
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC > 16 ? 16 : sizeof(T) * VEC) RotVec { T v[VEC]; };
+
+template <typename T, int VEC>
+__device__ __forceinline__ void rot_load(const T* p, float (&f)[VEC]) {
+    const RotVec<T, VEC> r = *reinterpret_cast<const RotVec<T, VEC>*>(p);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = rot_ld<T>(r.v[e]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void rot_store(T* p, const float (&f)[VEC]) {
+    RotVec<T, VEC> r;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r.v[e] = (T)f[e];
+    *reinterpret_cast<RotVec<T, VEC>*>(p) = r;
+}
+
+template <int VEC>
+__device__ __forceinline__ void rot_turn(float (&a)[VEC], float (&b)[VEC], const float (&c)[VEC], const float (&s)[VEC], bool interleaved) {
+    if (!interleaved || VEC == 1) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float x = a[e], y = b[e];
+            a[e] = __builtin_fmaf(x, c[e], -(y * s[e]));
+            b[e] = __builtin_fmaf(x, s[e], y * c[e]);
+        }
+    } else {      // the unit's 2 VEC consecutive elements hold its VEC pairs: (a0 a1) (a2 a3) .. (b0 b1) ..
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            float& x_ = 2 * e < VEC ? a[(2 * e) % VEC] : b[(2 * e) % VEC];
+            float& y_ = 2 * e < VEC ? a[(2 * e + 1) % VEC] : b[(2 * e + 1) % VEC];
+            const float x = x_, y = y_;
+            x_ = __builtin_fmaf(x, c[e], -(y * s[e]));
+            y_ = __builtin_fmaf(x, s[e], y * c[e]);
+        }
+    }
+}
+
+__device__ __forceinline__ float rot_group_sum(float v, int G) {
+    for (int o = G >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+template <typename T, int VEC, bool NORM, bool BWD>
+__global__ __launch_bounds__(256) void rotary_kernel(const RotArgs p) {
+    const int G = p.G, u = threadIdx.x & (G - 1), slots = 256 / G, slot = threadIdx.x / G;
+    const int U = p.d / (2 * VEC);
+    const bool live = u < U;
+    const bool inter = p.interleaved != 0;
+    int offa, offb;
+    if (inter) { offa = 2 * VEC * u; offb = offa + VEC; }
+    else if (u * VEC < p.P) { offa = u * VEC; offb = p.P + u * VEC; }
+    else { offa = 2 * p.P + 2 * (u * VEC - p.P); offb = offa + VEC; }
+    const int h_all = p.t[0].H + p.t[1].H;
+    const int h0 = blockIdx.y * p.heads_per_block, h1 = min(h0 + p.heads_per_block, h_all);
+    const long tokens = (long)p.B * p.n;
+    float acc[2][2][VEC];      // backward with the norm: gradient of the scale, [q / k][a / b]
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[w][0][e] = acc[w][1][e] = 0.f;
+
+    for (long tok0 = (long)blockIdx.x * slots; tok0 < tokens; tok0 += (long)gridDim.x * slots) {
+        const long tok = tok0 + slot;
+        const bool ok = tok < tokens && live;
+        const int b = ok ? (int)(tok / p.n) : 0, i = ok ? (int)(tok % p.n) : 0;
+        float c[VEC], s[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int pr = u * VEC + e;
+            c[e] = 1.f; s[e] = 0.f;
+            if (ok && pr < p.P) {
+                const int ax = (pr >= p.c1) + (pr >= p.c2) + (pr >= p.c3);
+                const double turns = (double)p.pos[b * p.pos_sb + (long)i * p.A + ax] * p.freq[pr] * 0.15915494309189533577;      // / (2 pi)
+                const float half_turns = (float)(2.0 * (turns - rint(turns)));
+                sincospif(half_turns, &s[e], &c[e]);
+                if (BWD) s[e] = -s[e];
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {      // q, then k
+            const RotT& t = p.t[w];
+            const int f = w ? p.t[0].H : 0;
+            const int a0 = max(h0 - f, 0), a1 = min(h1 - f, t.H);
+            float sa[VEC], sb[VEC];
+            if constexpr (NORM) {
+                if (a0 < a1) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) { sa[e] = live ? t.scale[offa + e] : 0.f; sb[e] = live ? t.scale[offb + e] : 0.f; }
+                }
+            }
+            for (int h = a0; h < a1; ++h) {
+                float xa[VEC], xb[VEC], ga[VEC], gb[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) xa[e] = xb[e] = ga[e] = gb[e] = 0.f;
+                if (ok) {
+                    if constexpr (!BWD || NORM) {
+                        const T* xp = reinterpret_cast<const T*>(t.x) + b * t.x_sb + (long)h * t.x_sh + (long)i * t.x_sn;
+                        rot_load<T, VEC>(xp + offa, xa); rot_load<T, VEC>(xp + offb, xb);
+                    }
+                    if constexpr (BWD) {
+                        const T* dp = reinterpret_cast<const T*>(t.dy) + b * t.d_sb + (long)h * t.d_sh + (long)i * t.d_sn;
+                        rot_load<T, VEC>(dp + offa, ga); rot_load<T, VEC>(dp + offb, gb);
+                    }
+                }
+                float inv = 1.f;
+                if constexpr (NORM) {
+                    float ss = 0.f;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) ss = __builtin_fmaf(xa[e], xa[e], __builtin_fmaf(xb[e], xb[e], ss));
+                    ss = rot_group_sum(ss, G);
+                    inv = 1.f / fmaxf(sqrtf(ss), 1e-12f);      // F.normalize eps (mmp.py:41-42)
+                }
+                if constexpr (!BWD) {
+                    if constexpr (NORM) {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) { xa[e] = xa[e] * inv * sa[e]; xb[e] = xb[e] * inv * sb[e]; }
+                    }
+                    rot_turn<VEC>(xa, xb, c, s, inter);
+                } else {
+                    rot_turn<VEC>(ga, gb, c, s, inter);
+                    if constexpr (NORM) {
+                        float dot = 0.f;
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            xa[e] *= inv; xb[e] *= inv;
+                            acc[w][0][e] = __builtin_fmaf(ga[e], xa[e], acc[w][0][e]);
+                            acc[w][1][e] = __builtin_fmaf(gb[e], xb[e], acc[w][1][e]);
+                            ga[e] *= sa[e]; gb[e] *= sb[e];
+                            dot = __builtin_fmaf(xa[e], ga[e], __builtin_fmaf(xb[e], gb[e], dot));
+                        }
+                        dot = rot_group_sum(dot, G);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) { xa[e] = __builtin_fmaf(-xa[e], dot, ga[e]) * inv; xb[e] = __builtin_fmaf(-xb[e], dot, gb[e]) * inv; }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) { xa[e] = ga[e]; xb[e] = gb[e]; }
+                    }
+                }
+                if (ok) {
+                    T* op = reinterpret_cast<T*>(t.out) + (tok * t.H + h) * p.d;
+                    rot_store<T, VEC>(op + offa, xa); rot_store<T, VEC>(op + offb, xb);
+                }
+            }
+        }
+    }
+    if constexpr (NORM && BWD) {      // the workgroup's part of the scales' gradients: its token slots added in slot order
+        extern __shared__ float sm[];      // [slots][2][d]
+        if (live) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    sm[(slot * 2 + w) * p.d + offa + e] = acc[w][0][e];
+                    sm[(slot * 2 + w) * p.d + offb + e] = acc[w][1][e];
+                }
+        }
+        __syncthreads();
+        float* part = p.part + (long)(blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.d;
+        for (int col = threadIdx.x; col < 2 * p.d; col += 256) {
+            float v = 0.f;
+            for (int sl = 0; sl < slots; ++sl) v += sm[sl * 2 * p.d + col];
+            part[col] = v;
+        }
+    }
+}
+
+struct RotPlan { int vec, G, gx, gy, hpb; };
+
+// VEC = 8 where rows and pairs allow 16-byte accesses, else one pair per lane.  Workgroups: every token slot once, up to 2048 (8 per CU; more only lengthen the
+// scales' reduction); with fewer than 512 of them the heads are split until the card has work (a step of a decoder: 32 tokens).
+RotPlan rot_plan(int B, int n, int H, int d, int vec) {
+    RotPlan r;
+    r.vec = vec;
+    int g = 1;
+    while (g < d / (2 * vec)) g *= 2;
+    r.G = g;
+    const long blocks = ((long)B * n + 256 / g - 1) / (256 / g);
+    r.gx = (int)(blocks < 2048 ? blocks : 2048);
+    int split = 1;
+    while ((long)r.gx * split * 2 <= 512 && split * 2 <= H) split *= 2;
+    r.hpb = (H + split - 1) / split;
+    r.gy = (H + r.hpb - 1) / r.hpb;
+    return r;
+}
+
+template <typename T, int VEC>
+void rot_launch(hipStream_t s, const RotArgs& a, const RotPlan& pl, bool norm, bool bwd) {
+    const dim3 g(pl.gx, pl.gy), blk(256);
+    const size_t sm = norm && bwd ? (size_t)(256 / pl.G) * 2 * a.d * sizeof(float) : 0;
+    if (norm && bwd) hipLaunchKernelGGL((rotary_kernel<T, VEC, true, true>), g, blk, sm, s, a);
+    else if (bwd) hipLaunchKernelGGL((rotary_kernel<T, VEC, false, true>), g, blk, 0, s, a);
+    else if (norm) hipLaunchKernelGGL((rotary_kernel<T, VEC, true, false>), g, blk, 0, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, VEC, false, false>), g, blk, 0, s, a);
+}
+
+bool rot_wide(const mm_rotary* r) {
+    int P = 0;
+    for (int a = 0; a < r->axes; ++a) P += r->sections[a];
+    const int per16 = r->dtype == MM_DT_F32 ? 4 : 8;
+    if (r->dim % 16 || (!r->interleaved && (P % 8 || (r->dim - 2 * P) % 16))) return false;
+    for (int w = 0; w < 2; ++w) {
+        const mm_rotary_side* t = w ? &r->k : &r->q;
+        if (t->heads == 0) continue;
+        if (((uintptr_t)t->x | (uintptr_t)t->dy | (uintptr_t)t->out) & 15) return false;
+        for (int i = 0; i < 3; ++i)
+            if ((t->x && t->x_stride[i] % per16) || (t->dy && t->dy_stride[i] % per16)) return false;
+    }
+    return true;
+}
+
+}  // namespace
+
+int k_attention_spans(hipStream_t s, const int32_t* cu_q, long q_sb, const int32_t* cu_k, long k_sb, const int32_t* prefix, long p_sb, int B, int docs, int n, int j,
+                      int causal, int32_t* out) {
+    if (B == 0 || n == 0) return MM_OK;
+    hipLaunchKernelGGL(attention_spans_kernel, dim3((n + 255) / 256, B), dim3(256), 0, s, cu_q, q_sb, cu_k, k_sb, prefix, p_sb, docs, n, j, causal, reinterpret_cast<int2*>(out));
+    return mm_check_launch("attention_spans_kernel");
+}
+
+// rows [2 dim] of the scales' partial gradients; -1: a head too long for one pair per lane (64 lanes) whose rows do not allow 16-byte accesses
+long k_rotary_parts(const mm_rotary* r) {
+    if (r->dim > 128 && !rot_wide(r)) return -1;
+    const RotPlan pl = rot_plan(r->batch, r->n, r->q.heads + r->k.heads, r->dim, rot_wide(r) ? 8 : 1);
+    return (long)pl.gx * pl.gy;
+}
+
+int k_rotary(hipStream_t s, const mm_rotary* r, bool bwd, float* ws, float* dscales) {
+    RotArgs a;
+    memset(&a, 0, sizeof(a));
+    for (int w = 0; w < 2; ++w) {
+        const mm_rotary_side* t = w ? &r->k : &r->q;
+        a.t[w].x = t->x; a.t[w].x_sb = t->x_stride[0]; a.t[w].x_sh = t->x_stride[1]; a.t[w].x_sn = t->x_stride[2];
+        a.t[w].dy = t->dy; a.t[w].d_sb = t->dy_stride[0]; a.t[w].d_sh = t->dy_stride[1]; a.t[w].d_sn = t->dy_stride[2];
+        a.t[w].out = t->out; a.t[w].scale = t->scale; a.t[w].H = t->heads;
+    }
+    a.pos = r->positions; a.pos_sb = r->pos_sb; a.A = r->axes; a.freq = r->freqs;
+    int cum[4] = {0, 0, 0, 0}, P = 0;
+    for (int i = 0; i < r->axes; ++i) { P += r->sections[i]; cum[i] = P; }
+    for (int i = r->axes; i < 4; ++i) cum[i] = P;
+    a.P = P; a.c1 = cum[0]; a.c2 = cum[1]; a.c3 = cum[2];
+    a.B = r->batch; a.n = r->n; a.d = r->dim; a.interleaved = r->interleaved;
+    const bool wide = rot_wide(r);
+    const RotPlan pl = rot_plan(r->batch, r->n, r->q.heads + r->k.heads, r->dim, wide ? 8 : 1);
+    a.G = pl.G; a.heads_per_block = pl.hpb; a.part = ws;
+    const bool norm = r->normalize != 0;
+    if (pl.gx > 0 && pl.gy > 0) {
+        if (r->dtype == MM_DT_F32) { if (wide) rot_launch<float, 8>(s, a, pl, norm, bwd); else rot_launch<float, 1>(s, a, pl, norm, bwd); }
+        else if (r->dtype == MM_DT_F16) { if (wide) rot_launch<_Float16, 8>(s, a, pl, norm, bwd); else rot_launch<_Float16, 1>(s, a, pl, norm, bwd); }
+        else { if (wide) rot_launch<__bf16, 8>(s, a, pl, norm, bwd); else rot_launch<__bf16, 1>(s, a, pl, norm, bwd); }
+        const int rc = mm_check_launch("rotary_kernel");
+        if (rc) return rc;
+    }
+    return norm && bwd ? k_colsum(s, ws, pl.gx * pl.gy, 2 * r->dim, dscales) : MM_OK;      // (no rows: zeros)
+}

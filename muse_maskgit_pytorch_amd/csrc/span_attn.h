@@ -1,0 +1,153 @@
+// Shared by the forward and the backward of the packed-row attention (attention_spans.hip, attention_spans_bwd.hip): arguments, tiles in LDS, masks, scores.
+#pragma once
+#include "common.h"
+#include "muse_hip_internal.h"
+
+struct SpanArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t* out;
+    float* lse;
+    const int32_t* spans; long spans_sb;
+    const uint8_t* kmask; long km_sb;
+    const float* slopes;
+    const int32_t *pos_q, *pos_k; long pq_sb, pk_sb;
+    long q_s[3], k_s[3], v_s[3], o_s[3];
+    int B, Hq, Hk, nq, nk, axes;
+    float scale, cap;
+    // forward, keys split over workgroups
+    int splits, row_tiles; float* part_o; float* part_ml;
+    // backward
+    const uint16_t* dout; long do_s[3];
+    uint16_t *dq, *dk, *dv; long dq_s[3], dk_s[3], dv_s[3];
+    float* delta; float* dsl_part; int2* hulls; int hull_tiles;
+};
+
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short sp_v4i16_t __attribute__((ext_vector_type(4)));
+
+constexpr float SPAN_LOG2E = 1.4426950408889634f, SPAN_LN2 = 0.6931471805599453f;
+constexpr float SPAN_LOW = -1.0e30f;      // start of a running maximum: finite, so that a masked score (-inf) minus it is -inf, not NaN
+
+// v_mfma_f32_32x32x16: A lane l holds row l & 31, contraction 8 (l >> 5) .. + 7; B the same with columns; C lane l holds column l & 31, rows 8 (r >> 2) + 4 (l >> 5)
+// + (r & 3).  A C fragment's registers 8 s .. 8 s + 7 are therefore a B operand over 16 of its rows, in the order (slot j of half h) = row 16 s + 8 (j >> 2) + 4 h +
+// (j & 3) -- the order in which two transposing LDS reads deliver the other operand.  No value crosses lanes between the two products.
+template <bool F16>
+__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+    if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (F16) return (uint32_t)f32_to_f16_bits(a) | ((uint32_t)f32_to_f16_bits(b) << 16);
+    else return pack_bf16x2(a, b);
+}
+template <bool F16> __device__ __forceinline__ float to_f32(uint16_t v) {
+    if constexpr (F16) return f16_bits_to_f32(v);
+    else return bf16_to_f32(v);
+}
+template <bool F16> __device__ __forceinline__ u32x4_t pack_slots(const f32x16_t& c, int s) {      // (s: a constant after unrolling)
+    return u32x4_t{pack2<F16>(c[8 * s], c[8 * s + 1]), pack2<F16>(c[8 * s + 2], c[8 * s + 3]), pack2<F16>(c[8 * s + 4], c[8 * s + 5]), pack2<F16>(c[8 * s + 6], c[8 * s + 7])};
+}
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+__device__ __forceinline__ float both_halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// A tile of ROWS rows x D elements in LDS as [D / 16][ROWS][16] (32-byte rows; 128 bytes between blocks keep the two column blocks of a transposing read on
+// different banks).  ONE image serves both operand forms: rows as they are (ds_read_b128: the wave reads 1 KiB in a row) and transposed (ds_read_b64_tr_b16).  Filled
+// by LDS-DMA, 32 rows x 16 columns per wave instruction; rows at or behind rows_ok are outside the descriptor and come as zeros.
+template <int D, int ROWS>
+struct Tile {
+    static constexpr int NB = D / 16, BS = ROWS * 32 + 128, BYTES = NB * BS;
+    template <int NW>      // waves that share the work, this one being w
+    static __device__ __forceinline__ void fill(unsigned char* lds, const uint16_t* base, int rows_ok, int stride, int w, int lane) {
+        typedef __attribute__((address_space(3))) void* lds_ptr_t;
+        const int sb = stride * 2;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, rows_ok > 0 ? (unsigned)((rows_ok - 1) * sb + D * 2) : 0u, 0x00020000);
+        const int v0 = (lane >> 1) * sb + (lane & 1) * 16;
+#pragma unroll
+        for (int i = 0; i < NB * (ROWS / 32) / NW; ++i) {
+            const int idx = i * NW + w, cb = idx % NB, rb = idx / NB;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(lds + cb * BS + rb * 1024), 16, v0 + rb * 32 * sb + cb * 32, 0, 0, 0);
+        }
+    }
+    // operand over columns 16 cb .. + 15, rows 32 rb .. + 31
+    static __device__ __forceinline__ u32x4_t rows(const unsigned char* lds, int cb, int rb, int lane) {
+        return *reinterpret_cast<const u32x4_t*>(lds + cb * BS + (rb * 32 + (lane & 31)) * 32 + (lane >> 5) * 16);
+    }
+    // operand over rows 16 s .. + 15 (in the slot order above), columns 32 cd .. + 31
+    static __device__ __forceinline__ u32x4_t cols(const unsigned char* lds, int s, int cd, int lane) {
+        typedef __attribute__((address_space(3))) sp_v4i16_t* lds_v4_t;
+        const unsigned char* p = lds + (2 * cd + ((lane >> 4) & 1)) * BS + (s * 16 + (lane >> 5) * 4 + ((lane & 15) >> 2)) * 32 + (lane & 3) * 8;
+        const sp_v4i16_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4_t)p), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4_t)(p + 256));
+        const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+        return u32x4_t{x.x, x.y, y.x, y.y};
+    }
+    // rows whose bit is clear become zeros (all threads of the workgroup; the caller's barriers)
+    static __device__ __forceinline__ void clear_rows(unsigned char* lds, unsigned long long keep, int t, int threads) {
+        for (int c = t; c < NB * ROWS * 2; c += threads) {
+            const int row = (c >> 1) % ROWS;
+            if (!((keep >> row) & 1ull)) *reinterpret_cast<u32x4_t*>(lds + (c / (2 * ROWS)) * BS + row * 32 + (c & 1) * 16) = u32x4_t{0, 0, 0, 0};
+        }
+    }
+};
+
+// bits a .. e - 1 of 64, both clamped
+__device__ __forceinline__ unsigned long long bit_range(int a, int e) {
+    a = max(a, 0); e = min(e, 64);
+    return e > a ? (~0ull >> (64 - (e - a))) << a : 0ull;
+}
+
+// s in units of log2: cap(scale q.k) * log2 e.  cap tanh(x / cap) = cap (1 - 2 / (exp(2 x / cap) + 1)): one exp2 and one reciprocal; the absolute error is an fp32
+// rounding of cap.  c1 = scale * log2 e without a cap, 2 * scale * log2 e / cap with one; c2 = cap * log2 e.
+__device__ __forceinline__ float span_tanh(float x, float c1) {
+    return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f), 1.f);
+}
+
+template <int AX>
+__device__ __forceinline__ float span_bias(const int (&pq)[AX ? AX : 1], const float (&sl)[AX ? AX : 1], const int* pk) {      // sum of slope (in log2 units) * distance
+    float v = 0.f;
+#pragma unroll
+    for (int a = 0; a < AX; ++a) v = __builtin_fmaf(sl[a], fabsf((float)(pq[a] - pk[a])), v);
+    return v;
+}
+
+// dot product of two rows by one lane
+template <int D, bool F16>
+__device__ __forceinline__ float row_dot(const uint16_t* x, const uint16_t* y) {
+    float s = 0.f;
+#pragma nounroll
+    for (int c = 0; c < D; c += 8) {
+        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(x + c), b = *reinterpret_cast<const u32x4_t*>(y + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            s = __builtin_fmaf(to_f32<F16>((uint16_t)a[e]), to_f32<F16>((uint16_t)b[e]), s);
+            s = __builtin_fmaf(to_f32<F16>((uint16_t)(a[e] >> 16)), to_f32<F16>((uint16_t)(b[e] >> 16)), s);
+        }
+    }
+    return s;
+}
+
+// score (log2 units) of one visible pair by one lane; *slope: derivative of the cap
+template <int D, bool F16, int AX>
+__device__ __forceinline__ float pair_score(const SpanArgs& p, const uint16_t* q, const uint16_t* k, int b, int h, int i, int key, float* slope) {
+    float x = row_dot<D, F16>(q, k);
+    *slope = 1.f;
+    if (p.cap > 0.f) {
+        const float t = span_tanh(x, 2.f * p.scale * SPAN_LOG2E / p.cap);
+        *slope = 1.f - t * t;
+        x = t * (p.cap * SPAN_LOG2E);
+    } else x *= p.scale * SPAN_LOG2E;
+#pragma unroll
+    for (int a = 0; a < AX; ++a)
+        x -= p.slopes[h * AX + a] * SPAN_LOG2E * fabsf((float)(p.pos_q[b * p.pq_sb + (long)i * AX + a] - p.pos_k[b * p.pk_sb + (long)key * AX + a]));
+    return x;
+}
+
+}  // namespace

@@ -1,0 +1,302 @@
+"""The packed-row operators on the GPU against their plain forms in 64 bits (tests/packed_rows.py): spans of documents, rotary positions, attention with spans, capped
+scores and a distance bias, their gradients."""
+import math
+import random
+
+import pytest
+import torch
+
+import packed_rows as R
+from muse_maskgit_pytorch_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+DT = dict(bf16=torch.bfloat16, fp16=torch.float16, fp32=torch.float32)
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def bounds(rng, docs, total):
+    cuts = sorted(rng.randint(0, total) for _ in range(docs))
+    return torch.tensor([0] + cuts, dtype=torch.int32)
+
+
+# ------------------------------------------------------------------------------------------------ spans
+@pytest.mark.parametrize('docs,n', [(0, 5), (1, 1), (1, 256), (3, 310), (40, 257), (5000, 9000)])
+@pytest.mark.parametrize('mode', ['all', 'causal', 'prefix', 'cross', 'cross_prefix'])
+def test_spans(docs, n, mode):
+    rng = random.Random(docs * 7 + n)
+    cu_q = bounds(rng, docs, max(0, n - 3))
+    cross = mode.startswith('cross')
+    j = n // 2 + 1 if cross else n
+    cu_k = bounds(rng, docs, j) if cross else None
+    prefix = torch.tensor([rng.randint(0, 50) for _ in range(docs)], dtype=torch.int32) if 'prefix' in mode else None
+    causal = mode in ('causal', 'prefix', 'cross_prefix')
+    got = ops.attention_spans(cu_q.to(DEV), n, cu_k=cu_k.to(DEV) if cross else None, j=j, prefix=prefix.to(DEV) if prefix is not None else None, causal=causal)
+    assert got.dtype == torch.int32 and torch.equal(got.cpu(), R.spans_of(cu_q, cu_k if cross else cu_q, prefix, n, causal))
+
+
+def test_spans_of_a_batch_and_of_bounds_that_do_not_start_at_zero():
+    cu = torch.tensor([[0, 3, 3, 10], [2, 4, 9, 12]], dtype=torch.int32)
+    got = ops.attention_spans(cu.to(DEV), 14, causal=True)
+    assert got.shape == (2, 14, 2)
+    for x in range(2):
+        assert torch.equal(got[x].cpu(), R.spans_of(cu[x], cu[x], None, 14, True))
+    # strided tables; bounds behind the keys are cut off
+    wide = torch.zeros(4, 6, dtype=torch.int32)
+    wide[:, ::2][:, :3] = torch.tensor([0, 4, 20], dtype=torch.int32)
+    got = ops.attention_spans(wide.to(DEV)[0, ::2], 8, cu_k=wide.to(DEV)[1, ::2], j=10)
+    assert got.cpu().tolist() == [[0, 4]] * 4 + [[4, 10]] * 4
+
+
+# ------------------------------------------------------------------------------------------------ rotary
+ROT = [  # b, n, hq, hk, d, sections, interleaved
+    (1, 1, 1, 1, 32, [16], False), (2, 37, 8, 8, 64, [16, 16], False), (3, 65, 4, 1, 128, [8, 20, 20], False), (2, 19, 6, 2, 64, [8, 8, 8], True),
+    (1, 300, 8, 2, 128, [64], True), (2, 33, 3, 3, 20, [3, 2], False), (1, 9, 2, 1, 24, [1, 2, 3, 4], True), (1, 70, 2, 2, 256, [32, 32, 64], False),
+    (1, 17, 2, 2, 256, [1, 2, 7], True), (2, 5, 1, 5, 128, [5, 7], False), (1, 4, 2, 2, 2, [1], False), (1, 130, 40, 40, 64, [32], False), (1, 6, 2, 1, 64, [0, 0], False)]
+
+
+def rot_inputs(b, n, hq, hk, d, sections, dtype, seed, far=3000):
+    g = gen(seed)
+    rows = torch.randn(b, n, hq + 2 * hk, d, generator=g).to(DT[dtype])
+    q, k = rows[:, :, :hq].transpose(1, 2), rows[:, :, hq:hq + hk].transpose(1, 2)
+    pos = torch.randint(-far, far + 1, (b, n, len(sections)), generator=g).to(torch.int32)
+    freqs = torch.cat([1000.0 ** (-torch.arange(s, dtype=torch.float64) / max(1, s)) for s in sections])
+    return rows, q, k, pos, freqs, 1 + 0.3 * torch.randn(d, generator=g), 1 + 0.3 * torch.randn(d, generator=g), g
+
+
+def rot_tol(want, mag, half):
+    """one rounding of the result; before it a few fp32 roundings of terms of the size of the pair (`mag`)"""
+    return half * 1.02 * want.abs() + 24 * R.F32 * mag + (2.0 ** -24 if half == R.HALF[torch.float16] else 1e-30)
+
+
+def pair_size(x, sections, interleaved):
+    """largest magnitude of a pair (of the element itself behind the pairs)"""
+    P = sum(sections)
+    y = x.abs().clone()
+    for p in range(P):
+        a, b = (2 * p, 2 * p + 1) if interleaved else (p, P + p)
+        m = torch.maximum(x[..., a].abs(), x[..., b].abs())
+        y[..., a] = y[..., b] = m
+    return y
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('norm', [False, True])
+@pytest.mark.parametrize('shape', ROT)
+def test_rotary(shape, norm, dtype):
+    b, n, hq, hk, d, sections, inter = shape
+    rows, q, k, pos, freqs, qs, ks, _ = rot_inputs(*shape[:6], dtype, 11)
+    dev_rows = rows.to(DEV)
+    dq_, dk_ = dev_rows[:, :, :hq].transpose(1, 2), dev_rows[:, :, hq:hq + hk].transpose(1, 2)
+    got = ops.rotary_axes(dq_, dk_, pos.to(DEV), freqs.to(DEV), sections, *((qs.to(DEV), ks.to(DEV)) if norm else ()), interleaved=inter)
+    for x, s, y, name in ((q, qs, got[0], 'q'), (k, ks, got[1], 'k')):
+        assert y.dtype == x.dtype and y.shape == x.shape
+        want = R.rotary(x, pos, freqs, sections, s if norm else None, inter)
+        z = x.double()
+        if norm:
+            z = z / z.norm(dim=-1, keepdim=True) * s.double()
+        R.check(y, want, rot_tol(want, pair_size(z, sections, inter) * (d / 8 if norm else 1), R.HALF[x.dtype]), name)
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('norm', [False, True])
+@pytest.mark.parametrize('shape', ROT)
+def test_rotary_bwd(shape, norm, dtype):
+    b, n, hq, hk, d, sections, inter = shape
+    rows, q, k, pos, freqs, qs, ks, g = rot_inputs(*shape[:6], dtype, 12)
+    dq = torch.randn(b, n, hq, d, generator=g).to(DT[dtype]).transpose(1, 2)
+    dk = torch.randn(b, hk, n, d, generator=g).to(DT[dtype])
+    args = dict(q=q.to(DEV), k=k.to(DEV), q_scale=qs.to(DEV), k_scale=ks.to(DEV)) if norm else {}
+    got = ops.rotary_axes_bwd(dq.to(DEV), dk.to(DEV), pos.to(DEV), freqs.to(DEV), sections, interleaved=inter, **args)
+    again = ops.rotary_axes_bwd(dq.to(DEV), dk.to(DEV), pos.to(DEV), freqs.to(DEV), sections, interleaved=inter, **args)
+    for x, s, dy, dx, ds, name in ((q, qs, dq, got[0], got[2], 'q'), (k, ks, dk, got[1], got[3], 'k')):
+        gr = R.turn(dy.double(), pos, freqs, sections, inter, back=True)
+        half, size = R.HALF[x.dtype], pair_size(dy.double(), sections, inter)
+        if not norm:
+            assert ds is None
+            R.check(dx, gr, rot_tol(gr, size, half), name)
+            continue
+        x, s = x.double(), s.double()
+        ln = x.norm(dim=-1, keepdim=True)
+        xh, gs = x / ln, gr * s
+        want = (gs - xh * (xh * gs).sum(-1, keepdim=True)) / ln
+        mag = (size * s.abs() + xh.abs() * (xh.abs() * size * s.abs()).sum(-1, keepdim=True)) / ln
+        R.check(dx, want, rot_tol(want, mag * d / 8, half), name)
+        R.check(ds, (gr * xh).sum((0, 1, 2)), (R.F32 * (24 + d + 2 * math.sqrt(b * n * hq))) * (size * xh.abs()).sum((0, 1, 2)), name + ' scale')
+    for x, y in zip(got, again):
+        assert x is None and y is None or torch.equal(x, y)
+
+
+def test_rotary_far_positions_keep_their_angle():
+    n, d = 64, 64
+    pos = (2 ** 30 - 1 - 977 * torch.arange(n)).to(torch.int32)[:, None]
+    freqs = 10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32)
+    x = torch.randn(1, 2, n, d, generator=gen(3))
+    got, none = ops.rotary_axes(x.to(DEV), None, pos.to(DEV), freqs.to(DEV), [32])
+    assert none is None
+    want = R.rotary(x, pos[None], freqs, [32])
+    # the product of position and frequency in 64 bits: 2^30 * 2^-53 radians
+    R.check(got, want, rot_tol(want, pair_size(x.double(), [32], False), R.HALF[torch.float32]) + 2.0 ** -22 * pair_size(x.double(), [32], False), 'far')
+
+
+def test_rotary_gradient_against_differences():
+    b, n, h, d, sections = 1, 3, 2, 16, [3, 4]
+    _, q, _, pos, freqs, qs, _, g = rot_inputs(b, n, h, 1, d, sections, 'fp32', 5)
+    q = q.contiguous()
+    w = torch.randn(b, h, n, d, generator=g)
+    dq, _, ds, _ = ops.rotary_axes_bwd(w.to(DEV), None, pos.to(DEV), freqs.to(DEV), sections, q=q.to(DEV), q_scale=qs.to(DEV))
+    f = lambda x, s: float((R.rotary(x, pos, freqs, sections, s) * w.double()).sum())
+    q, qs, eps = q.double(), qs.double(), 1e-6
+    for idx in [(0, 0, 0, 0), (0, 1, 2, 7), (0, 0, 1, 15), (0, 1, 0, 9)]:
+        e = torch.zeros_like(q)
+        e[idx] = eps
+        assert abs((f(q + e, qs) - f(q - e, qs)) / (2 * eps) - float(dq[idx])) < 2e-5
+    for c in (0, 8, 15):
+        e = torch.zeros_like(qs)
+        e[c] = eps
+        assert abs((f(q, qs + e) - f(q, qs - e)) / (2 * eps) - float(ds[c])) < 2e-5
+
+
+def test_rotary_of_nothing_and_of_a_zero_row():
+    freqs = torch.ones(16, dtype=torch.float64, device=DEV)
+    z = torch.zeros(1, 2, 0, 32, device=DEV, dtype=torch.bfloat16)
+    p0 = torch.zeros(0, 1, dtype=torch.int32, device=DEV)
+    assert ops.rotary_axes(z, z, p0, freqs, [16])[0].shape == z.shape
+    s = torch.ones(32, device=DEV)
+    _, _, ds, dks = ops.rotary_axes_bwd(z, z, p0, freqs, [16], q=z, k=z, q_scale=s, k_scale=s)
+    assert ds.tolist() == [0.0] * 32 and dks.tolist() == [0.0] * 32
+    x = torch.zeros(1, 1, 1, 32, device=DEV)
+    y, _ = ops.rotary_axes(x, None, torch.zeros(1, 1, dtype=torch.int32, device=DEV), freqs, [16], q_scale=s)
+    assert torch.equal(y, x)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def att_inputs(b, hq, hk, n, j, d, dtype, mask, cap, axes, seed, unit=None):
+    """operands on the CPU, spans, key mask, positions; the key rows are views of wider rows, as a projection leaves them"""
+    g, rng = gen(seed), random.Random(seed)
+    t = DT[dtype]
+    unit = cap == 0.0 if unit is None else unit
+    q = torch.randn(b, n, hq, d, generator=g)
+    kv = torch.randn(b, j, 2 * hk, d, generator=g)
+    if unit:
+        q = q / q.norm(dim=-1, keepdim=True)
+        kv[:, :, :hk] /= kv[:, :, :hk].norm(dim=-1, keepdim=True).clamp(min=1e-3)
+    scale = 8.0 if unit else 2.0 * d ** -0.5
+    spans = key_mask = None
+    if mask in ('docs', 'prefix', 'causal', 'cross'):
+        docs = max(1, n // 40)
+        cu = bounds(rng, docs, n - n // 20)
+        cu_k = cu if n == j else bounds(rng, docs, j)
+        prefix = torch.tensor([rng.randint(0, 30) for _ in range(docs)], dtype=torch.int32) if mask == 'prefix' else None
+        spans = R.spans_of(cu, cu_k, prefix, n, mask in ('prefix', 'causal'))
+    elif mask == 'any':          # per row of the batch, in no order, empty and out of range ones among them
+        lo = torch.randint(-5, j + 5, (b, n), generator=g)
+        spans = torch.stack([lo, lo + torch.randint(-3, max(2, j), (b, n), generator=g)], 2).to(torch.int32)
+    elif mask == 'keys':
+        key_mask = torch.rand(b, j, generator=g) < 0.6
+        key_mask[0] = False
+    elif mask == 'both':
+        key_mask = torch.rand(b, j, generator=g) < 0.7
+        lo = torch.randint(0, max(1, j // 2), (n,), generator=g)
+        spans = torch.stack([lo, lo + torch.randint(0, j // 2 + 1, (n,), generator=g)], 1).to(torch.int32)
+    slopes = pos_q = pos_k = None
+    if axes:
+        slopes = 0.02 + 0.2 * torch.rand(hq, axes, generator=g)
+        shape = (b, n, axes) if mask == 'any' else (n, axes)
+        pos_q = torch.randint(0, 40, shape, generator=g).to(torch.int32)
+        pos_k = torch.randint(0, 40, (j, axes), generator=g).to(torch.int32)
+    return dict(q=q.to(t).transpose(1, 2), kv=kv.to(t), scale=scale, cap=cap, spans=spans, key_mask=key_mask, slopes=slopes, pos_q=pos_q, pos_k=pos_k, hk=hk)
+
+
+def on_gpu(x):
+    mv = lambda t: None if t is None else t.to(DEV)
+    kv = x['kv'].to(DEV)
+    return (x['q'].to(DEV), kv[:, :, :x['hk']].transpose(1, 2), kv[:, :, x['hk']:].transpose(1, 2), mv(x['spans'])), \
+        dict(scale=x['scale'], softcap=x['cap'], slopes=mv(x['slopes']), positions=mv(x['pos_q']), key_positions=mv(x['pos_k']), key_mask=mv(x['key_mask']))
+
+
+def plain(x, **more):
+    b, _, n, _ = x['q'].shape
+    k, v = x['kv'][:, :, :x['hk']].transpose(1, 2), x['kv'][:, :, x['hk']:].transpose(1, 2)
+    seen = R.visible(n, k.shape[2], x['spans'], x['key_mask'], b)
+    return R.attention(x['q'], k, v, seen, x['scale'], x['cap'], x['slopes'], x['pos_q'], x['pos_k'], **more)
+
+
+ATT = [  # b, hq, hk, n, j, d, dtype, mask, cap, axes        -- few rows (keys split over waves and workgroups)
+    (1, 1, 1, 1, 1, 64, 'bf16', 'none', 0.0, 0), (2, 8, 2, 1, 2000, 128, 'fp16', 'none', 30.0, 0), (3, 4, 4, 1, 700, 64, 'bf16', 'any', 0.0, 1),
+    (1, 8, 8, 256, 256, 64, 'bf16', 'none', 0.0, 2), (1, 8, 8, 33, 65, 32, 'bf16', 'none', 0.0, 0), (2, 6, 3, 5, 999, 32, 'fp16', 'keys', 0.0, 3),
+    (1, 16, 1, 3, 4097, 128, 'bf16', 'both', 20.0, 1), (2, 2, 1, 129, 31, 64, 'fp16', 'any', 0.0, 0), (1, 4, 2, 300, 300, 128, 'bf16', 'prefix', 30.0, 2),
+    (1, 2, 2, 200, 90, 64, 'bf16', 'cross', 0.0, 0), (1, 3, 1, 64, 0, 64, 'bf16', 'none', 0.0, 0), (4, 12, 4, 2, 128, 64, 'bf16', 'keys', 50.0, 0),
+    # many rows (128 queries a workgroup)
+    (8, 16, 4, 200, 200, 32, 'bf16', 'docs', 0.0, 0), (8, 16, 16, 130, 257, 64, 'bf16', 'none', 0.0, 0), (4, 16, 8, 400, 400, 64, 'bf16', 'docs', 0.0, 2),
+    (2, 16, 4, 1000, 1000, 128, 'bf16', 'prefix', 30.0, 0), (8, 16, 2, 256, 191, 64, 'fp16', 'any', 0.0, 1), (4, 32, 32, 256, 64, 128, 'fp16', 'keys', 0.0, 3),
+    (4, 16, 16, 512, 63, 32, 'bf16', 'both', 10.0, 3), (2, 64, 1, 250, 250, 64, 'bf16', 'causal', 0.0, 1), (4, 32, 4, 129, 1, 128, 'bf16', 'none', 0.0, 0),
+    (16, 16, 16, 129, 0, 32, 'fp16', 'none', 0.0, 0)]
+
+
+@pytest.mark.parametrize('case', ATT, ids=lambda c: '-'.join(map(str, c)))
+def test_attend_spans(case):
+    x = att_inputs(*case, seed=21)
+    args, kw = on_gpu(x)
+    out, lse = ops.attend_spans(*args, **kw, return_lse=True)
+    want = plain(x)
+    R.check(lse, want['lse'], want['lse_tol'], 'lse')
+    R.check(out, want['out'], want['out_tol'], 'out')
+    rows = ops.attend_spans(*args, **kw, out_rows=True)
+    b, hq, n, d = out.shape
+    assert torch.equal(rows, out.permute(0, 2, 1, 3).reshape(b * n, hq * d))
+
+
+@pytest.mark.parametrize('case', [(1, 2, 1, 300, 300, 64, 'bf16', 'docs', 0.0, 0), (8, 16, 16, 200, 200, 64, 'bf16', 'docs', 0.0, 2), (8, 16, 4, 200, 200, 128, 'fp16', 'both', 30.0, 0),
+                                  (2, 8, 2, 1, 3000, 128, 'fp16', 'any', 0.0, 1), (2, 4, 4, 40, 200, 32, 'bf16', 'both', 0.0, 0)], ids=lambda c: '-'.join(map(str, c)))
+@pytest.mark.parametrize('where', ['sevenths', 'second half'])
+@pytest.mark.parametrize('value', [math.nan, math.inf])
+def test_attend_spans_what_is_hidden_stays_out(case, value, where):
+    """infinities and NaN in keys and values that a row does not see, rows of other documents and rows behind the last document among them, never reach it"""
+    x = att_inputs(*case, seed=22)
+    b, _, n, _ = x['q'].shape
+    j = x['kv'].shape[1]
+    seen = R.visible(n, j, x['spans'], x['key_mask'], b)
+    want = plain(x)
+    broken = ~seen.any(1)                                # keys that nothing sees, and every seventh, or all that the first half of the rows does not see
+    if where == 'second half' or n == 1:                 # (a single long row sees some of the sevenths)
+        broken = ~seen[:, :(n + 1) // 2].any(1)
+    else:
+        broken[:, ::7] = True
+    x['kv'][broken] = value
+    args, kw = on_gpu(x)
+    out, lse = ops.attend_spans(*args, **kw, return_lse=True)
+    clean = ~(seen & broken[:, None]).any(-1)            # rows that see no broken key
+    assert clean.any()
+    c = clean[:, None].expand(lse.shape)
+    R.check(lse.cpu()[c], want['lse'][c], want['lse_tol'][c], 'lse')
+    R.check(out.cpu()[c], want['out'][c], want['out_tol'][c], 'out')
+    rest = ~c
+    if rest.any():
+        assert not out.cpu()[rest].isfinite().all(-1).any()
+
+
+def test_attend_spans_sees_through_strides_and_expanded_operands():
+    """keys shared by a batch (batch stride 0), token-major and head-major operands, a slice of a longer cache"""
+    g = gen(9)
+    cache = torch.randn(2, 4, 500, 64, generator=g).to(torch.bfloat16).to(DEV)
+    q = torch.randn(3, 8, 70, 64, generator=g).to(torch.bfloat16).to(DEV)
+    k, v = cache[0, :, 17:317].expand(3, 4, 300, 64), cache[1, :, 17:317].expand(3, 4, 300, 64)
+    a = ops.attend_spans(q, k, v, scale=0.125)
+    b = ops.attend_spans(q.contiguous(), k.contiguous(), v.contiguous(), scale=0.125)
+    assert torch.equal(a, b)
+
+
+def test_attend_spans_wide_and_narrow_agree_and_repeat():
+    """the same rows alone (keys split) and among many (128 queries a workgroup): within two roundings of P and of the result, and each the same bits every time"""
+    x = att_inputs(16, 16, 16, 150, 150, 64, 'bf16', 'docs', 0.0, 2, seed=31)
+    args, kw = on_gpu(x)
+    many = ops.attend_spans(*args, **kw)
+    assert torch.equal(many, ops.attend_spans(*args, **kw))
+    one = ops.attend_spans(args[0][:1], args[1][:1], args[2][:1], args[3], **kw)
+    assert torch.equal(one, ops.attend_spans(args[0][:1], args[1][:1], args[2][:1], args[3], **kw))
+    want = plain(x)
+    R.check(one - many[:1].float(), torch.zeros_like(want['out'][:1]), 2 * want['out_tol'][:1], 'difference')
