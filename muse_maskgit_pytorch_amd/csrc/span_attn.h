@@ -19,7 +19,7 @@ struct SpanArgs {
     // backward
     const uint16_t* dout; long do_s[3];
     uint16_t *dq, *dk, *dv; long dq_s[3], dk_s[3], dv_s[3];
-    float* delta; float* dsl_part; int2* hulls; int hull_tiles;
+    float* delta; float* dsl_part; int4* hulls; int hull_tiles;
 };
 
 namespace {

@@ -1070,3 +1070,34 @@ def attend_spans(q, k, v, spans=None, scale=8.0, softcap=0.0, slopes=None, posit
     if out_rows:
         out = out.permute(0, 2, 1, 3).reshape(b * n, hq * d)
     return (out, lse) if return_lse else out
+
+
+def attend_spans_bwd(q, k, v, out, lse, dout, spans=None, scale=8.0, softcap=0.0, slopes=None, positions=None, key_positions=None, key_mask=None):
+    """Gradients of attend_spans (bf16) from its inputs, its out (b, hq, n, d) and lse, and dout, the gradient of out: (dq, dk, dv, dslopes) -- dq (b, hq, n, d),
+    dk / dv (b, hk, j, d) as views of rows, dslopes fp32 (hq, axes) or None without slopes.  dk and dv are summed over the heads that share a key head.  Rows that
+    see nothing (lse -inf) and keys that nothing sees get and give 0, whatever they hold.  No atomics: the same bits every time."""
+    for name, t in (('out', out), ('dout', dout)):
+        _need(t.shape == q.shape and t.dtype == q.dtype, f'attend_spans_bwd: {name} {t.dtype} {tuple(t.shape)} beside q {q.dtype} {tuple(q.shape)}')
+        _need(t.stride(3) == 1 or t.numel() == 0, 'attend_spans_bwd: the elements of a head must be contiguous')
+    _need(q.dtype == torch.bfloat16, f'attend_spans_bwd: bf16, not {q.dtype}')
+    _need(lse.dtype == torch.float32 and lse.shape == q.shape[:3], f'attend_spans_bwd: lse fp32 {tuple(q.shape[:3])}')
+    desc, keep = _span_desc(q, k, v, spans, float(scale), float(softcap), slopes, positions, key_positions, key_mask, extra=(out, lse, dout))
+    b, hq, n, d = q.shape
+    hk, j = k.shape[1], k.shape[2]
+    lse = lse.contiguous()
+    dq, dk, dv = _heads_view(b, n, hq, d, q), _heads_view(b, j, hk, d, q), _heads_view(b, j, hk, d, q)
+    for name, t in (('out', out), ('dout', dout), ('dq', dq), ('dk', dk), ('dv', dv)):
+        setattr(desc, name, L.ptr(t))
+        setattr(desc, name + '_stride', _heads_st(t))
+    desc.lse = L.ptr(lse)
+    dslopes = None
+    if slopes is not None:
+        dslopes = torch.empty(slopes.shape, dtype=torch.float32, device=q.device)
+        desc.dslopes = L.ptr(dslopes)
+        if b * n == 0:
+            dslopes.zero_()
+    lib = L.lib()
+    nbytes = lib.mm_span_attention_bwd_workspace_bytes(L.C.byref(desc))
+    ws = _span_ws(nbytes, q)
+    L.check(lib.mm_span_attention_bwd(L.stream(), L.C.byref(desc), L.ptr(ws), nbytes), 'mm_span_attention_bwd')
+    return dq, dk, dv, dslopes

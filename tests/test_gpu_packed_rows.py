@@ -300,3 +300,195 @@ def test_attend_spans_wide_and_narrow_agree_and_repeat():
     assert torch.equal(one, ops.attend_spans(args[0][:1], args[1][:1], args[2][:1], args[3], **kw))
     want = plain(x)
     R.check(one - many[:1].float(), torch.zeros_like(want['out'][:1]), 2 * want['out_tol'][:1], 'difference')
+
+
+BWD = [c for c in ATT if c[6] == 'bf16'] + [(2, 4, 1, 700, 130, 128, 'bf16', 'any', 20.0, 1), (1, 2, 2, 17000, 40, 32, 'bf16', 'none', 0.0, 1), (1, 3, 3, 60, 700, 64, 'bf16', 'both', 0.0, 3),
+                                            (2, 8, 2, 257, 257, 128, 'bf16', 'docs', 0.0, 3)]
+
+
+def bwd_inputs(case, seed):
+    x = att_inputs(*case, seed=seed)
+    f = plain(x)
+    dt = DT[case[6]]
+    out, lse = f['out'].to(dt), f['lse'].float()
+    dout = torch.randn(out.shape, generator=gen(seed + 1)).to(dt)
+    return x, out, lse, dout
+
+
+@pytest.mark.parametrize('case', BWD, ids=lambda c: '-'.join(map(str, c)))
+def test_attend_spans_bwd(case):
+    x, out, lse, dout = bwd_inputs(case, 41)
+    args, kw = on_gpu(x)
+    # gradients arrive as a projection's rows: (b, n, h, d)
+    rows = dout.transpose(1, 2).contiguous().to(DEV).transpose(1, 2)
+    got = ops.attend_spans_bwd(*args[:3], out.to(DEV), lse.to(DEV), rows, args[3], **kw)
+    want = plain(x, dout=dout, out=out, lse=lse)
+    for name, t in zip(('dq', 'dk', 'dv', 'dslopes'), got):
+        if name == 'dslopes' and x['slopes'] is None:
+            assert t is None
+            continue
+        R.check(t, want[name], want[name + '_tol'], name)
+    again = ops.attend_spans_bwd(*args[:3], out.to(DEV), lse.to(DEV), rows, args[3], **kw)
+    for a, c in zip(got, again):
+        assert a is None or torch.equal(a, c)
+
+
+@pytest.mark.parametrize('case', [(1, 2, 1, 300, 300, 64, 'bf16', 'docs', 0.0, 0), (2, 4, 2, 200, 200, 128, 'bf16', 'both', 30.0, 1), (2, 2, 2, 150, 90, 32, 'bf16', 'any', 0.0, 0)],
+                         ids=lambda c: '-'.join(map(str, c)))
+@pytest.mark.parametrize('value', [math.nan, math.inf])
+def test_attend_spans_bwd_what_is_hidden_stays_out(case, value):
+    """broken keys and broken gradient rows: queries that see no broken key and keys that no broken row sees have the gradients of a clean batch"""
+    x, out, lse, dout = bwd_inputs(case, 42)
+    b, _, n, _ = x['q'].shape
+    j = x['kv'].shape[1]
+    seen = R.visible(n, j, x['spans'], x['key_mask'], b)
+    want = plain(x, dout=dout, out=out, lse=lse)
+    keys = ~seen[:, :n // 2].any(1)                          # keys that the first half of the rows does not see
+    x['kv'][keys] = value
+    rows = ~seen.any(-1)                                     # rows that see nothing, and a few of the second half
+    rows[:, n // 2 + 3::17] = True
+    dout.transpose(1, 2)[rows] = value
+    x['q'].transpose(1, 2)[~seen.any(-1)] = value
+    out.transpose(1, 2)[~seen.any(-1)] = value
+    args, kw = on_gpu(x)
+    dq, dk, dv, ds = ops.attend_spans_bwd(*args[:3], out.to(DEV), lse.to(DEV), dout.to(DEV), args[3], **kw)
+    cq = ~(seen & keys[:, None]).any(-1) & (~rows | ~seen.any(-1))
+    ck = ~(seen & rows[:, :, None]).any(1) & ~(keys & seen.any(1))
+    assert cq.any() and ck.any()
+    cq, ck = cq[:, None].expand(dq.shape[:3]), ck[:, None].expand(dk.shape[:3])
+    R.check(dq.cpu()[cq], want['dq'][cq], want['dq_tol'][cq], 'dq')
+    R.check(dk.cpu()[ck], want['dk'][ck], want['dk_tol'][ck], 'dk')
+    R.check(dv.cpu()[ck], want['dv'][ck], want['dv_tol'][ck], 'dv')
+
+
+def test_attend_spans_gradients_against_differences():
+    """scale 1, two heads over one key head, capped, biased: the kernel's gradients against central differences of the 64-bit forward along random directions"""
+    case = (1, 2, 1, 24, 24, 32, 'bf16', 'causal', 5.0, 2)
+    x = att_inputs(*case, seed=51)
+    f = plain(x)
+    out, lse = f['out'].to(torch.bfloat16), f['lse'].float()
+    g = gen(52)
+    dout = torch.randn(out.shape, generator=g).to(torch.bfloat16)
+    args, kw = on_gpu(x)
+    got = ops.attend_spans_bwd(*args[:3], out.to(DEV), lse.to(DEV), dout.to(DEV), args[3], **kw)
+    seen = R.visible(24, 24, x['spans'])
+    q, k, v, s = x['q'].double(), x['kv'][:, :, :1].transpose(1, 2).double(), x['kv'][:, :, 1:].transpose(1, 2).double(), x['slopes'].double()
+
+    def value(q, k, v, s):
+        t = q @ k.transpose(2, 3) * x['scale']
+        t = 5.0 * torch.tanh(t / 5.0)
+        t = t - torch.einsum('ha,nja->hnj', s, (x['pos_q'][:, None] - x['pos_k'][None]).abs().double())
+        p = torch.softmax(t.masked_fill(~seen[:, None], -1e300), -1) * seen[:, None]
+        return float(((p @ v) * dout.double()).sum())
+    eps = 1e-6
+    for n, t in enumerate((q, k, v, s)):
+        e = torch.randn(t.shape, generator=g).double()
+        up, down = [q, k, v, s], [q, k, v, s]
+        up[n], down[n] = t + eps * e, t - eps * e
+        diff = (value(*up) - value(*down)) / (2 * eps)
+        grad = got[n].detach().cpu().double()
+        # three roundings to bf16 (out, an operand, the result) of every term
+        assert abs(float((grad * e).sum()) - diff) < 3 * 2.0 ** -8 * float((grad * e).abs().sum()) + 1e-6, ('q', 'k', 'v', 'slopes')[n]
+
+
+def test_packed_training_pass_of_all_operators_together():
+    """a layer's attention over a packed row, as a model runs it: projection rows -> l2norm, scales and positions -> attention by document with a distance bias, and
+    the way back; against the same chain in 64 bits"""
+    rng, g = random.Random(7), gen(7)
+    h, d, n = 4, 64, 331
+    sections, freqs = [16, 16], torch.cat([100.0 ** (-torch.arange(16, dtype=torch.float64) / 16)] * 2)
+    cu = torch.tensor([0, 64, 64, 180, 316], dtype=torch.int32)
+    prefix = torch.tensor([10, 0, 30, 0], dtype=torch.int32)
+    pos = torch.stack([torch.arange(n) // 16, torch.arange(n) % 16], 1).to(torch.int32)
+    rows = torch.randn(1, n, 3 * h, d, generator=g).to(torch.bfloat16)
+    qs, ks = 1 + 0.2 * torch.randn(d, generator=g), 1 + 0.2 * torch.randn(d, generator=g)
+    slopes = 0.05 + 0.1 * torch.rand(h, 2, generator=g)
+    w = torch.randn(1, n, h, d, generator=g).to(torch.bfloat16).transpose(1, 2)
+    r = rows.to(DEV)
+    q, k, v = (r[:, :, x * h:(x + 1) * h].transpose(1, 2) for x in range(3))
+    p, f, s = pos.to(DEV), freqs.to(DEV), slopes.to(DEV)
+    spans = ops.attention_spans(cu.to(DEV), n, prefix=prefix.to(DEV), causal=True)
+    qr, kr = ops.rotary_axes(q, k, p, f, sections, q_scale=qs.to(DEV), k_scale=ks.to(DEV))
+    out, lse = ops.attend_spans(qr, kr, v, spans, slopes=s, positions=p, return_lse=True)
+    dqr, dkr, dv, dsl = ops.attend_spans_bwd(qr, kr, v, out, lse, w.to(DEV), spans, slopes=s, positions=p)
+    dq, dk, dqs, dks = ops.rotary_axes_bwd(dqr, dkr, p, f, sections, q=q, k=k, q_scale=qs.to(DEV), k_scale=ks.to(DEV))
+    leaves = [t.double().requires_grad_() for t in (rows, qs, ks, slopes)]
+    x = leaves[0]
+    z = [x[:, :, a * h:(a + 1) * h].transpose(1, 2) for a in range(3)]
+    z[0], z[1] = (turn_autograd(t / t.norm(dim=-1, keepdim=True) * sc, pos, freqs) for t, sc in ((z[0], leaves[1]), (z[1], leaves[2])))
+    seen = R.visible(n, n, R.spans_of(cu, cu, prefix, n, True))
+    t = z[0] @ z[1].transpose(2, 3) * 8 - torch.einsum('ha,nja->hnj', leaves[3], (pos[:, None] - pos[None]).abs().double())
+    pr = torch.softmax(t.masked_fill(~seen[:, None], -1e300), -1) * seen[:, None]
+    o = pr @ z[2]
+    grads = torch.autograd.grad((o * w.double()).sum(), leaves)
+    # bf16 between the operators: the scores (|s| up to 8 |q_scale k_scale|) move by a few 2^-8 of themselves, everything behind them by as much in relation to its size
+    rel = lambda a, b: float((a.cpu().double() - b).norm() / b.norm())
+    bound = 8 * 2.0 ** -8
+    assert rel(out, o.detach()) < bound
+    assert rel(torch.cat([dq, dk, dv], 1).transpose(1, 2), grads[0]) < bound
+    assert rel(dqs, grads[1]) < bound and rel(dks, grads[2]) < bound and rel(dsl, grads[3]) < bound
+    assert not out[:, :, 316:].any() and not dq[:, :, 316:].any() and not dk[:, :, 316:].any() and not dv[:, :, 316:].any()
+
+
+def turn_autograd(x, pos, freqs):
+    ang = pos.double()[:, [0] * 16 + [1] * 16] * freqs
+    a, b = x[..., :32], x[..., 32:]
+    return torch.cat([a * ang.cos() - b * ang.sin(), a * ang.sin() + b * ang.cos()], -1)
+
+
+def test_packed_rows_in_a_captured_graph():
+    """the whole chain captured once and replayed over new inputs, with eager work between the replays; a second graph of the same operators beside it"""
+    g = gen(61)
+    h, d, n = 8, 64, 400
+    f, s = torch.ones(32, dtype=torch.float64, device=DEV) * 0.1, torch.rand(h, 1, generator=g).to(DEV) * 0.1
+    pos = torch.arange(n, dtype=torch.int32, device=DEV)[:, None]
+    cu = torch.tensor([0, 100, 250, 390], dtype=torch.int32, device=DEV)
+    scale = torch.ones(d, device=DEV)
+
+    def chain(rows, w):
+        q, k, v = (rows[:, :, x * h:(x + 1) * h].transpose(1, 2) for x in range(3))
+        spans = ops.attention_spans(cu, n)
+        qr, kr = ops.rotary_axes(q, k, pos, f, [32], q_scale=scale, k_scale=scale)
+        out, lse = ops.attend_spans(qr, kr, v, spans, slopes=s, positions=pos, return_lse=True)
+        one = ops.attend_spans(qr[:, :, -20:-19], kr, v, slopes=s, positions=pos[-20:-19], key_positions=pos, softcap=9.0)
+        return (out, lse, one) + ops.attend_spans_bwd(qr, kr, v, out, lse, w, spans, slopes=s, positions=pos)
+
+    new = lambda: (torch.randn(1, n, 3 * h, d, generator=g).to(torch.bfloat16).to(DEV), torch.randn(1, n, h, d, generator=g).to(torch.bfloat16).to(DEV).transpose(1, 2))
+    graphs = []
+    for _ in range(2):
+        rows, w = new()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            chain(rows, w)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            got = chain(rows, w)
+        graphs.append((gr, rows, w, got))
+    for turn in range(4):
+        for gr, rows, w, got in graphs:
+            a, b = new()
+            rows.copy_(a)
+            w.copy_(b)
+            gr.replay()
+            want = chain(a, b)
+            torch.cuda.synchronize()
+            for x, y in zip(got, want):
+                assert torch.equal(x, y), turn
+
+
+def test_packed_rows_on_a_stream_of_their_own():
+    g = gen(71)
+    x = torch.randn(2, 200, 12, 64, generator=g).to(torch.bfloat16).to(DEV)
+    q, k, v = (x[:, :, a * 4:(a + 1) * 4].transpose(1, 2) for a in range(3))
+    want, wl = ops.attend_spans(q, k, v, return_lse=True)
+    wb = ops.attend_spans_bwd(q, k, v, want, wl, q)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        out, lse = ops.attend_spans(q, k, v, return_lse=True)
+        got = ops.attend_spans_bwd(q, k, v, out, lse, q)
+    side.synchronize()
+    assert torch.equal(out, want) and torch.equal(lse, wl) and all(torch.equal(a, c) for a, c in zip(got[:3], wb[:3]))

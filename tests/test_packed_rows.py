@@ -59,6 +59,19 @@ def test_attention_refusals(match, change):
     refuses(match, ops.attend_spans, **att(**change))
 
 
+def test_attention_bwd_refusals():
+    a = att()
+    lse = torch.zeros(2, 4, 5)
+    for match, change in [('out', dict(out=a['q'][:, :2])), ('dout', dict(dout=a['q'].float())), ('lse', dict(lse=lse.double())), ('lse', dict(lse=lse[:, :2])),
+                          ('contiguous', dict(dout=torch.zeros(2, 4, 64, 5, dtype=BF).transpose(2, 3)))]:
+        refuses(match, ops.attend_spans_bwd, **{**a, **dict(out=a['q'], lse=lse, dout=a['q']), **change})
+    h = {n: t.half() for n, t in a.items()}
+    refuses('bf16, not', ops.attend_spans_bwd, **h, out=h['q'], lse=lse, dout=h['q'])
+    for match, change in ATT_REFUSALS[2:]:
+        if 'q' not in change:
+            refuses(match, ops.attend_spans_bwd, **{**a, **dict(out=a['q'], lse=lse, dout=a['q']), **change})
+
+
 def span_desc(**change):
     """a descriptor whose pointers are never followed: the C checks come first"""
     d = _lib.SpanAttn()
