@@ -78,6 +78,7 @@ class VaeDesc(C.Structure):
 MM_DT_BF16, MM_DT_F16, MM_DT_F32 = 0, 1, 2
 
 
+# (descriptors of the packed-row operators: ops.py packs them in one go, struct.Struct('=...') of the same fields)
 class RotarySide(C.Structure):
     _fields_ = [(n, c_vp) for n in ('x', 'dy', 'out', 'scale')] + [('x_stride', c_i64 * 3), ('dy_stride', c_i64 * 3), ('heads', C.c_int32), ('reserved', C.c_int32)]
 
@@ -157,13 +158,13 @@ SIGNATURES = {
     'mm_sum_parts_bf16': (c_int, [c_vp, c_vp, c_int, c_i64, c_vp]),
     'mm_attention_bwd': (c_int, [c_vp] + [c_vp, c_i64, c_i64, c_i64] * 8 + [c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_f32]),
     'mm_attention_spans': (c_int, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_int, c_int, c_int, c_int, c_int, c_vp]),
-    'mm_rotary_axes': (c_int, [c_vp, C.POINTER(Rotary)]),
-    'mm_rotary_axes_bwd_workspace_bytes': (c_sz, [C.POINTER(Rotary)]),
-    'mm_rotary_axes_bwd': (c_int, [c_vp, C.POINTER(Rotary), c_vp, c_vp, c_sz]),
-    'mm_span_attention_workspace_bytes': (c_sz, [C.POINTER(SpanAttn)]),
-    'mm_span_attention': (c_int, [c_vp, C.POINTER(SpanAttn), c_vp, c_sz]),
-    'mm_span_attention_bwd_workspace_bytes': (c_sz, [C.POINTER(SpanAttn)]),
-    'mm_span_attention_bwd': (c_int, [c_vp, C.POINTER(SpanAttn), c_vp, c_sz]),
+    'mm_rotary_axes': (c_int, [c_vp, c_vp]),
+    'mm_rotary_axes_bwd_workspace_bytes': (c_sz, [c_vp]),
+    'mm_rotary_axes_bwd': (c_int, [c_vp, c_vp, c_vp, c_vp, c_sz]),
+    'mm_span_attention_workspace_bytes': (c_sz, [c_vp]),
+    'mm_span_attention': (c_int, [c_vp, c_vp, c_vp, c_sz]),
+    'mm_span_attention_bwd_workspace_bytes': (c_sz, [c_vp]),
+    'mm_span_attention_bwd': (c_int, [c_vp, c_vp, c_vp, c_sz]),
     'mm_qk_norm_bwd_blocks': (c_i64, [c_i64]),
     'mm_qk_norm_bwd': (c_int, [c_vp, c_vp, c_i64, c_vp, c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_vp]),
     'mm_train_step_workspace_bytes': (c_sz, [C.POINTER(TrainDesc), c_int, c_int, c_int, c_int]),

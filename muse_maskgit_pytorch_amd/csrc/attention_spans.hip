@@ -267,7 +267,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
 }
 
 template <int D, bool F16, int AX>
-__global__ __launch_bounds__(256) void span_attn_narrow(const SpanArgs p) {
+__global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
     typedef Tile<D, 32> T;
     constexpr int POS = AX * 32 * 4, STAGE = 2 * T::BYTES + POS, OS = D + 4;      // OS: row of the joined output in floats
     extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
@@ -477,14 +477,14 @@ __global__ __launch_bounds__(256) void span_attn_join(const SpanArgs p) {
 
 struct SpanPlan { bool narrow; int row_tiles, splits; };
 
-// The narrow form where the wide grid would leave CUs without a workgroup (< 256 of them).  There: 2 workgroups' worth of splits per CU, at least 256 keys each
-// (two tiles a wave).
+// The narrow form where the wide one would leave CUs without a workgroup (< 256 of them) or most of a workgroup's 128 rows empty (up to 32 queries: 16 new positions
+// over caches of 16384 keys, 16 / 4 heads of 128: 505 us wide).  There: 2 workgroups' worth of splits per CU, at least 256 keys each (two tiles a wave).
 SpanPlan span_plan(const mm_span_attn* a) {
     SpanPlan r;
     const long wide = (long)a->batch * a->heads_q * ((a->nq + WQ - 1) / WQ);
     const long rows = (long)(a->heads_q / a->heads_k) * a->nq;
     r.row_tiles = (int)((rows + 31) / 32);
-    r.narrow = wide < 256;
+    r.narrow = wide < 256 || a->nq <= 32;
     const long wgs = (long)a->batch * a->heads_k * r.row_tiles;
     long s = (512 + wgs - 1) / wgs;
     const long most = (a->nk + 255) / 256;
@@ -494,11 +494,10 @@ SpanPlan span_plan(const mm_span_attn* a) {
 
 template <int D, bool F16, int AX>
 int launch_fwd(hipStream_t s, const SpanArgs& a, const SpanPlan& pl) {
-    hipError_t e;
     if (!pl.narrow) {
         constexpr int sm = 2 * (2 * Tile<D, KT>::BYTES + AX * KT * 4) + 64;
-        e = hipFuncSetAttribute(reinterpret_cast<const void*>(span_attn_wide<D, F16, AX>), hipFuncAttributeMaxDynamicSharedMemorySize, sm);
-        if (e != hipSuccess) return mm_set_hip_error(e, "span_attn_wide LDS");
+        static std::atomic<unsigned long long> lds{0};
+        if (const int rc = span_allow_lds(reinterpret_cast<const void*>(span_attn_wide<D, F16, AX>), sm, lds)) return rc;
         const int tiles = (a.nq + WQ - 1) / WQ;
         const long total = (long)a.B * a.Hq * tiles, per = (total + 7) / 8;
         hipLaunchKernelGGL((span_attn_wide<D, F16, AX>), dim3((unsigned)(per * 8)), dim3(256), sm, s, a);
@@ -506,10 +505,10 @@ int launch_fwd(hipStream_t s, const SpanArgs& a, const SpanPlan& pl) {
     }
     constexpr int st = 8 * (2 * Tile<D, 32>::BYTES + AX * 32 * 4), jo = 4 * 32 * (D + 4) * 4;
     constexpr int sm = (st > jo ? st : jo) + 4 * 32 * 2 * 4;
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(span_attn_narrow<D, F16, AX>), hipFuncAttributeMaxDynamicSharedMemorySize, sm);
-    if (e != hipSuccess) return mm_set_hip_error(e, "span_attn_narrow LDS");
+    static std::atomic<unsigned long long> lds{0};
+    if (const int rc = span_allow_lds(reinterpret_cast<const void*>(span_attn_narrow<D, F16, AX>), sm, lds)) return rc;
     hipLaunchKernelGGL((span_attn_narrow<D, F16, AX>), dim3((unsigned)(a.B * a.Hk * pl.row_tiles), pl.splits), dim3(256), sm, s, a);
-    int rc = mm_check_launch("span_attn_narrow");
+    const int rc = mm_check_launch("span_attn_narrow");
     if (rc || pl.splits == 1) return rc;
     const long rows = (long)a.B * a.Hk * pl.row_tiles * 32, blocks = (rows + 256 / (D / 4) - 1) / (256 / (D / 4));
     hipLaunchKernelGGL((span_attn_join<D, F16>), dim3((unsigned)blocks), dim3(256), 0, s, a);

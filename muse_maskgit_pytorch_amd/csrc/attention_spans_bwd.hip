@@ -517,7 +517,6 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
 
 template <int D, int AX>
 int launch_bwd(hipStream_t s, const SpanArgs& a) {
-    hipError_t e;
     int rc;
     if (a.nq > 0) {
         const long rows = (long)a.B * a.Hq * a.nq;
@@ -526,16 +525,16 @@ int launch_bwd(hipStream_t s, const SpanArgs& a) {
         hipLaunchKernelGGL(span_bwd_hulls, dim3((unsigned)(((long)a.B * a.hull_tiles + 7) / 8)), dim3(256), 0, s, a);
         if ((rc = mm_check_launch("span_bwd_hulls"))) return rc;
         constexpr int sm = 2 * (2 * Tile<D, BT>::BYTES + AX * BT * 4) + 64;
-        e = hipFuncSetAttribute(reinterpret_cast<const void*>(span_bwd_dq<D, AX>), hipFuncAttributeMaxDynamicSharedMemorySize, sm);
-        if (e != hipSuccess) return mm_set_hip_error(e, "span_bwd_dq LDS");
+        static std::atomic<unsigned long long> lds{0};
+        if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dq<D, AX>), sm, lds))) return rc;
         const long total = (long)a.B * a.Hq * ((a.nq + BQ - 1) / BQ);
         hipLaunchKernelGGL((span_bwd_dq<D, AX>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), sm, s, a);
         if ((rc = mm_check_launch("span_bwd_dq"))) return rc;
     }
     if (a.nk > 0) {
         constexpr int sm = 2 * (2 * Tile<D, BT>::BYTES + (4 + AX) * BT * 4) + 256 * 4 + 512 * 16 + 16;
-        e = hipFuncSetAttribute(reinterpret_cast<const void*>(span_bwd_dkv<D, AX>), hipFuncAttributeMaxDynamicSharedMemorySize, sm);
-        if (e != hipSuccess) return mm_set_hip_error(e, "span_bwd_dkv LDS");
+        static std::atomic<unsigned long long> lds{0};
+        if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dkv<D, AX>), sm, lds))) return rc;
         const long total = (long)a.B * a.Hk * ((a.nk + BK - 1) / BK);
         hipLaunchKernelGGL((span_bwd_dkv<D, AX>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), sm, s, a);
         if ((rc = mm_check_launch("span_bwd_dkv"))) return rc;

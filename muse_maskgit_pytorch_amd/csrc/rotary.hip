@@ -282,8 +282,9 @@ bool rot_wide(const mm_rotary* r) {
         const mm_rotary_side* t = w ? &r->k : &r->q;
         if (t->heads == 0) continue;
         if (((uintptr_t)t->x | (uintptr_t)t->dy | (uintptr_t)t->out) & 15) return false;
+        const int size[3] = {r->batch, t->heads, r->n};      // (a dimension of one element has no stride)
         for (int i = 0; i < 3; ++i)
-            if ((t->x && t->x_stride[i] % per16) || (t->dy && t->dy_stride[i] % per16)) return false;
+            if (size[i] > 1 && ((t->x && t->x_stride[i] % per16) || (t->dy && t->dy_stride[i] % per16))) return false;
     }
     return true;
 }

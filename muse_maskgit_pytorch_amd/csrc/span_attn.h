@@ -1,5 +1,7 @@
 // Shared by the forward and the backward of the packed-row attention (attention_spans.hip, attention_spans_bwd.hip): arguments, tiles in LDS, masks, scores.
 #pragma once
+#include <atomic>
+
 #include "common.h"
 #include "muse_hip_internal.h"
 
@@ -148,6 +150,17 @@ __device__ __forceinline__ float pair_score(const SpanArgs& p, const uint16_t* q
     for (int a = 0; a < AX; ++a)
         x -= p.slopes[h * AX + a] * SPAN_LOG2E * fabsf((float)(p.pos_q[b * p.pq_sb + (long)i * AX + a] - p.pos_k[b * p.pk_sb + (long)key * AX + a]));
     return x;
+}
+
+// more than 64 KiB of dynamic LDS has to be allowed once per kernel and device (`done`: a bit per device)
+inline int span_allow_lds(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && (dev > 63 || !((done.load() >> dev) & 1ull))) {
+        e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == hipSuccess && dev < 64) done.fetch_or(1ull << dev);
+    }
+    return e == hipSuccess ? MM_OK : mm_set_hip_error(e, "span attention LDS");
 }
 
 }  // namespace

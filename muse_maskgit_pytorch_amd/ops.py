@@ -1,6 +1,7 @@
 """Tensor-level wrappers over the C ABI (include/muse_hip.h).  torch supplies device memory and the stream only;
 every computation below happens inside libmuse_hip.so.  All tensors must live on the current gfx950 device."""
 import math
+import struct
 
 import torch
 
@@ -845,37 +846,44 @@ def cfg_mix(emb_cond, emb_null, cond_scale, D, products=None):
 
 
 # ------------------------------------------------------------------------------------------------ packed rows: spans, rotary positions, attention
+# These calls are short (a few microseconds of GPU time for a small batch), so their host side is kept lean: one plain test per rule, the descriptor packed in one go
+# (mm_rotary / mm_span_attn: no padding between their fields), the stream handle without a Stream object.
 _DT = {torch.bfloat16: L.MM_DT_BF16, torch.float16: L.MM_DT_F16, torch.float32: L.MM_DT_F32}
+_ROTARY = struct.Struct('=10q2i10q2i3q12i')
+_SPAN = struct.Struct('=26q8i2f17q')
+_Err = L.MuseHipError
 
 
-def _need(ok, msg):
-    if not ok:
-        raise L.MuseHipError(msg)
-
-
-def _same_device(first, *ts):
-    """every tensor on the device of `first`, which is the current one (the library launches on the current device's stream)"""
+def _one_device(first, *ts):
+    """every tensor on the device of `first`, which is the current one; returns that device's current stream"""
+    dev = first.get_device()
     for t in ts:
-        _need(t is None or t.device == first.device, f'tensors on {first.device} and {t.device if t is not None else None}')
-    _chk_cuda(first)
-    _need(first.device.index == torch.cuda.current_device(), f'tensors on {first.device}, but the current device is cuda:{torch.cuda.current_device()}')
+        if t is not None and t.get_device() != dev:
+            raise _Err(f'tensors on {first.device} and {t.device}')
+    if dev < 0 or not L._device_ok:
+        _chk_cuda(first)
+    if dev != torch._C._cuda_getDevice():
+        raise _Err(f'tensors on {first.device}, but the current device is cuda:{torch.cuda.current_device()}')
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _heads_st(t):
-    """(batch, head, token) strides; a dimension of one element has none (torch leaves any value there)"""
-    return tuple(0 if t.shape[i] == 1 else t.stride(i) for i in range(3))
-
-
-def _heads_view(b, n, h, d, like):
+def _rows_out(b, n, h, d, like):
     """(b, h, n, d) view of fresh [b, n, h, d] rows (heads merged per token, as the projections and mmp.py:161 have them)"""
-    return torch.empty(b, n, h, d, dtype=like.dtype, device=like.device).permute(0, 2, 1, 3)
+    return torch.empty_strided((b, h, n, d), (n * h * d, d, h * d, 1), dtype=like.dtype, device=like.device)
 
 
 def _per_row(t, name, b, n, width):
     """int32 [n, width] or [b, n, width] -> (contiguous tensor, batch stride)"""
-    _need(t.dtype == torch.int32, f'{name}: int32, not {t.dtype}')
-    _need(tuple(t.shape) in ((n, width), (b, n, width)), f'{name}: shape {tuple(t.shape)}, not ({n}, {width}) or ({b}, {n}, {width})')
-    return t.contiguous(), (n * width if t.dim() == 3 else 0)
+    s = t.shape
+    if t.dtype != torch.int32:
+        raise _Err(f'{name}: int32, not {t.dtype}')
+    if s != (n, width) and s != (b, n, width):
+        raise _Err(f'{name}: shape {tuple(s)}, not ({n}, {width}) or ({b}, {n}, {width})')
+    return t.contiguous(), (n * width if len(s) == 3 else 0)
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def attention_spans(cu_q, n, cu_k=None, j=None, prefix=None, causal=False):
@@ -884,89 +892,103 @@ def attention_spans(cu_q, n, cu_k=None, j=None, prefix=None, causal=False):
     queries and lk keys sees the first i + 1 + lk - lq keys, and at least the first prefix[doc] (int32 [docs], needs causal).  [b, docs + 1] tables
     (and [b, docs] prefixes) give [b, n, 2].  Rows of no document see nothing: (0, 0).  What the bounds hold is not checked (they are on the GPU):
     they must not decrease; what lies outside the j keys is cut off."""
-    tables = [t for t in (cu_q, cu_k, prefix) if t is not None]
-    for t in tables:
-        _need(t.dtype == torch.int32 and t.dim() in (1, 2), 'attention_spans: int32 tables of one or two dimensions')
-    docs = cu_q.shape[-1] - 1
-    _need(docs >= 0, 'attention_spans: cu_q needs at least one bound')
-    _need(cu_k is None or cu_k.shape[-1] == docs + 1, 'attention_spans: cu_q and cu_k of one length')
-    _need(prefix is None or prefix.shape[-1] == docs, 'attention_spans: one prefix per document')
-    _need(prefix is None or causal, 'attention_spans: a prefix without causal order says nothing')
-    _need(cu_k is None or j is not None, 'attention_spans: cu_k needs the number of keys j')
-    j = n if j is None else j
-    _need(0 <= n < 2 ** 31 and 0 <= j < 2 ** 31, 'attention_spans: n and j from 0 to 2^31 - 1')
-    batches = {t.shape[0] for t in tables if t.dim() == 2}
-    _need(len(batches) <= 1, 'attention_spans: tables of different batch sizes')
-    b = batches.pop() if batches else 1
-    _same_device(cu_q, *tables)
-    tables = {id(t): t.contiguous() for t in tables}
-
-    def arg(t):
-        t = None if t is None else tables[id(t)]
-        return L.ptr(t), (t.shape[-1] if t is not None and t.dim() == 2 else 0)
-    out = torch.empty(b, n, 2, dtype=torch.int32, device=cu_q.device)
-    L.check(L.lib().mm_attention_spans(L.stream(), *arg(cu_q), *arg(cu_q if cu_k is None else cu_k), *arg(prefix), b, docs, n, j, int(causal), L.ptr(out)),
-            'mm_attention_spans')
-    return out if any(t.dim() == 2 for t in tables.values()) else out[0]
-
-
-def _rotary_desc(q, k, positions, freqs, sections, q_scale, k_scale, interleaved, dq=None, dk=None):
-    like, other = (q, k) if dq is None else (dq, dk)
-    sides = [('q', q, dq, q_scale), ('k', k, dk, k_scale)]
-    _need(like.dim() == 4, 'rotary: (batch, heads, tokens, width) tensors')
-    b, _, n, d = like.shape
-    _need(like.dtype in _DT, f'rotary: bf16, fp16 or fp32, not {like.dtype}')
-    sections = [int(s) for s in sections]
-    _need(1 <= len(sections) <= 4 and all(s >= 0 for s in sections), 'rotary: 1 to 4 sections')
-    _need(d % 2 == 0 and 2 <= d <= 256 and 2 * sum(sections) <= d, f'rotary: width {d} even, at most 256, at least twice the sum of the sections {sections}')
-    _need(freqs.dtype == torch.float64 and tuple(freqs.shape) == (sum(sections),), f'rotary: freqs float64 [{sum(sections)}] (one per pair)')
-    norm = q_scale is not None
-    _need(other is None or (k_scale is not None) == norm, 'rotary: both scales or none')
-    _need(other is not None or k_scale is None, 'rotary: k_scale without k')
-    used = [freqs, positions]
-    desc = L.Rotary()
-    for name, x, dy, scale in sides:
-        present = x if dy is None else dy
-        if present is None:
+    docs = cu_q.shape[-1] - 1 if cu_q.dim() else -1
+    if j is None:
+        if cu_k is not None:
+            raise _Err('attention_spans: cu_k needs the number of keys j')
+        j = n
+    if not (0 <= n < 2 ** 31 and 0 <= j < 2 ** 31):
+        raise _Err('attention_spans: n and j from 0 to 2^31 - 1')
+    if prefix is not None and not causal:
+        raise _Err('attention_spans: a prefix without causal order says nothing')
+    b, args, keep = 0, [], []
+    for t, width, what in ((cu_q, docs + 1, 'cu_q needs at least one bound'), (cu_q if cu_k is None else cu_k, docs + 1, 'cu_q and cu_k of one length'),
+                           (prefix, docs, 'one prefix per document')):
+        if t is None:
+            args += (None, 0)
             continue
-        _need(dy is None or not norm or x is not None, f'rotary: the gradient behind the norm needs {name}')
-        for t in (x, dy):
-            if t is None:
-                continue
-            _need(t.dim() == 4 and t.shape[0] == b and t.shape[2] == n and t.shape[3] == d and t.shape[1] == present.shape[1],
-                  f'rotary: {name} of shape {tuple(t.shape)} beside {tuple(like.shape)}')
-            _need(t.dtype == like.dtype, f'rotary: {t.dtype} beside {like.dtype}')
-            _need(t.stride(3) == 1 or t.numel() == 0, 'rotary: the elements of a head must be contiguous')
-            used.append(t)
-        if scale is not None:
-            _need(scale.dtype == torch.float32 and tuple(scale.shape) == (d,), f'rotary: {name}_scale fp32 [{d}]')
-            used.append(scale)
-    pos, pos_sb = _per_row(positions, 'rotary: positions', b, n, len(sections))
-    _same_device(like, *used)
-    keep = [pos, freqs.contiguous()]
-    outs = []
-    for name, x, dy, scale in sides:
-        present = x if dy is None else dy
-        side = getattr(desc, name)
-        if present is None:
+        s = t.shape
+        if t.dtype != torch.int32 or not 1 <= len(s) <= 2:
+            raise _Err(f'attention_spans: int32 tables of one or two dimensions, not {t.dtype} {tuple(s)}')
+        if s[-1] != width or docs < 0:
+            raise _Err('attention_spans: ' + what)
+        if len(s) == 2:
+            if b and s[0] != b:
+                raise _Err('attention_spans: tables of different batch sizes')
+            b = s[0]
+        t = t.contiguous()
+        keep.append(t)
+        args += (t.data_ptr(), width if len(s) == 2 else 0)
+    batched = any(t.dim() == 2 for t in keep)
+    stream = _one_device(*keep)
+    out = torch.empty((b, n, 2) if batched else (n, 2), dtype=torch.int32, device=cu_q.device)
+    L.check(L.lib().mm_attention_spans(stream, *args, b if batched else 1, docs, n, j, int(causal), out.data_ptr()), 'mm_attention_spans')
+    return out
+
+
+def _rotary(q, k, positions, freqs, sections, q_scale, k_scale, interleaved, bwd, dq=None, dk=None):
+    """the descriptor of both directions (q / k: inputs of the forward, needed for the gradient behind the norm only; dq / dk: gradients of the outputs)"""
+    like, other = (dq, dk) if bwd else (q, k)
+    norm = q_scale is not None
+    shape = like.shape
+    if len(shape) != 4:
+        raise _Err(f'rotary: (batch, heads, tokens, width) tensors, not {tuple(shape)}')
+    b, _, n, d = shape
+    dt = like.dtype
+    if dt not in _DT:
+        raise _Err(f'rotary: bf16, fp16 or fp32, not {dt}')
+    axes, P = len(sections), sum(sections)
+    if not 1 <= axes <= 4 or min(sections) < 0:
+        raise _Err('rotary: 1 to 4 sections')
+    if d % 2 or not 2 <= d <= 256 or 2 * P > d:
+        raise _Err(f'rotary: width {d} even, at most 256, at least twice the sum of the sections {list(sections)}')
+    if freqs.dtype != torch.float64 or freqs.shape != (P,):
+        raise _Err(f'rotary: freqs float64 [{P}] (one per pair)')
+    if other is None:
+        if k_scale is not None:
+            raise _Err('rotary: k_scale without k')
+    elif (k_scale is not None) != norm:
+        raise _Err('rotary: both scales or none')
+    pos, pos_sb = _per_row(positions, 'rotary: positions', b, n, axes)
+    freqs = freqs.contiguous()
+    used, sides, outs = [pos, freqs], [], []
+    for name, x, dy, scale in (('q', q, dq, q_scale), ('k', k, dk, k_scale)):
+        lead = dy if bwd else x
+        if lead is None:
+            sides += (0,) * 12
             outs.append(None)
             continue
-        out = _heads_view(b, n, present.shape[1], d, like)
-        side.heads, side.out = present.shape[1], L.ptr(out)
-        if x is not None and (dy is None or norm):
-            side.x, side.x_stride = L.ptr(x), _heads_st(x)
-        if dy is not None:
-            side.dy, side.dy_stride = L.ptr(dy), _heads_st(dy)
+        if bwd and not norm:
+            x = None
+        elif x is None:
+            raise _Err(f'rotary: the gradient behind the norm needs {name}')
+        st = []
+        for t in (x, dy):
+            if t is None:
+                st += (0, 0, 0)
+                continue
+            s = t.shape
+            if len(s) != 4 or s[0] != b or s[2] != n or s[3] != d or s[1] != lead.shape[1] or t.dtype != dt:
+                raise _Err(f'rotary: {name} {t.dtype} {tuple(s)} beside {dt} {tuple(shape)}')
+            z = t.stride()
+            if z[3] != 1 and t.numel():
+                raise _Err('rotary: the elements of a head must be contiguous')
+            st += z[:3]
+            used.append(t)
         if scale is not None:
+            if scale.dtype != torch.float32 or scale.shape != (d,):
+                raise _Err(f'rotary: {name}_scale fp32 [{d}]')
             scale = scale.contiguous()
-            keep.append(scale)
-            side.scale = L.ptr(scale)
-        outs.append(out)
-    desc.positions, desc.pos_sb, desc.freqs = L.ptr(pos), pos_sb, L.ptr(keep[1])
-    desc.sections[:len(sections)] = sections
-    desc.axes, desc.batch, desc.n, desc.dim, desc.dtype = len(sections), b, n, d, _DT[like.dtype]
-    desc.interleaved, desc.normalize = int(interleaved), int(norm)
-    return desc, outs, keep
+            used.append(scale)
+        sides += (_ptr(x), _ptr(dy), lead, _ptr(scale), *st, lead.shape[1], 0)
+        outs.append(lead)
+    stream = _one_device(*used)
+    for i, lead in enumerate(outs):
+        if lead is not None:
+            outs[i] = _rows_out(b, n, lead.shape[1], d, like)
+            sides[12 * i + 2] = outs[i].data_ptr()
+    desc = _ROTARY.pack(*sides, pos.data_ptr(), pos_sb, freqs.data_ptr(), *sections, *(0,) * (4 - axes), axes, b, n, d, _DT[dt], int(interleaved), int(norm), 0)
+    return desc, outs, stream, used
 
 
 def rotary_axes(q, k, positions, freqs, sections, q_scale=None, k_scale=None, interleaved=False):
@@ -975,80 +997,91 @@ def rotary_axes(q, k, positions, freqs, sections, q_scale=None, k_scale=None, in
     radians per unit of position.  Pairs are elements (p, P + p), interleaved: (2p, 2p + 1); the elements behind the pairs pass.  With q_scale / k_scale fp32 [d]
     the heads are l2-normalised and scaled first (mmp.py:151-153).  d even, up to 128 (256 where rows are 16-byte aligned and the sections add up to a multiple of
     8 with a rest of whole 16 elements).  Returns (q', k') as (b, h, n, d) views of [b, n, h, d] rows."""
-    desc, outs, keep = _rotary_desc(q, k, positions, freqs, sections, q_scale, k_scale, interleaved)
-    L.check(L.lib().mm_rotary_axes(L.stream(), L.C.byref(desc)), 'mm_rotary_axes')
+    desc, outs, stream, keep = _rotary(q, k, positions, freqs, sections, q_scale, k_scale, interleaved, False)
+    L.check(L.lib().mm_rotary_axes(stream, desc), 'mm_rotary_axes')
     return tuple(outs)
 
 
 def rotary_axes_bwd(dq, dk, positions, freqs, sections, q=None, k=None, q_scale=None, k_scale=None, interleaved=False):
     """Gradients of rotary_axes from those of its outputs: (dq, dk, dq_scale, dk_scale) with respect to q, k (their dtype) and the scales (fp32 [d]; None without
     them).  With scales q and k, the inputs of the forward, are needed again."""
-    norm = q_scale is not None
-    desc, outs, keep = _rotary_desc(q, k, positions, freqs, sections, q_scale, k_scale, interleaved, dq, dk)
+    desc, outs, stream, keep = _rotary(q, k, positions, freqs, sections, q_scale, k_scale, interleaved, True, dq, dk)
     lib = L.lib()
-    d = dq.shape[3]
-    ds = torch.empty(2, d, dtype=torch.float32, device=dq.device) if norm else None
-    nbytes = lib.mm_rotary_axes_bwd_workspace_bytes(L.C.byref(desc))
+    if q_scale is None:
+        L.check(lib.mm_rotary_axes_bwd(stream, desc, None, None, 0), 'mm_rotary_axes_bwd')
+        return outs[0], outs[1], None, None
+    ds = torch.empty(2, dq.shape[3], dtype=torch.float32, device=dq.device)
+    nbytes = lib.mm_rotary_axes_bwd_workspace_bytes(desc)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dq.device) if nbytes else None
-    if norm and dq.shape[0] * dq.shape[2] == 0:
+    if dq.shape[0] * dq.shape[2] == 0:
         ds.zero_()
     else:
-        L.check(lib.mm_rotary_axes_bwd(L.stream(), L.C.byref(desc), L.ptr(ds), L.ptr(ws), nbytes), 'mm_rotary_axes_bwd')
-    return outs[0], outs[1], (ds[0] if norm else None), (ds[1] if norm and dk is not None else None)
+        L.check(lib.mm_rotary_axes_bwd(stream, desc, ds.data_ptr(), _ptr(ws), nbytes), 'mm_rotary_axes_bwd')
+    return outs[0], outs[1], ds[0], (ds[1] if dk is not None else None)
 
 
-def _span_desc(q, k, v, spans, scale, softcap, slopes, positions, key_positions, key_mask, extra=()):
-    for name, t in (('q', q), ('k', k), ('v', v)):
-        _need(t.dim() == 4, f'attend_spans: {name} (batch, heads, tokens, width)')
-        _need(t.dtype in (torch.bfloat16, torch.float16) and t.dtype == q.dtype, f'attend_spans: bf16 or fp16 of one type, not {q.dtype} / {t.dtype}')
-        _need(t.stride(3) == 1 or t.numel() == 0, 'attend_spans: the elements of a head must be contiguous')
-    b, hq, n, d = q.shape
-    hk, j = k.shape[1], k.shape[2]
-    _need(k.shape == v.shape and k.shape[0] == b and k.shape[3] == d, f'attend_spans: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}')
-    _need(d in (32, 64, 128), f'attend_spans: width 32, 64 or 128, not {d}')
-    _need(hq > 0 and hk > 0 and hq % hk == 0, f'attend_spans: {hq} query heads over {hk} key heads')
-    _need(math.isfinite(scale) and scale > 0, f'attend_spans: scale {scale} is not positive')
-    _need(math.isfinite(softcap) and softcap >= 0, f'attend_spans: softcap {softcap} is neither 0 nor positive')
-    desc = L.SpanAttn()
-    keep = []
-    used = [k, v, *extra]
-    if spans is not None:
-        sp, desc.spans_sb = _per_row(spans, 'attend_spans: spans', b, n, 2)
-        if sp.data_ptr() % 8:
-            sp = sp.clone()
-        keep.append(sp)
-        used.append(sp)
-        desc.spans = L.ptr(sp)
-    if key_mask is not None:
-        _need(tuple(key_mask.shape) == (b, j) and key_mask.dtype in (torch.bool, torch.uint8), f'attend_spans: key_mask bool or uint8 ({b}, {j})')
-        km = key_mask.contiguous()
-        keep.append(km)
-        used.append(km)
-        desc.key_mask, desc.key_mask_sb = L.ptr(km), j
-    _need((slopes is None) == (positions is None), 'attend_spans: slopes and positions, or neither')
-    _need(key_positions is None or positions is not None, 'attend_spans: key_positions without positions')
+def _span_args(q, k, v, spans, scale, softcap, slopes, positions, key_positions, key_mask, extra):
+    """the checked front of the descriptor: (fields up to q / k / v strides, sizes, stream, tensors to keep)"""
+    qs, ks, dt = q.shape, k.shape, q.dtype
+    if len(qs) != 4 or len(ks) != 4:
+        raise _Err(f'attend_spans: (batch, heads, tokens, width) tensors, not {tuple(qs)} / {tuple(ks)}')
+    if dt != torch.bfloat16 and dt != torch.float16 or k.dtype != dt or v.dtype != dt:
+        raise _Err(f'attend_spans: bf16 or fp16 of one type, not {dt} / {k.dtype} / {v.dtype}')
+    b, hq, n, d = qs
+    _, hk, j, _ = ks
+    if v.shape != ks or ks[0] != b or ks[3] != d:
+        raise _Err(f'attend_spans: q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)}')
+    if d not in (32, 64, 128):
+        raise _Err(f'attend_spans: width 32, 64 or 128, not {d}')
+    if hk < 1 or hq < 1 or hq % hk:
+        raise _Err(f'attend_spans: {hq} query heads over {hk} key heads')
+    if not 0 < scale < 1e30:
+        raise _Err(f'attend_spans: scale {scale} is not positive')
+    if not 0 <= softcap < 1e30:
+        raise _Err(f'attend_spans: softcap {softcap} is neither 0 nor positive')
+    st = []
+    for t in (q, k, v):
+        z = t.stride()
+        if z[3] != 1 and t.numel():
+            raise _Err('attend_spans: the elements of a head must be contiguous')
+        st += z[:3]
+    used = [q, k, v, *extra]
+    sp = sp_sb = km = pq = pq_sb = pk = pk_sb = sl = 0
     axes = 0
-    if slopes is not None:
+    if spans is not None:
+        t, sp_sb = _per_row(spans, 'attend_spans: spans', b, n, 2)
+        sp = t.data_ptr()
+        if sp % 8:
+            t = t.clone()
+            sp = t.data_ptr()
+        used.append(t)
+    if key_mask is not None:
+        if key_mask.shape != (b, j) or key_mask.dtype not in (torch.bool, torch.uint8):
+            raise _Err(f'attend_spans: key_mask bool or uint8 ({b}, {j})')
+        t = key_mask.contiguous()
+        km = t.data_ptr()
+        used.append(t)
+    if slopes is None:
+        if positions is not None:
+            raise _Err('attend_spans: slopes and positions, or neither')
+        if key_positions is not None:
+            raise _Err('attend_spans: key_positions without positions')
+    else:
         axes = slopes.shape[-1]
-        _need(slopes.dtype == torch.float32 and slopes.dim() == 2 and slopes.shape[0] == hq and 1 <= axes <= 3, f'attend_spans: slopes fp32 ({hq}, 1 .. 3)')
-        _need(key_positions is not None or n == j, 'attend_spans: key_positions where queries and keys differ in number')
-        sl = slopes.contiguous()
-        pq, desc.positions_q_sb = _per_row(positions, 'attend_spans: positions', b, n, axes)
-        pk, desc.positions_k_sb = _per_row(key_positions, 'attend_spans: key_positions', b, j, axes) if key_positions is not None else (pq, desc.positions_q_sb)
-        keep += [sl, pq, pk]
-        used += [sl, pq, pk]
-        desc.slopes, desc.positions_q, desc.positions_k = L.ptr(sl), L.ptr(pq), L.ptr(pk)
-    _same_device(q, *used)
-    for name, t in (('q', q), ('k', k), ('v', v)):
-        setattr(desc, name, L.ptr(t))
-        setattr(desc, name + '_stride', _heads_st(t))
-    desc.batch, desc.heads_q, desc.heads_k, desc.nq, desc.nk, desc.dim, desc.axes, desc.dtype = b, hq, hk, n, j, d, axes, _DT[q.dtype]
-    desc.scale, desc.softcap = scale, softcap
-    return desc, keep
-
-
-def _span_ws(nbytes, like):
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+        if positions is None:
+            raise _Err('attend_spans: slopes and positions, or neither')
+        if slopes.dtype != torch.float32 or slopes.dim() != 2 or slopes.shape[0] != hq or not 1 <= axes <= 3:
+            raise _Err(f'attend_spans: slopes fp32 ({hq}, 1 .. 3)')
+        if key_positions is None and n != j:
+            raise _Err('attend_spans: key_positions where queries and keys differ in number')
+        t = slopes.contiguous()
+        u, pq_sb = _per_row(positions, 'attend_spans: positions', b, n, axes)
+        w, pk_sb = (u, pq_sb) if key_positions is None else _per_row(key_positions, 'attend_spans: key_positions', b, j, axes)
+        sl, pq, pk = t.data_ptr(), u.data_ptr(), w.data_ptr()
+        used += (t, u, w)
+    stream = _one_device(*used)
+    head = (sp, sp_sb, km, j, sl, pq, pq_sb, pk, pk_sb, *st)
+    return head, (b, hq, hk, n, j, d, axes, _DT[dt]), stream, used
 
 
 def attend_spans(q, k, v, spans=None, scale=8.0, softcap=0.0, slopes=None, positions=None, key_positions=None, key_mask=None, return_lse=False, out_rows=False):
@@ -1058,18 +1091,21 @@ def attend_spans(q, k, v, spans=None, scale=8.0, softcap=0.0, slopes=None, posit
     key_positions default: positions): sum over the axes of slope * |distance| is taken off the score; |position| < 2^30.  A row that sees nothing gives 0
     (lse -inf); what a row does not see never reaches it, infinities and NaN included.  Returns (b, hq, n, d) (a view of rows), out_rows: [b * n, hq * d], and with
     return_lse also the log of the sum of exp(score), fp32 (b, hq, n)."""
-    desc, keep = _span_desc(q, k, v, spans, float(scale), float(softcap), slopes, positions, key_positions, key_mask)
-    b, hq, n, d = q.shape
-    out = _heads_view(b, n, hq, d, q)
+    head, sizes, stream, keep = _span_args(q, k, v, spans, scale, softcap, slopes, positions, key_positions, key_mask, ())
+    b, hq, hk, n, j, d = sizes[:6]
+    out = _rows_out(b, n, hq, d, q)
     lse = torch.empty(b, hq, n, dtype=torch.float32, device=q.device) if return_lse else None
-    desc.out, desc.out_stride, desc.lse = L.ptr(out), _heads_st(out), L.ptr(lse)
+    desc = _SPAN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), *head, n * hq * d, d, hq * d, b, hq, hk, n, j, *sizes[5:], scale, softcap, *_NO_GRADS)
     lib = L.lib()
-    nbytes = lib.mm_span_attention_workspace_bytes(L.C.byref(desc))
-    ws = _span_ws(nbytes, q)
-    L.check(lib.mm_span_attention(L.stream(), L.C.byref(desc), L.ptr(ws), nbytes), 'mm_span_attention')
+    nbytes = lib.mm_span_attention_workspace_bytes(desc)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    L.check(lib.mm_span_attention(stream, desc, _ptr(ws), nbytes), 'mm_span_attention')
     if out_rows:
         out = out.permute(0, 2, 1, 3).reshape(b * n, hq * d)
     return (out, lse) if return_lse else out
+
+
+_NO_GRADS = (0,) * 17
 
 
 def attend_spans_bwd(q, k, v, out, lse, dout, spans=None, scale=8.0, softcap=0.0, slopes=None, positions=None, key_positions=None, key_mask=None):
@@ -1077,27 +1113,27 @@ def attend_spans_bwd(q, k, v, out, lse, dout, spans=None, scale=8.0, softcap=0.0
     dk / dv (b, hk, j, d) as views of rows, dslopes fp32 (hq, axes) or None without slopes.  dk and dv are summed over the heads that share a key head.  Rows that
     see nothing (lse -inf) and keys that nothing sees get and give 0, whatever they hold.  No atomics: the same bits every time."""
     for name, t in (('out', out), ('dout', dout)):
-        _need(t.shape == q.shape and t.dtype == q.dtype, f'attend_spans_bwd: {name} {t.dtype} {tuple(t.shape)} beside q {q.dtype} {tuple(q.shape)}')
-        _need(t.stride(3) == 1 or t.numel() == 0, 'attend_spans_bwd: the elements of a head must be contiguous')
-    _need(q.dtype == torch.bfloat16, f'attend_spans_bwd: bf16, not {q.dtype}')
-    _need(lse.dtype == torch.float32 and lse.shape == q.shape[:3], f'attend_spans_bwd: lse fp32 {tuple(q.shape[:3])}')
-    desc, keep = _span_desc(q, k, v, spans, float(scale), float(softcap), slopes, positions, key_positions, key_mask, extra=(out, lse, dout))
-    b, hq, n, d = q.shape
-    hk, j = k.shape[1], k.shape[2]
+        if t.shape != q.shape or t.dtype != q.dtype:
+            raise _Err(f'attend_spans_bwd: {name} {t.dtype} {tuple(t.shape)} beside q {q.dtype} {tuple(q.shape)}')
+        if t.dim() == 4 and t.stride(3) != 1 and t.numel():
+            raise _Err('attend_spans_bwd: the elements of a head must be contiguous')
+    if q.dtype != torch.bfloat16:
+        raise _Err(f'attend_spans_bwd: bf16, not {q.dtype}')
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:3]:
+        raise _Err(f'attend_spans_bwd: lse fp32 {tuple(q.shape[:3])}')
+    head, sizes, stream, keep = _span_args(q, k, v, spans, scale, softcap, slopes, positions, key_positions, key_mask, (out, lse, dout))
+    b, hq, hk, n, j, d = sizes[:6]
     lse = lse.contiguous()
-    dq, dk, dv = _heads_view(b, n, hq, d, q), _heads_view(b, j, hk, d, q), _heads_view(b, j, hk, d, q)
-    for name, t in (('out', out), ('dout', dout), ('dq', dq), ('dk', dk), ('dv', dv)):
-        setattr(desc, name, L.ptr(t))
-        setattr(desc, name + '_stride', _heads_st(t))
-    desc.lse = L.ptr(lse)
+    dq, dk, dv = _rows_out(b, n, hq, d, q), _rows_out(b, j, hk, d, q), _rows_out(b, j, hk, d, q)
     dslopes = None
     if slopes is not None:
         dslopes = torch.empty(slopes.shape, dtype=torch.float32, device=q.device)
-        desc.dslopes = L.ptr(dslopes)
         if b * n == 0:
             dslopes.zero_()
+    grads = (dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dslopes), *dout.stride()[:3], n * hq * d, d, hq * d, *(j * hk * d, d, hk * d) * 2)
+    desc = _SPAN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *head, *out.stride()[:3], b, hq, hk, n, j, *sizes[5:], scale, softcap, *grads)
     lib = L.lib()
-    nbytes = lib.mm_span_attention_bwd_workspace_bytes(L.C.byref(desc))
-    ws = _span_ws(nbytes, q)
-    L.check(lib.mm_span_attention_bwd(L.stream(), L.C.byref(desc), L.ptr(ws), nbytes), 'mm_span_attention_bwd')
+    nbytes = lib.mm_span_attention_bwd_workspace_bytes(desc)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    L.check(lib.mm_span_attention_bwd(stream, desc, _ptr(ws), nbytes), 'mm_span_attention_bwd')
     return dq, dk, dv, dslopes

@@ -72,6 +72,23 @@ def test_attention_bwd_refusals():
             refuses(match, ops.attend_spans_bwd, **{**a, **dict(out=a['q'], lse=lse, dout=a['q']), **change})
 
 
+def test_packed_descriptors_have_the_fields_of_the_c_structs():
+    for packer, cls in ((ops._ROTARY, _lib.Rotary), (ops._SPAN, _lib.SpanAttn)):
+        assert packer.size == _lib.C.sizeof(cls)
+        d = cls.from_buffer_copy(packer.pack(*range(1, len(packer.unpack(bytes(packer.size))) + 1)))
+
+        def flat(x):
+            for f, t in x._fields_:
+                v = getattr(x, f)
+                if isinstance(v, _lib.C.Structure):
+                    yield from flat(v)
+                elif isinstance(v, _lib.C.Array):
+                    yield from v
+                else:
+                    yield v
+        assert list(flat(d)) == list(range(1, len(list(flat(d))) + 1))
+
+
 def span_desc(**change):
     """a descriptor whose pointers are never followed: the C checks come first"""
     d = _lib.SpanAttn()
