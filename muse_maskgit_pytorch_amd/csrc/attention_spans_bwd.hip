@@ -100,13 +100,12 @@ __device__ __forceinline__ void query_again(const SpanArgs& p, int b, int h, int
 
 // gradients of one key row from the queries that see it alone, by one wave (lane = query, then lane = element)
 template <int D, int AX>
-__device__ __forceinline__ void key_again(const SpanArgs& p, int b, int hk, int key, int lane, float (&dk)[2], float (&dv)[2]) {
-    const int group = p.Hq / p.Hk;
+__device__ __forceinline__ void key_again(const SpanArgs& p, int b, int hk, int h0, int h1, int key, int lane, float (&dk)[2], float (&dv)[2]) {
     const uint16_t* k = p.k + b * p.k_s[0] + hk * p.k_s[1] + (long)key * p.k_s[2];
     const uint16_t* v = p.v + b * p.v_s[0] + hk * p.v_s[1] + (long)key * p.v_s[2];
     dk[0] = dk[1] = dv[0] = dv[1] = 0.f;
 #pragma nounroll
-    for (int h = hk * group; h < (hk + 1) * group; ++h)
+    for (int h = h0; h < h1; ++h)
 #pragma nounroll
         for (int t0 = 0; t0 < p.nq; t0 += 64) {
             const int i = t0 + lane;
@@ -136,7 +135,7 @@ __device__ __forceinline__ void key_again(const SpanArgs& p, int b, int hk, int 
         }
 }
 
-template <int D, int AX>
+template <int D, int AX, bool CAP>
 __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
     typedef Tile<D, BT> T;
     extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
@@ -184,8 +183,7 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
     const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1];
     const uint8_t* km = p.kmask ? p.kmask + b * p.km_sb : nullptr;
     const int* pkp = AX ? p.pos_k + b * p.pk_sb : nullptr;
-    const bool capped = p.cap > 0.f;
-    const float c1 = capped ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E, c2 = p.cap * SPAN_LOG2E;
+    const float c1 = CAP ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E, c2 = p.cap * SPAN_LOG2E;
 
 #define SPAN_ISSUE(it_)                                                                                                \
     {                                                                                                                  \
@@ -242,7 +240,7 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
                     for (int e = 0; e < 4; ++e) {
                         const int r = g4 * 4 + e;
                         float x = s[r], slope = 1.f, far[AX ? AX : 1];
-                        if (capped) { const float th = span_tanh(x, c1); slope = __builtin_fmaf(-th, th, 1.f); x = th * c2; }
+                        if constexpr (CAP) { const float th = span_tanh(x, c1); slope = __builtin_fmaf(-th, th, 1.f); x = th * c2; }
                         else x *= c1;
 #pragma unroll
                         for (int a = 0; a < AX; ++a) {
@@ -254,8 +252,9 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
                         if (!(wb & (1u << (8 * g4 + e)))) d = 0.f;
 #pragma unroll
                         for (int a = 0; a < AX; ++a) ds_sl[a] = __builtin_fmaf(d, far[a], ds_sl[a]);
-                        s[r] = d * slope;
+                        s[r] = CAP ? d * slope : d;
                     }
+                    __builtin_amdgcn_sched_barrier(0);      // (four scores at a time: all sixteen at once cost 60 registers more, and the second workgroup of a CU)
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -312,7 +311,7 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
     }
 }
 
-template <int D, int AX>
+template <int D, int AX, bool CAP>
 __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const SpanArgs p) {
     typedef Tile<D, BT> T;
     extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
@@ -322,10 +321,11 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
     int* cnt = reinterpret_cast<int*>(hull + 512);                            // [4]
     const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int tiles = (p.nk + BK - 1) / BK, total = p.B * p.Hk * tiles, per = (total + 7) / 8;
+    const int tiles = (p.nk + BK - 1) / BK, total = p.B * p.Hk * p.splits * tiles, per = (total + 7) / 8;
     const int item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || item >= total) return;
-    const int tile = item % tiles, hk = (item / tiles) % p.Hk, b = item / tiles / p.Hk, group = p.Hq / p.Hk;
+    const int tile = item % tiles, part = (item / tiles) % p.splits, hk = (item / tiles / p.splits) % p.Hk, b = item / tiles / p.splits / p.Hk;
+    const int heads = p.Hq / p.Hk / p.splits, h0 = (hk * p.splits + part) * heads, h1 = h0 + heads;      // the query heads of this workgroup
     const int t0 = tile * BK, t1 = min(t0 + BK, p.nk), w0 = t0 + w * 32;      // the wave's keys: w0 .. w0 + 31
     const int key = w0 + (lane & 31);
     const bool live = key < p.nk && (!p.kmask || p.kmask[b * p.km_sb + key]);      // a key that is not there or masked: zeros, no weight
@@ -344,8 +344,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
     int pk[AX ? AX : 1];
 #pragma unroll
     for (int a = 0; a < AX; ++a) pk[a] = key < p.nk ? p.pos_k[b * p.pk_sb + (long)key * AX + a] : 0;
-    const bool capped = p.cap > 0.f;
-    const float c1 = capped ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E, c2 = p.cap * SPAN_LOG2E;
+    const float c1 = CAP ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E, c2 = p.cap * SPAN_LOG2E;
     f32x16_t dk[D / 32], dv[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
@@ -356,31 +355,27 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
     float lsev = 0.f, delv = 0.f;
     int2 spv = make_int2(0, 0);
     int posv[AX ? AX : 1];
-    // (row bookkeeping: lane = row of the 64-row tile, every wave the same; wave 0 writes it to LDS)
-#define SPAN_TILE(it_) const int h_ = hk * group + (it_) / n_list, q0_ = list[(it_) % n_list] * BT;
-#define SPAN_ISSUE(it_)                                                                                                                                    \
-    {                                                                                                                                                      \
-        SPAN_TILE(it_)                                                                                                                                     \
-        unsigned char* st_ = smem + ((it_) & 1) * STAGE;                                                                                                   \
-        const int qs_ = __builtin_amdgcn_readfirstlane(q0_), ok_ = min(BT, p.nq - qs_);                                                                    \
-        T::template fill<4>(st_, p.q + b * p.q_s[0] + h_ * p.q_s[1] + (long)qs_ * p.q_s[2], ok_, (int)p.q_s[2], w, lane);                                  \
-        T::template fill<4>(st_ + T::BYTES, p.dout + b * p.do_s[0] + h_ * p.do_s[1] + (long)qs_ * p.do_s[2], ok_, (int)p.do_s[2], w, lane);                \
+    // the tile being fetched: entry f_at of the list, head f_h (its rows: lane = row of the 64, every wave the same; wave 0 writes them to LDS)
+    int f_at = 0, f_h = h0, f_stage = 0;
+    const uint16_t *f_q = p.q + b * p.q_s[0] + f_h * p.q_s[1], *f_g = p.dout + b * p.do_s[0] + f_h * p.do_s[1];
+#define SPAN_ISSUE()                                                                                                              \
+    {                                                                                                                             \
+        unsigned char* st_ = smem + f_stage * STAGE;                                                                              \
+        const int q0_ = __builtin_amdgcn_readfirstlane(list[f_at]) * BT, ok_ = min(BT, p.nq - q0_);                               \
+        T::template fill<4>(st_, f_q + (long)q0_ * p.q_s[2], ok_, (int)p.q_s[2], w, lane);                                        \
+        T::template fill<4>(st_ + T::BYTES, f_g + (long)q0_ * p.do_s[2], ok_, (int)p.do_s[2], w, lane);                           \
+        const int i_ = q0_ + lane;                                                                                                \
+        spv = make_int2(0, 0); lsev = 0.f; delv = 0.f;                                                                            \
+        if (i_ < p.nq) {                                                                                                          \
+            const long row_ = ((long)b * p.Hq + f_h) * p.nq + i_;                                                                 \
+            spv = row_span(p, b, f_h, i_);                                                                                        \
+            lsev = p.lse[row_] * SPAN_LOG2E; delv = p.delta[row_];                                                                \
+            _Pragma("unroll") for (int a = 0; a < AX; ++a) posv[a] = p.pos_q[b * p.pq_sb + (long)i_ * AX + a];                    \
+        }                                                                                                                         \
     }
-#define SPAN_ROW_LOAD(it_)                                                                                   \
-    {                                                                                                        \
-        SPAN_TILE(it_)                                                                                       \
-        const int i_ = q0_ + lane;                                                                           \
-        spv = make_int2(0, 0); lsev = 0.f; delv = 0.f;                                                       \
-        if (i_ < p.nq) {                                                                                     \
-            const long row_ = ((long)b * p.Hq + h_) * p.nq + i_;                                             \
-            spv = row_span(p, b, h_, i_);                                                                    \
-            lsev = p.lse[row_] * SPAN_LOG2E; delv = p.delta[row_];                                           \
-            _Pragma("unroll") for (int a = 0; a < AX; ++a) posv[a] = p.pos_q[b * p.pq_sb + (long)i_ * AX + a]; \
-        }                                                                                                    \
-    }
-#define SPAN_ROW_STORE(it_)                                                                                  \
+#define SPAN_ROW_STORE()                                                                                     \
     if (w == 0) {                                                                                            \
-        float* rw_ = reinterpret_cast<float*>(smem + ((it_) & 1) * STAGE + 2 * T::BYTES);                    \
+        float* rw_ = reinterpret_cast<float*>(smem + f_stage * STAGE + 2 * T::BYTES);                        \
         rw_[lane] = lsev; rw_[BT + lane] = delv;                                                             \
         reinterpret_cast<int*>(rw_)[2 * BT + lane] = spv.x; reinterpret_cast<int*>(rw_)[3 * BT + lane] = spv.y; \
         _Pragma("unroll") for (int a = 0; a < AX; ++a) reinterpret_cast<int*>(rw_)[(4 + a) * BT + lane] = posv[a]; \
@@ -401,26 +396,33 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
             const unsigned long long m = __ballot(in);
             if (lane == 0) cnt[w] = __popcll(m);
             __syncthreads();
-            int at = __popcll(m & ((1ull << lane) - 1ull));
-            for (int x = 0; x < w; ++x) at += cnt[x];
+            int to = __popcll(m & ((1ull << lane) - 1ull));
+            for (int x = 0; x < w; ++x) to += cnt[x];
             n_list = __builtin_amdgcn_readfirstlane(cnt[0] + cnt[1] + cnt[2] + cnt[3]);
-            if (in) { list[at] = qt; hull[2 * at] = a; hull[2 * at + 1] = e; }
+            if (in) { list[to] = qt; hull[2 * to] = a; hull[2 * to + 1] = e; }
             __syncthreads();
         }
-        const int steps = n_list * group;
-        if (steps > 0) { SPAN_ISSUE(0); SPAN_ROW_LOAD(0); SPAN_ROW_STORE(0); }
-        for (int it = 0; it < steps; ++it) {
-            unsigned char* Qs = smem + (it & 1) * STAGE;
+        if (n_list == 0) continue;
+        f_at = 0; f_h = h0; f_stage = 0;
+        f_q = p.q + b * p.q_s[0] + f_h * p.q_s[1]; f_g = p.dout + b * p.do_s[0] + f_h * p.do_s[1];
+        SPAN_ISSUE();
+        SPAN_ROW_STORE();
+        for (bool more = true; more;) {
+            const int at = f_at, stage = f_stage, h = f_h;
+            unsigned char* Qs = smem + stage * STAGE;
             unsigned char* Gs = Qs + T::BYTES;
             const float* rw = reinterpret_cast<const float*>(Gs + T::BYTES);
             const int* ri = reinterpret_cast<const int*>(rw);
             const unsigned long long keep = __ballot(spv.x < t1 && spv.y > t0);      // rows that see some key of the tile
             float sl[AX ? AX : 1];
 #pragma unroll
-            for (int a = 0; a < AX; ++a) sl[a] = p.slopes[(hk * group + it / n_list) * AX + a] * SPAN_LOG2E;
+            for (int a = 0; a < AX; ++a) sl[a] = p.slopes[h * AX + a] * SPAN_LOG2E;
+            if (++f_at == n_list) { f_at = 0; ++f_h; f_q += p.q_s[1]; f_g += p.do_s[1]; }
+            more = f_h < h1;
+            f_stage ^= 1;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (it + 1 < steps) { SPAN_ISSUE(it + 1); SPAN_ROW_LOAD(it + 1); }
+            if (more) SPAN_ISSUE();
             if (keep != ~0ull) {      // the others' values take no part, whatever they hold (rows behind the last document)
                 T::clear_rows(Qs, keep, t, 256);
                 T::clear_rows(Gs, keep, t, 256);
@@ -428,7 +430,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                const int4 hl = hull[2 * (it % n_list) + n];
+                const int4 hl = hull[2 * at + n];
                 if (!(hl.x < min(w0 + 32, t1) && hl.y > w0)) continue;
                 const bool masked = !all_live || !(hl.z <= w0 && hl.w >= w0 + 32) || (uint32_t)(keep >> (32 * n)) != 0xFFFFFFFFu;
                 f32x16_t s, g;
@@ -453,7 +455,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
                         const int r = g4 * 4 + e;
 #define SPAN_E4(v_) (e == 0 ? v_.x : (e == 1 ? v_.y : (e == 2 ? v_.z : v_.w)))
                         float x = s[r], slope = 1.f;
-                        if (capped) { const float th = span_tanh(x, c1); slope = __builtin_fmaf(-th, th, 1.f); x = th * c2; }
+                        if constexpr (CAP) { const float th = span_tanh(x, c1); slope = __builtin_fmaf(-th, th, 1.f); x = th * c2; }
                         else x *= c1;
 #pragma unroll
                         for (int a = 0; a < AX; ++a) x = __builtin_fmaf(-sl[a], fabsf((float)(SPAN_E4(qq[a]) - pk[a])), x);
@@ -461,8 +463,9 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
                         if (masked && !(live && SPAN_E4(lo4) <= key && key < SPAN_E4(hi4))) { pr = 0.f; d = 0.f; }
 #undef SPAN_E4
                         s[r] = pr;
-                        g[r] = d * slope;
+                        g[r] = CAP ? d * slope : d;
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -474,12 +477,10 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
                     }
                 }
             }
-            if (it + 1 < steps) SPAN_ROW_STORE(it + 1);
+            if (more) SPAN_ROW_STORE();
         }
     }
-#undef SPAN_TILE
 #undef SPAN_ISSUE
-#undef SPAN_ROW_LOAD
 #undef SPAN_ROW_STORE
     float bad = 0.f;
 #pragma unroll
@@ -488,7 +489,21 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
         for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(dk[c][r], 0.f, __builtin_fmaf(dv[c][r], 0.f, bad));
     bad = both_halves_sum(bad);
     const bool redo = live && bad != 0.f;
-    if (key < p.nk && !redo) {
+    const long prow = ((long)b * p.Hk + hk) * p.nk, pall = (long)p.B * p.Hk * p.nk;      // partial sums: [splits][dk, dv][rows][D]
+    if (p.splits > 1) {
+        if (key < p.nk && !redo) {
+            float* kp = p.part_o + ((long)part * 2 * pall + prow + key) * D + half * 4;
+            float* vp = kp + pall * D;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+                    *reinterpret_cast<float4*>(kp + c * 32 + g * 8) = live ? make_float4(dk[c][4 * g], dk[c][4 * g + 1], dk[c][4 * g + 2], dk[c][4 * g + 3]) : z;
+                    *reinterpret_cast<float4*>(vp + c * 32 + g * 8) = live ? make_float4(dv[c][4 * g], dv[c][4 * g + 1], dv[c][4 * g + 2], dv[c][4 * g + 3]) : z;
+                }
+        }
+    } else if (key < p.nk && !redo) {
         uint16_t* kp = p.dk + b * p.dk_s[0] + hk * p.dk_s[1] + (long)key * p.dk_s[2] + half * 4;
         uint16_t* vp = p.dv + b * p.dv_s[0] + hk * p.dv_s[1] + (long)key * p.dv_s[2] + half * 4;
 #pragma unroll
@@ -507,7 +522,14 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
         const int r = __builtin_ctzll(todo);
         todo &= todo - 1;
         float a[2], c[2];
-        key_again<D, AX>(p, b, hk, w0 + r, lane, a, c);
+        key_again<D, AX>(p, b, hk, h0, h1, w0 + r, lane, a, c);
+        if (p.splits > 1) {
+            float* kp = p.part_o + ((long)part * 2 * pall + prow + w0 + r) * D;
+            float* vp = kp + pall * D;
+            if (lane < D) { kp[lane] = a[0]; vp[lane] = c[0]; }
+            if (D > 64) { kp[lane + 64] = a[1]; vp[lane + 64] = c[1]; }
+            continue;
+        }
         uint16_t* kp = p.dk + b * p.dk_s[0] + hk * p.dk_s[1] + (long)(w0 + r) * p.dk_s[2];
         uint16_t* vp = p.dv + b * p.dv_s[0] + hk * p.dv_s[1] + (long)(w0 + r) * p.dv_s[2];
         if (lane < D) { kp[lane] = f32_to_bf16(a[0] * p.scale); vp[lane] = f32_to_bf16(c[0]); }
@@ -515,7 +537,37 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
     }
 }
 
-template <int D, int AX>
+// adds the head splits of a key row in split order; masked keys' parts are zeros.  4 elements a thread
+template <int D>
+__global__ __launch_bounds__(256) void span_bwd_join(const SpanArgs p) {
+    const long pall = (long)p.B * p.Hk * p.nk, x = (long)blockIdx.x * 256 + threadIdx.x;
+    const long row = x / (D / 4);
+    const int c = (int)(x % (D / 4)) * 4;
+    if (row >= 2 * pall) return;
+    float4 v = *reinterpret_cast<const float4*>(p.part_o + row * D + c);
+    for (int s = 1; s < p.splits; ++s) {
+        const float4 y = *reinterpret_cast<const float4*>(p.part_o + (s * 2 * pall + row) * D + c);
+        v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+    }
+    const bool is_v = row >= pall;
+    const long r = is_v ? row - pall : row;
+    const int key = (int)(r % p.nk), hk = (int)(r / p.nk % p.Hk), b = (int)(r / p.nk / p.Hk);
+    const float f = is_v ? 1.f : p.scale;
+    uint16_t* o = is_v ? p.dv + b * p.dv_s[0] + hk * p.dv_s[1] + (long)key * p.dv_s[2] : p.dk + b * p.dk_s[0] + hk * p.dk_s[1] + (long)key * p.dk_s[2];
+    *reinterpret_cast<uint2*>(o + c) = make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
+}
+
+// Query heads that share a key head go to workgroups of their own, fp32 partial sums joined in order, as far as that fills the card: the smallest divisor of the group
+// that gives 512 workgroups (two per CU), or the whole group.
+int head_splits(const mm_span_attn* a) {
+    const int group = a->heads_q / a->heads_k;
+    const long wgs = (long)a->batch * a->heads_k * ((a->nk + BK - 1) / BK);
+    for (int s = 1; s < group; ++s)
+        if (group % s == 0 && wgs * s >= 512) return s;
+    return group;
+}
+
+template <int D, int AX, bool CAP>
 int launch_bwd(hipStream_t s, const SpanArgs& a) {
     int rc;
     if (a.nq > 0) {
@@ -526,33 +578,40 @@ int launch_bwd(hipStream_t s, const SpanArgs& a) {
         if ((rc = mm_check_launch("span_bwd_hulls"))) return rc;
         constexpr int sm = 2 * (2 * Tile<D, BT>::BYTES + AX * BT * 4) + 64;
         static std::atomic<unsigned long long> lds{0};
-        if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dq<D, AX>), sm, lds))) return rc;
+        if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dq<D, AX, CAP>), sm, lds))) return rc;
         const long total = (long)a.B * a.Hq * ((a.nq + BQ - 1) / BQ);
-        hipLaunchKernelGGL((span_bwd_dq<D, AX>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), sm, s, a);
+        hipLaunchKernelGGL((span_bwd_dq<D, AX, CAP>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), sm, s, a);
         if ((rc = mm_check_launch("span_bwd_dq"))) return rc;
     }
     if (a.nk > 0) {
         constexpr int sm = 2 * (2 * Tile<D, BT>::BYTES + (4 + AX) * BT * 4) + 256 * 4 + 512 * 16 + 16;
         static std::atomic<unsigned long long> lds{0};
-        if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dkv<D, AX>), sm, lds))) return rc;
-        const long total = (long)a.B * a.Hk * ((a.nk + BK - 1) / BK);
-        hipLaunchKernelGGL((span_bwd_dkv<D, AX>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), sm, s, a);
+        if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dkv<D, AX, CAP>), sm, lds))) return rc;
+        const long total = (long)a.B * a.Hk * a.splits * ((a.nk + BK - 1) / BK);
+        hipLaunchKernelGGL((span_bwd_dkv<D, AX, CAP>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), sm, s, a);
         if ((rc = mm_check_launch("span_bwd_dkv"))) return rc;
+        if (a.splits > 1) {
+            const long work = 2L * a.B * a.Hk * a.nk * (D / 4);
+            hipLaunchKernelGGL(span_bwd_join<D>, dim3((unsigned)((work + 255) / 256)), dim3(256), 0, s, a);
+            if ((rc = mm_check_launch("span_bwd_join"))) return rc;
+        }
     }
     return MM_OK;
 }
 
-template <int D>
+template <int D, bool CAP>
 int launch_bwd_axes(hipStream_t s, const SpanArgs& a) {
     switch (a.axes) {
-        case 0: return launch_bwd<D, 0>(s, a);
-        case 1: return launch_bwd<D, 1>(s, a);
-        case 2: return launch_bwd<D, 2>(s, a);
-        default: return launch_bwd<D, 3>(s, a);
+        case 0: return launch_bwd<D, 0, CAP>(s, a);
+        case 1: return launch_bwd<D, 1, CAP>(s, a);
+        case 2: return launch_bwd<D, 2, CAP>(s, a);
+        default: return launch_bwd<D, 3, CAP>(s, a);
     }
 }
+template <int D>
+int launch_bwd_dim(hipStream_t s, const SpanArgs& a) { return a.cap > 0.f ? launch_bwd_axes<D, true>(s, a) : launch_bwd_axes<D, false>(s, a); }
 
-struct BwdLayout { size_t hulls, delta, slopes, bytes; int hull_tiles; long slope_parts; };
+struct BwdLayout { size_t hulls, delta, slopes, parts, bytes; int hull_tiles, splits; long slope_parts; };
 BwdLayout bwd_layout(const mm_span_attn* a) {
     BwdLayout r;
     r.hull_tiles = (a->nq + 31) / 32;
@@ -561,6 +620,9 @@ BwdLayout bwd_layout(const mm_span_attn* a) {
     r.hulls = at; at += (size_t)a->batch * r.hull_tiles * sizeof(int4);
     r.delta = at; at += ((size_t)a->batch * a->heads_q * a->nq * sizeof(float) + 15) / 16 * 16;
     r.slopes = at; at += (size_t)r.slope_parts * a->heads_q * a->axes * sizeof(float);
+    at = (at + 15) / 16 * 16;
+    r.splits = head_splits(a);
+    r.parts = at; at += r.splits > 1 ? (size_t)r.splits * 2 * a->batch * a->heads_k * a->nk * a->dim * sizeof(float) : 0;
     r.bytes = at;
     return r;
 }
@@ -576,8 +638,10 @@ int k_span_attn_bwd(hipStream_t s, const mm_span_attn* a, void* ws) {
     p.hulls = reinterpret_cast<int4*>((char*)ws + l.hulls);
     p.hull_tiles = l.hull_tiles;
     p.delta = reinterpret_cast<float*>((char*)ws + l.delta);
+    p.splits = l.splits;
+    p.part_o = reinterpret_cast<float*>((char*)ws + l.parts);
     p.dsl_part = l.slope_parts ? reinterpret_cast<float*>((char*)ws + l.slopes) : nullptr;
-    const int rc = a->dim == 32 ? launch_bwd_axes<32>(s, p) : (a->dim == 64 ? launch_bwd_axes<64>(s, p) : launch_bwd_axes<128>(s, p));
+    const int rc = a->dim == 32 ? launch_bwd_dim<32>(s, p) : (a->dim == 64 ? launch_bwd_dim<64>(s, p) : launch_bwd_dim<128>(s, p));
     if (rc || !a->slopes || !a->dslopes) return rc;
     return k_colsum(s, p.dsl_part, (int)l.slope_parts, (long)a->heads_q * a->axes, a->dslopes);      // (no rows: zeros)
 }

@@ -61,6 +61,13 @@ __device__ __forceinline__ float both_halves_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// ds_read_b64_tr_b16.  __restrict__: the access gets alias information of its own; without any the compiler takes every LDS-DMA in flight (the NEXT tile's, into the
+// other stage) for a write to it and waits for all of them in the middle of a tile (s_waitcnt vmcnt(0)).  The kernels wait for a tile themselves, before its barrier.
+__device__ __forceinline__ sp_v4i16_t tr_read(const unsigned char* __restrict__ p) {
+    typedef __attribute__((address_space(3))) sp_v4i16_t* lds_v4_t;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4_t)p);
+}
+
 // A tile of ROWS rows x D elements in LDS as [D / 16][ROWS][16] (32-byte rows; 128 bytes between blocks keep the two column blocks of a transposing read on
 // different banks).  ONE image serves both operand forms: rows as they are (ds_read_b128: the wave reads 1 KiB in a row) and transposed (ds_read_b64_tr_b16).  Filled
 // by LDS-DMA, 32 rows x 16 columns per wave instruction; rows at or behind rows_ok are outside the descriptor and come as zeros.
@@ -76,7 +83,7 @@ struct Tile {
 #pragma unroll
         for (int i = 0; i < NB * (ROWS / 32) / NW; ++i) {
             const int idx = i * NW + w, cb = idx % NB, rb = idx / NB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(lds + cb * BS + rb * 1024), 16, v0 + rb * 32 * sb + cb * 32, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)(lds + cb * BS + rb * 1024), 16, v0, rb * 32 * sb + cb * 32, 0, 0);
         }
     }
     // operand over columns 16 cb .. + 15, rows 32 rb .. + 31
@@ -85,10 +92,8 @@ struct Tile {
     }
     // operand over rows 16 s .. + 15 (in the slot order above), columns 32 cd .. + 31
     static __device__ __forceinline__ u32x4_t cols(const unsigned char* lds, int s, int cd, int lane) {
-        typedef __attribute__((address_space(3))) sp_v4i16_t* lds_v4_t;
         const unsigned char* p = lds + (2 * cd + ((lane >> 4) & 1)) * BS + (s * 16 + (lane >> 5) * 4 + ((lane & 15) >> 2)) * 32 + (lane & 3) * 8;
-        const sp_v4i16_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4_t)p), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4_t)(p + 256));
-        const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+        const uint2 x = __builtin_bit_cast(uint2, tr_read(p)), y = __builtin_bit_cast(uint2, tr_read(p + 256));
         return u32x4_t{x.x, x.y, y.x, y.y};
     }
     // rows whose bit is clear become zeros (all threads of the workgroup; the caller's barriers)
