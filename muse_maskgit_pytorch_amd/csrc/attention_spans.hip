@@ -39,61 +39,66 @@ __device__ __forceinline__ void row_again(const SpanArgs& p, int b, int h, int i
     }
 }
 
-// scores of NS 32-key blocks of one tile (raw products in) -> log2 units with cap, bias and mask; returns the lane's largest
-template <int AX, int NS>
-__device__ __forceinline__ float scores(f32x16_t (&s)[NS], float cap, float c1, float c2, const int (&pq)[AX ? AX : 1], const float (&sl)[AX ? AX : 1], const int* pk, int half,
-                                        bool masked, unsigned long long bits) {
-    if (cap > 0.f) {
+// A score passes through three forms.  raw: the product q.k.  y: what the maximum is taken of --
+//     no cap:          raw - sum (slope / scale) |distance|,     score = ka y,       ka = scale log2 e
+//     cap, no bias:    r = 1 / (exp(2 raw scale / cap) + 1),     score = ka y + kb,  ka = -2 cap log2 e, kb = cap log2 e   (cap tanh(x) = cap - 2 cap r: smallest r)
+//     cap and bias:    cap tanh(..) - sum slope |distance|,      score = y           (all in units of log2)
+// and p = exp2(ka y + (kb - m)): one fused multiply-add in front of exp2 whatever the form.
+template <bool CAP, int AX>
+struct Form {
+    static constexpr bool falls = CAP && AX == 0;      // the score falls with y
+    float pre, ka, kb, sl[AX ? AX : 1];
+    __device__ __forceinline__ void init(const SpanArgs& p, int h) {
+        const float c1 = p.scale * SPAN_LOG2E;
+        pre = CAP ? 2.f * c1 / p.cap : 1.f;
+        ka = CAP ? (AX ? 1.f : -2.f * p.cap * SPAN_LOG2E) : c1;
+        kb = CAP && !AX ? p.cap * SPAN_LOG2E : 0.f;
+        c2 = p.cap * SPAN_LOG2E;
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[n][r] = span_tanh(s[n][r], c1) * c2;
-    } else {
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[n][r] *= c1;
+        for (int a = 0; a < AX; ++a) sl[a] = CAP ? p.slopes[h * AX + a] * SPAN_LOG2E : p.slopes[h * AX + a] / p.scale;
     }
-    if constexpr (AX > 0) {
+    float c2;
+    // 4 consecutive keys (pk: their positions, [axis][stride])
+    __device__ __forceinline__ void y4(f32x16_t& s, int r, const int (&pq)[AX ? AX : 1], const int* pk, int stride) const {
+        float v[4] = {s[r], s[r + 1], s[r + 2], s[r + 3]};
+        if constexpr (CAP) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                int4 kp[AX];
-#pragma unroll
-                for (int a = 0; a < AX; ++a) kp[a] = *reinterpret_cast<const int4*>(pk + a * NS * 32 + n * 32 + g * 8 + half * 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int a = 0; a < AX; ++a) {
-                        const int kv = e == 0 ? kp[a].x : (e == 1 ? kp[a].y : (e == 2 ? kp[a].z : kp[a].w));
-                        s[n][g * 4 + e] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - kv)), s[n][g * 4 + e]);
-                    }
+            for (int e = 0; e < 4; ++e) {
+                v[e] = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v[e] * pre) + 1.f);
+                if constexpr (AX > 0) v[e] = __builtin_fmaf(v[e], -2.f * c2, c2);
             }
+        }
+#pragma unroll
+        for (int a = 0; a < AX; ++a) {
+            const int4 k = *reinterpret_cast<const int4*>(pk + a * stride);
+            v[0] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.x)), v[0]);
+            v[1] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.y)), v[1]);
+            v[2] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.z)), v[2]);
+            v[3] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.w)), v[3]);
+        }
+        s[r] = v[0]; s[r + 1] = v[1]; s[r + 2] = v[2]; s[r + 3] = v[3];
     }
-    if (masked) {
-        bits >>= 4 * half;
+    // hidden keys out: w bit 8 (r >> 2) + (r & 3) of block n for register r (already shifted by the half)
+    __device__ __forceinline__ void hide(f32x16_t& s, uint32_t w) const {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            const uint32_t w = (uint32_t)(bits >> (32 * n));
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (!(w & (1u << (8 * (r >> 2) + (r & 3))))) s[n][r] = -INFINITY;
+        for (int r = 0; r < 16; ++r) {
+            const uint32_t t = (uint32_t)((int)(w << (31 - (8 * (r >> 2) + (r & 3)))) >> 31);      // all ones: visible
+            s[r] = __uint_as_float((t & __float_as_uint(s[r])) | (~t & (falls ? 0x7F800000u : 0xFF800000u)));
         }
     }
-    float m = s[0][0];
+    __device__ __forceinline__ float extreme(const f32x16_t& s, float m) const {
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) m = fmaxf(m, s[n][r]);
-    return m;
-}
+        for (int r = 0; r < 16; ++r) m = falls ? fminf(m, s[r]) : fmaxf(m, s[r]);
+        return m;
+    }
+    static __device__ __forceinline__ float worst() { return falls ? INFINITY : -INFINITY; }
+    __device__ __forceinline__ float score(float y) const { return __builtin_fmaf(y, ka, kb); }
+};
 
-// one tile into the running state (m: same in both halves; l: this half's part)
-template <int D, bool F16, int NS>
-__device__ __forceinline__ void soften(f32x16_t (&s)[NS], float tmax, float& m, float& l, f32x16_t (&o)[D / 32], u32x4_t (&pf)[2 * NS]) {
+// the running maximum moves only when some row's grows by more than 2^8: P stays below 2^8, exact enough in 16 bits, and most tiles rescale nothing
+template <int D>
+__device__ __forceinline__ void rescale(float tmax, float& m, float& l, f32x16_t (&o)[D / 32]) {
     tmax = both_halves_max(tmax);
-    // the maximum moves only when some row's grows by more than 2^8: P stays below 2^8, exact enough in 16 bits, and most tiles rescale nothing
     if (__any(tmax > m + 8.f)) {
         const float mn = fmaxf(m, tmax), f = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
@@ -103,24 +108,28 @@ __device__ __forceinline__ void soften(f32x16_t (&s)[NS], float tmax, float& m, 
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[c][r] *= f;
     }
-    float sum = 0.f;
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - m);
-            sum += s[n][r];
-        }
-        // rounding of P to 16 bits: the products with V need it; the sum takes the unrounded values
-        pf[2 * n] = pack_slots<F16>(s[n], 0);
-        pf[2 * n + 1] = pack_slots<F16>(s[n], 1);
-    }
-    l += sum;
 }
 
-template <int D, bool F16, int AX>
+// 8 probabilities of a lane -> an operand.  Rounding of P to 16 bits: the product with V needs it; the sum takes the unrounded values
+template <bool F16>
+__device__ __forceinline__ u32x4_t probs(const f32x16_t& s, int x, float ka, float kbm, float& l) {
+    float q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * x + e], ka, kbm));
+    l += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+    return u32x4_t{pack2<F16>(q[0], q[1]), pack2<F16>(q[2], q[3]), pack2<F16>(q[4], q[5]), pack2<F16>(q[6], q[7])};
+}
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+// AHEAD (128 wide heads): the product of tile it + 1's keys with the queries is issued between the instructions that turn tile it's scores into probabilities
+// (independent work for the matrix and the vector pipe from one wave); K then runs one tile ahead of V in the two stages.  It needs a second set of scores: narrower
+// heads lose their third wave per SIMD to it and are slower (16300 rows of packed images, 64 wide, two axes: 81 against 66 us; 128 wide, capped: 138 against 155).
+template <int D, bool F16, int AX, bool CAP>
 __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
     typedef Tile<D, KT> T;
+    constexpr bool AHEAD = D == 128;
     extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
     constexpr int POS = AX * KT * 4, STAGE = 2 * T::BYTES + POS;
     int* red = reinterpret_cast<int*>(smem + 2 * STAGE);
@@ -153,12 +162,11 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) qf[c] = *reinterpret_cast<const u32x4_t*>(qp + c * 16);
     }
-    float sl[AX ? AX : 1]; int pq[AX ? AX : 1];
+    int pq[AX ? AX : 1];
 #pragma unroll
-    for (int a = 0; a < AX; ++a) {
-        sl[a] = p.slopes[h * AX + a] * SPAN_LOG2E;
-        pq[a] = ok ? p.pos_q[b * p.pq_sb + (long)i * AX + a] : 0;
-    }
+    for (int a = 0; a < AX; ++a) pq[a] = ok ? p.pos_q[b * p.pq_sb + (long)i * AX + a] : 0;
+    Form<CAP, AX> F;
+    F.init(p, h);
     __syncthreads();
     const int k0 = __builtin_amdgcn_readfirstlane(min(min(red[0], red[1]), min(red[2], red[3])));
     const int k1 = __builtin_amdgcn_readfirstlane(max(max(red[4], red[5]), max(red[6], red[7])));
@@ -168,69 +176,138 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
     const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1];
     const uint8_t* km = p.kmask ? p.kmask + b * p.km_sb : nullptr;
     const int* pkp = AX ? p.pos_k + b * p.pk_sb : nullptr;
-    const bool capped = p.cap > 0.f;
-    const float c1 = capped ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E, c2 = p.cap * SPAN_LOG2E;
-
-#define SPAN_ISSUE(it_)                                                                                                \
-    {                                                                                                                  \
-        const int t0_ = k0 + (it_) * KT;                                                                               \
-        unsigned char* st_ = smem + ((it_) & 1) * STAGE;                                                               \
-        T::template fill<4>(st_, kp + (long)t0_ * p.k_s[2], min(KT, k1 - t0_), (int)p.k_s[2], w, lane);                \
-        T::template fill<4>(st_ + T::BYTES, vp + (long)t0_ * p.v_s[2], min(KT, k1 - t0_), (int)p.v_s[2], w, lane);     \
-    }
-#define SPAN_POS_LOAD(it_) \
-    if constexpr (AX > 0) { if (t < KT * AX) { const int key_ = k0 + (it_) * KT + t / AX; posv = key_ < k1 ? pkp[(long)key_ * AX + t % AX] : 0; } }
-#define SPAN_POS_STORE(it_) \
-    if constexpr (AX > 0) { if (t < KT * AX) reinterpret_cast<int*>(smem + ((it_) & 1) * STAGE + 2 * T::BYTES)[(t % AX) * KT + t / AX] = posv; }
 
     float m = SPAN_LOW, l = 0.f;
-    f32x16_t o[D / 32];
+    f32x16_t o[D / 32], sa[2], sb[2];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[c][r] = 0.f;
     int posv = 0;
-    if (nt > 0) {
-        SPAN_ISSUE(0);
-        SPAN_POS_LOAD(0);
-        SPAN_POS_STORE(0);
-    }
-    for (int it = 0; it < nt; ++it) {
+    const auto fill_k = [&](int it) {
         const int t0 = k0 + it * KT;
-        unsigned char* Ks = smem + (it & 1) * STAGE;
-        unsigned char* Vs = Ks + T::BYTES;
+        T::template fill<4>(smem + (it & 1) * STAGE, kp + (long)t0 * p.k_s[2], min(KT, k1 - t0), (int)p.k_s[2], w, lane);
+    };
+    const auto fill_v = [&](int it) {
+        const int t0 = k0 + it * KT;
+        T::template fill<4>(smem + (it & 1) * STAGE + T::BYTES, vp + (long)t0 * p.v_s[2], min(KT, k1 - t0), (int)p.v_s[2], w, lane);
+    };
+    const auto pos_load = [&](int it) {
+        if constexpr (AX > 0) {
+            if (t < KT * AX) { const int key = k0 + it * KT + t / AX; posv = key < k1 ? pkp[(long)key * AX + t % AX] : 0; }
+        }
+    };
+    const auto pos_store = [&](int it) {
+        if constexpr (AX > 0) {
+            if (t < KT * AX) reinterpret_cast<int*>(smem + (it & 1) * STAGE + 2 * T::BYTES)[(t % AX) * KT + t / AX] = posv;
+        }
+    };
+    const auto sees = [&](int it) { return it < nt && __any(lo < k0 + it * KT + KT && hi > k0 + it * KT); };
+    constexpr int NC = D / 16, E = 8 / NC;      // product steps; groups of 4 scores beside each
+    // scores of the next tile (into sn) and y of this tile's (s), together or one of them
+    const auto mix = [&](int it, f32x16_t (&s)[2], f32x16_t (&sn)[2], auto with_next, auto with_this) {
+        const unsigned char* Kn = smem + ((it + 1) & 1) * STAGE;
+        int pos = (it & 1) * STAGE + 2 * T::BYTES + half * 16;
+        u32x4_t f0, f1;
+        if constexpr (with_next.value) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sn[0][r] = sn[1][r] = 0.f;
+            f0 = T::rows(Kn, 0, 0, lane); f1 = T::rows(Kn, 0, 1, lane);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if constexpr (with_next.value) {
+                const u32x4_t a0 = f0, a1 = f1;
+                if (c + 1 < NC) { f0 = T::rows(Kn, c + 1, 0, lane); f1 = T::rows(Kn, c + 1, 1, lane); }
+                sn[0] = mfma32<F16>(a0, qf[c], sn[0]);
+                sn[1] = mfma32<F16>(a1, qf[c], sn[1]);
+            }
+            if constexpr (with_this.value && (CAP || AX > 0)) {
+#pragma unroll
+                for (int x = 0; x < E; ++x) {
+                    const int g = c * E + x;
+                    F.y4(s[g >> 2], (g & 3) * 4, pq, reinterpret_cast<const int*>(smem + pos) + (g >> 2) * 32 + (g & 3) * 8, KT);
+                    // y of these four now, the next group's positions behind it: left alone, the compiler moves three of the four behind the branch on the mask and keeps
+                    // the positions of all 64 keys until then (32 registers an axis: a wave per SIMD)
+                    if constexpr (AX > 0) {
+                        f32x16_t& y = s[g >> 2];
+                        const int r = (g & 3) * 4;
+                        float y0 = y[r], y1 = y[r + 1], y2 = y[r + 2], y3 = y[r + 3];
+                        asm volatile("" : "+v"(pos), "+v"(y0), "+v"(y1), "+v"(y2), "+v"(y3));
+                        y[r] = y0; y[r + 1] = y1; y[r + 2] = y2; y[r + 3] = y3;
+                    }
+                }
+            }
+        }
+    };
+    const auto step = [&](int it, f32x16_t (&s)[2], f32x16_t (&sn)[2]) {
+        const int t0 = k0 + it * KT;
+        unsigned char* Vs = smem + (it & 1) * STAGE + T::BYTES;
         unsigned long long keep = ~0ull;
         if (km) keep = __ballot(t0 + lane < k1 && km[t0 + lane]);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();      // this tile has landed for every wave, and every wave is done with the other stage
-        if (it + 1 < nt) { SPAN_ISSUE(it + 1); SPAN_POS_LOAD(it + 1); }
+        __syncthreads();      // V of tile it and K of tile it (+ 1: AHEAD) have landed for every wave, and every wave is done with what the fills below write over
+        if (it + 1 < nt) {
+            if constexpr (!AHEAD) fill_k(it + 1);
+            fill_v(it + 1);
+            pos_load(it + 1);
+        }
+        if (AHEAD && it + 2 < nt) fill_k(it + 2);
         if (keep != ~0ull) {
             T::clear_rows(Vs, keep, t, 256);
             __syncthreads();
         }
-        if (__any(lo < t0 + KT && hi > t0)) {
-            f32x16_t s[2];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-                s[0] = mfma32<F16>(T::rows(Ks, c, 0, lane), qf[c], s[0]);
-                s[1] = mfma32<F16>(T::rows(Ks, c, 1, lane), qf[c], s[1]);
-            }
-            const bool masked = keep != ~0ull || !__all(lo <= t0 && hi >= t0 + KT);
-            const float tmax = scores<AX, 2>(s, p.cap, c1, c2, pq, sl, reinterpret_cast<const int*>(Ks + 2 * T::BYTES), half, masked, masked ? bit_range(lo - t0, hi - t0) & keep : 0ull);
-            u32x4_t pf[4];
-            soften<D, F16, 2>(s, tmax, m, l, o, pf);
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) o[c] = mfma32<F16>(T::cols(Vs, ks, c, lane), pf[ks], o[c]);
+        const bool now = sees(it);
+        if constexpr (AHEAD) {
+            const bool next = sees(it + 1);
+            if (now && next) mix(it, s, sn, Yes(), Yes());
+            else if (next) mix(it, s, sn, Yes(), No());
+            else if (now) mix(it, s, sn, No(), Yes());
+        } else if (now) {
+            mix(it - 1, s, s, Yes(), No());
+            mix(it, s, s, No(), Yes());
         }
-        if (it + 1 < nt) SPAN_POS_STORE(it + 1);
+        if (now) {
+            if (keep != ~0ull || !__all(lo <= t0 && hi >= t0 + KT)) {
+                const unsigned long long bits = (bit_range(lo - t0, hi - t0) & keep) >> (4 * half);
+                F.hide(s[0], (uint32_t)bits);
+                F.hide(s[1], (uint32_t)(bits >> 32));
+            }
+            rescale<D>(F.score(F.extreme(s[1], F.extreme(s[0], Form<CAP, AX>::worst()))), m, l, o);
+            const float kbm = F.kb - m;
+            u32x4_t pf = probs<F16>(s[0], 0, F.ka, kbm, l);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                u32x4_t vf[D / 32];
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) vf[c] = T::cols(Vs, ks, c, lane);
+                const u32x4_t pc = pf;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) o[c] = mfma32<F16>(vf[c], pc, o[c]);
+                if (ks < 3) pf = probs<F16>(s[(ks + 1) >> 1], (ks + 1) & 1, F.ka, kbm, l);
+            }
+        }
+        if (it + 1 < nt) pos_store(it + 1);
+    };
+    if (nt > 0) {
+        fill_k(0);
+        pos_load(0);
+        pos_store(0);
+        if constexpr (AHEAD) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            fill_v(0);
+            if (nt > 1) fill_k(1);
+            if (sees(0)) mix(-1, sb, sa, Yes(), No());
+            for (int it = 0; it < nt; it += 2) {
+                step(it, sa, sb);
+                if (it + 1 < nt) step(it + 1, sb, sa);
+            }
+        } else {
+            fill_v(0);
+            for (int it = 0; it < nt; ++it) step(it, sa, sa);
+        }
     }
-#undef SPAN_ISSUE
-#undef SPAN_POS_LOAD
-#undef SPAN_POS_STORE
 
     l = both_halves_sum(l);
     const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -266,7 +343,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
     }
 }
 
-template <int D, bool F16, int AX>
+template <int D, bool F16, int AX, bool CAP>
 __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
     typedef Tile<D, 32> T;
     constexpr int POS = AX * 32 * 4, STAGE = 2 * T::BYTES + POS, OS = D + 4;      // OS: row of the joined output in floats
@@ -305,18 +382,15 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) qf[c] = *reinterpret_cast<const u32x4_t*>(qp + c * 16);
     }
-    float sl[AX ? AX : 1]; int pq[AX ? AX : 1];
+    int pq[AX ? AX : 1];
 #pragma unroll
-    for (int a = 0; a < AX; ++a) {
-        sl[a] = p.slopes[h * AX + a] * SPAN_LOG2E;
-        pq[a] = p.pos_q[b * p.pq_sb + (long)i * AX + a];
-    }
+    for (int a = 0; a < AX; ++a) pq[a] = p.pos_q[b * p.pq_sb + (long)i * AX + a];
+    Form<CAP, AX> F;
+    F.init(p, h);
     const uint16_t* kp = p.k + b * p.k_s[0] + hk * p.k_s[1];
     const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1];
     const uint8_t* km = p.kmask ? p.kmask + b * p.km_sb : nullptr;
     const int* pkp = AX ? p.pos_k + b * p.pk_sb : nullptr;
-    const bool capped = p.cap > 0.f;
-    const float c1 = capped ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E, c2 = p.cap * SPAN_LOG2E;
     unsigned char* mine = smem + w * 2 * STAGE;
 
     float m = SPAN_LOW, l = 0.f;
@@ -351,19 +425,23 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
         if (tt + 4 < nt) SPAN_ISSUE(tt + 4, st ^ 1);
         if (keep != 0xFFFFFFFFu) T::clear_rows(Vs, keep, lane, 64);
         __builtin_amdgcn_wave_barrier();
-        f32x16_t s[1];
+        f32x16_t s;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) s[0] = mfma32<F16>(T::rows(Ks, c, 0, lane), qf[c], s[0]);
-        const bool masked = keep != 0xFFFFFFFFu || !__all(lo <= t0 && hi >= t0 + 32);
-        const float tmax = scores<AX, 1>(s, p.cap, c1, c2, pq, sl, pks, half, masked, masked ? bit_range(lo - t0, hi - t0) & (unsigned long long)keep : 0ull);
-        u32x4_t pf[2];
-        soften<D, F16, 1>(s, tmax, m, l, o, pf);
+        for (int c = 0; c < D / 16; ++c) s = mfma32<F16>(T::rows(Ks, c, 0, lane), qf[c], s);
+        if constexpr (CAP || AX > 0)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+            for (int g = 0; g < 4; ++g) F.y4(s, g * 4, pq, pks + g * 8 + half * 4, 32);
+        if (keep != 0xFFFFFFFFu || !__all(lo <= t0 && hi >= t0 + 32)) F.hide(s, (uint32_t)((bit_range(lo - t0, hi - t0) & (unsigned long long)keep) >> (4 * half)));
+        rescale<D>(F.score(F.extreme(s, Form<CAP, AX>::worst())), m, l, o);
+        const float kbm = F.kb - m;
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) o[c] = mfma32<F16>(T::cols(Vs, ks, c, lane), pf[ks], o[c]);
+        for (int ks = 0; ks < 2; ++ks) {
+            const u32x4_t pf = probs<F16>(s, ks, F.ka, kbm, l);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) o[c] = mfma32<F16>(T::cols(Vs, ks, c, lane), pf, o[c]);
+        }
     }
 #undef SPAN_ISSUE
     // ---- join the four waves: common maximum, then the sums in wave order
@@ -492,22 +570,22 @@ SpanPlan span_plan(const mm_span_attn* a) {
     return r;
 }
 
-template <int D, bool F16, int AX>
+template <int D, bool F16, int AX, bool CAP>
 int launch_fwd(hipStream_t s, const SpanArgs& a, const SpanPlan& pl) {
     if (!pl.narrow) {
         constexpr int sm = 2 * (2 * Tile<D, KT>::BYTES + AX * KT * 4) + 64;
         static std::atomic<unsigned long long> lds{0};
-        if (const int rc = span_allow_lds(reinterpret_cast<const void*>(span_attn_wide<D, F16, AX>), sm, lds)) return rc;
+        if (const int rc = span_allow_lds(reinterpret_cast<const void*>(span_attn_wide<D, F16, AX, CAP>), sm, lds)) return rc;
         const int tiles = (a.nq + WQ - 1) / WQ;
         const long total = (long)a.B * a.Hq * tiles, per = (total + 7) / 8;
-        hipLaunchKernelGGL((span_attn_wide<D, F16, AX>), dim3((unsigned)(per * 8)), dim3(256), sm, s, a);
+        hipLaunchKernelGGL((span_attn_wide<D, F16, AX, CAP>), dim3((unsigned)(per * 8)), dim3(256), sm, s, a);
         return mm_check_launch("span_attn_wide");
     }
     constexpr int st = 8 * (2 * Tile<D, 32>::BYTES + AX * 32 * 4), jo = 4 * 32 * (D + 4) * 4;
     constexpr int sm = (st > jo ? st : jo) + 4 * 32 * 2 * 4;
     static std::atomic<unsigned long long> lds{0};
-    if (const int rc = span_allow_lds(reinterpret_cast<const void*>(span_attn_narrow<D, F16, AX>), sm, lds)) return rc;
-    hipLaunchKernelGGL((span_attn_narrow<D, F16, AX>), dim3((unsigned)(a.B * a.Hk * pl.row_tiles), pl.splits), dim3(256), sm, s, a);
+    if (const int rc = span_allow_lds(reinterpret_cast<const void*>(span_attn_narrow<D, F16, AX, CAP>), sm, lds)) return rc;
+    hipLaunchKernelGGL((span_attn_narrow<D, F16, AX, CAP>), dim3((unsigned)(a.B * a.Hk * pl.row_tiles), pl.splits), dim3(256), sm, s, a);
     const int rc = mm_check_launch("span_attn_narrow");
     if (rc || pl.splits == 1) return rc;
     const long rows = (long)a.B * a.Hk * pl.row_tiles * 32, blocks = (rows + 256 / (D / 4) - 1) / (256 / (D / 4));
@@ -515,14 +593,19 @@ int launch_fwd(hipStream_t s, const SpanArgs& a, const SpanPlan& pl) {
     return mm_check_launch("span_attn_join");
 }
 
-template <int D, bool F16>
+template <int D, bool F16, bool CAP>
 int launch_axes(hipStream_t s, const SpanArgs& a, const SpanPlan& pl) {
     switch (a.axes) {
-        case 0: return launch_fwd<D, F16, 0>(s, a, pl);
-        case 1: return launch_fwd<D, F16, 1>(s, a, pl);
-        case 2: return launch_fwd<D, F16, 2>(s, a, pl);
-        default: return launch_fwd<D, F16, 3>(s, a, pl);
+        case 0: return launch_fwd<D, F16, 0, CAP>(s, a, pl);
+        case 1: return launch_fwd<D, F16, 1, CAP>(s, a, pl);
+        case 2: return launch_fwd<D, F16, 2, CAP>(s, a, pl);
+        default: return launch_fwd<D, F16, 3, CAP>(s, a, pl);
     }
+}
+template <int D>
+int launch_dim(hipStream_t s, const SpanArgs& a, const SpanPlan& pl, bool f16) {
+    if (a.cap > 0.f) return f16 ? launch_axes<D, true, true>(s, a, pl) : launch_axes<D, false, true>(s, a, pl);
+    return f16 ? launch_axes<D, true, false>(s, a, pl) : launch_axes<D, false, false>(s, a, pl);
 }
 
 }  // namespace
@@ -556,7 +639,7 @@ int k_span_attn(hipStream_t s, const mm_span_attn* a, void* ws) {
     p.part_o = (float*)ws;
     p.part_ml = p.part_o ? p.part_o + (size_t)pl.splits * a->batch * a->heads_k * pl.row_tiles * 32 * a->dim : nullptr;
     const bool f16 = a->dtype == MM_DT_F16;
-    if (a->dim == 32) return f16 ? launch_axes<32, true>(s, p, pl) : launch_axes<32, false>(s, p, pl);
-    if (a->dim == 64) return f16 ? launch_axes<64, true>(s, p, pl) : launch_axes<64, false>(s, p, pl);
-    return f16 ? launch_axes<128, true>(s, p, pl) : launch_axes<128, false>(s, p, pl);
+    if (a->dim == 32) return launch_dim<32>(s, p, pl, f16);
+    if (a->dim == 64) return launch_dim<64>(s, p, pl, f16);
+    return launch_dim<128>(s, p, pl, f16);
 }

@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
                         for (int a = 0; a < AX; ++a) ds_sl[a] = __builtin_fmaf(d, far[a], ds_sl[a]);
                         s[r] = CAP ? d * slope : d;
                     }
-                    __builtin_amdgcn_sched_barrier(0);      // (four scores at a time: all sixteen at once cost 60 registers more, and the second workgroup of a CU)
+                    asm volatile("" ::: "memory");      // (four scores at a time: all sixteen at once cost 60 registers more, and the second workgroup of a CU)
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -465,7 +465,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
                         s[r] = pr;
                         g[r] = CAP ? d * slope : d;
                     }
-                    __builtin_amdgcn_sched_barrier(0);
+                    asm volatile("" ::: "memory");
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
