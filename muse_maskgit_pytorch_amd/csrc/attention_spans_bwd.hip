@@ -12,6 +12,8 @@
 #include "span_attn.h"
 
 void span_args(const mm_span_attn* a, SpanArgs& p);
+long span_order_tiles(const mm_span_attn* a);
+int span_order_run(hipStream_t s, const mm_span_attn* a, int32_t* order);
 
 namespace {
 
@@ -143,10 +145,10 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
     int* red = reinterpret_cast<int*>(smem + 2 * STAGE);
     const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int tiles = (p.nq + BQ - 1) / BQ, total = p.B * p.Hq * tiles, per = (total + 7) / 8;
-    const int item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);      // (as the forward's: a contiguous part per XCD)
-    if ((int)(blockIdx.x >> 3) >= per || item >= total) return;
-    const int tile = tiles - 1 - item % tiles, h = (item / tiles) % p.Hq, b = item / tiles / p.Hq, hk = h / (p.Hq / p.Hk);
+    const int tiles = (p.nq + BQ - 1) / BQ;
+    int rt, h;
+    if (!span_item(p.order, p.Hq, p.B * tiles, rt, h)) return;
+    const int tile = rt % tiles, b = rt / tiles, hk = h / (p.Hq / p.Hk);
     const int i = tile * BQ + w * 32 + (lane & 31);
     const bool ok = i < p.nq;
     int lo = 0, hi = 0;
@@ -579,8 +581,7 @@ int launch_bwd(hipStream_t s, const SpanArgs& a) {
         constexpr int sm = 2 * (2 * Tile<D, BT>::BYTES + AX * BT * 4) + 64;
         static std::atomic<unsigned long long> lds{0};
         if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dq<D, AX, CAP>), sm, lds))) return rc;
-        const long total = (long)a.B * a.Hq * ((a.nq + BQ - 1) / BQ);
-        hipLaunchKernelGGL((span_bwd_dq<D, AX, CAP>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), sm, s, a);
+        hipLaunchKernelGGL((span_bwd_dq<D, AX, CAP>), dim3((unsigned)(a.B * a.Hq * ((a.nq + BQ - 1) / BQ))), dim3(256), sm, s, a);
         if ((rc = mm_check_launch("span_bwd_dq"))) return rc;
     }
     if (a.nk > 0) {
@@ -611,7 +612,7 @@ int launch_bwd_axes(hipStream_t s, const SpanArgs& a) {
 template <int D>
 int launch_bwd_dim(hipStream_t s, const SpanArgs& a) { return a.cap > 0.f ? launch_bwd_axes<D, true>(s, a) : launch_bwd_axes<D, false>(s, a); }
 
-struct BwdLayout { size_t hulls, delta, slopes, parts, bytes; int hull_tiles, splits; long slope_parts; };
+struct BwdLayout { size_t hulls, delta, order, slopes, parts, bytes; int hull_tiles, splits; long slope_parts; };
 BwdLayout bwd_layout(const mm_span_attn* a) {
     BwdLayout r;
     r.hull_tiles = (a->nq + 31) / 32;
@@ -619,6 +620,7 @@ BwdLayout bwd_layout(const mm_span_attn* a) {
     size_t at = 0;
     r.hulls = at; at += (size_t)a->batch * r.hull_tiles * sizeof(int4);
     r.delta = at; at += ((size_t)a->batch * a->heads_q * a->nq * sizeof(float) + 15) / 16 * 16;
+    r.order = at; at += span_order_tiles(a) * sizeof(int32_t);
     r.slopes = at; at += (size_t)r.slope_parts * a->heads_q * a->axes * sizeof(float);
     at = (at + 15) / 16 * 16;
     r.splits = head_splits(a);
@@ -639,6 +641,10 @@ int k_span_attn_bwd(hipStream_t s, const mm_span_attn* a, void* ws) {
     p.hull_tiles = l.hull_tiles;
     p.delta = reinterpret_cast<float*>((char*)ws + l.delta);
     p.splits = l.splits;
+    if (span_order_tiles(a)) {
+        p.order = reinterpret_cast<int32_t*>((char*)ws + l.order);
+        if (const int rc = span_order_run(s, a, reinterpret_cast<int32_t*>((char*)ws + l.order))) return rc;
+    }
     p.part_o = reinterpret_cast<float*>((char*)ws + l.parts);
     p.dsl_part = l.slope_parts ? reinterpret_cast<float*>((char*)ws + l.slopes) : nullptr;
     const int rc = a->dim == 32 ? launch_bwd_dim<32>(s, p) : (a->dim == 64 ? launch_bwd_dim<64>(s, p) : launch_bwd_dim<128>(s, p));

@@ -16,6 +16,7 @@ struct SpanArgs {
     long q_s[3], k_s[3], v_s[3], o_s[3];
     int B, Hq, Hk, nq, nk, axes;
     float scale, cap;
+    const int32_t* order;      // [B * tiles] tiles of 128 rows, the longest first (NULL: as they come, last first)
     // forward, keys split over workgroups
     int splits, row_tiles; float* part_o; float* part_ml;
     // backward
@@ -104,6 +105,20 @@ struct Tile {
         }
     }
 };
+
+// Which (tile, head) a workgroup takes.  Workgroups go to the 8 XCDs in turn: with a multiple of 8 heads each XCD keeps its own heads (their keys are read into one
+// L2), neighbours among them; otherwise heads in turn.  Tiles in the order of `order`, heads innermost, so the long ones of every head start first.
+__device__ __forceinline__ bool span_item(const int32_t* order, int heads, int rows, int& row_tile, int& head) {      // rows: tiles over the batch
+    const unsigned id = blockIdx.x;
+    int rank;
+    if (heads % 8 == 0) {
+        const unsigned own = heads / 8, slot = id >> 3;
+        rank = slot / own; head = (id & 7) * own + slot % own;
+    } else { rank = id / heads; head = id % heads; }
+    if (rank >= rows) return false;
+    row_tile = order ? order[rank] : rows - 1 - rank;
+    return true;
+}
 
 // bits a .. e - 1 of 64, both clamped
 __device__ __forceinline__ unsigned long long bit_range(int a, int e) {
