@@ -70,7 +70,7 @@ struct Form {
         }
 #pragma unroll
         for (int a = 0; a < AX; ++a) {
-            const int4 k = *reinterpret_cast<const int4*>(pk + a * stride);
+            const i32x4_t k = lds_i4(pk + a * stride);
             v[0] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.x)), v[0]);
             v[1] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.y)), v[1]);
             v[2] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.z)), v[2]);

@@ -235,9 +235,9 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
                 const uint32_t wb = (uint32_t)(bits >> (32 * n));
 #pragma unroll
                 for (int g4 = 0; g4 < 4; ++g4) {
-                    int4 kq[AX ? AX : 1];
+                    i32x4_t kq[AX ? AX : 1];
 #pragma unroll
-                    for (int a = 0; a < AX; ++a) kq[a] = *reinterpret_cast<const int4*>(pks + a * BT + n * 32 + g4 * 8 + half * 4);
+                    for (int a = 0; a < AX; ++a) kq[a] = lds_i4(pks + a * BT + n * 32 + g4 * 8 + half * 4);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = g4 * 4 + e;
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
                         else x *= c1;
 #pragma unroll
                         for (int a = 0; a < AX; ++a) {
-                            const int kv = e == 0 ? kq[a].x : (e == 1 ? kq[a].y : (e == 2 ? kq[a].z : kq[a].w));
+                            const int kv = kq[a][e];
                             far[a] = fabsf((float)(pq[a] - kv));
                             x = __builtin_fmaf(-sl[a], far[a], x);
                         }
@@ -313,18 +313,54 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
     }
 }
 
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+// What turns a raw product q.k into p and into the factor of ds (compare Form in attention_spans.hip: one fused multiply-add in front of exp2):
+//     p = exp2(ka y - lse'),   ds = p (dout.v - delta) w
+//   no cap:  y = raw - sum (slope / scale) |distance|,  ka = scale log2 e,                          lse' = lse log2 e,        w = 1
+//   cap:     r = 1 / (exp(2 raw scale / cap) + 1),      tanh = 1 - 2 r,  1 - tanh^2 = 4 r (1 - r),  w = r (1 - r), the 4 in the factor at the end
+//            without a bias y = r, ka = -2 cap log2 e, lse' = lse log2 e - cap log2 e;  with one y = cap log2 e (1 - 2 r) - sum slope log2 e |distance|, ka = 1
+template <bool CAP, int AX>
+struct BwdForm {
+    float pre, ka, kb, c2, end, per;      // per: units of y in one of a slope
+    __device__ __forceinline__ void init(const SpanArgs& p) {
+        const float c1 = p.scale * SPAN_LOG2E;
+        pre = CAP ? 2.f * c1 / p.cap : 1.f;
+        c2 = p.cap * SPAN_LOG2E;
+        ka = CAP ? (AX ? 1.f : -2.f * c2) : c1;
+        kb = CAP && !AX ? c2 : 0.f;
+        end = CAP ? 4.f * p.scale : p.scale;
+        per = CAP ? SPAN_LOG2E : 1.f / p.scale;
+    }
+    // raw -> y (in front of the bias); w: factor of ds
+    __device__ __forceinline__ float y(float raw, float& w) const {
+        w = 1.f;
+        if constexpr (!CAP) return raw;
+        const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(raw * pre) + 1.f);
+        w = __builtin_fmaf(-r, r, r);
+        return AX ? __builtin_fmaf(r, -2.f * c2, c2) : r;
+    }
+};
+
+// 128 keys of a key head against the query tiles that see them: a wave holds 32 keys as operands (K, V) and their gradients as accumulators.
+// ROLES (128 wide heads): 8 waves, the first four take dV, the others dK of the same keys -- both gradients and both operands are 192 registers, which leaves one wave
+// per SIMD and every latency in the open (942 us for 2 x 16 heads of 4096 x 4096, the matrix pipe busy a quarter of the time); S is computed in both for it, 5 products
+// for 4.  Narrower heads take both gradients in one wave, two or three of which fit a SIMD.
 template <int D, int AX, bool CAP>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const SpanArgs p) {
+__global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bwd_dkv(const SpanArgs p) {
     typedef Tile<D, BT> T;
+    constexpr bool ROLES = D == 128;
+    constexpr int NW = ROLES ? 8 : 4, NT = NW * 64;
     extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
-    constexpr int ROWB = (4 + AX) * BT * 4, STAGE = 2 * T::BYTES + ROWB;      // Q, dO, then per row: lse (log2 units), delta, lo, hi, positions
+    constexpr int ROWB = (4 + AX) * BT * 4, STAGE = 2 * T::BYTES + ROWB;      // Q, dO, then per row: lse', delta, lo, hi, positions
     int* list = reinterpret_cast<int*>(smem + 2 * STAGE);                     // [256] query tiles
     int4* hull = reinterpret_cast<int4*>(list + 256);                         // [256][2] bounds of their two 32-row halves
     int* cnt = reinterpret_cast<int*>(hull + 512);                            // [4]
     const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
-    const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6), w = ROLES ? wave & 3 : wave;
     const int tiles = (p.nk + BK - 1) / BK, total = p.B * p.Hk * p.splits * tiles, per = (total + 7) / 8;
-    const int item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    const int item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);      // (a contiguous part of (row, key head, split, tile) per XCD)
     if ((int)(blockIdx.x >> 3) >= per || item >= total) return;
     const int tile = item % tiles, part = (item / tiles) % p.splits, hk = (item / tiles / p.splits) % p.Hk, b = item / tiles / p.splits / p.Hk;
     const int heads = p.Hq / p.Hk / p.splits, h0 = (hk * p.splits + part) * heads, h1 = h0 + heads;      // the query heads of this workgroup
@@ -332,211 +368,246 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void span_bwd_dkv(const Span
     const int key = w0 + (lane & 31);
     const bool live = key < p.nk && (!p.kmask || p.kmask[b * p.km_sb + key]);      // a key that is not there or masked: zeros, no weight
     const bool all_live = __all(live);
-    u32x4_t kf[D / 16], vf[D / 16];
-    {
-        const uint16_t* kp = p.k + b * p.k_s[0] + hk * p.k_s[1] + (long)(live ? key : 0) * p.k_s[2] + half * 8;
-        const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1] + (long)(live ? key : 0) * p.v_s[2] + half * 8;
-        const u32x4_t z = {0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-            const u32x4_t x = *reinterpret_cast<const u32x4_t*>(kp + c * 16), y = *reinterpret_cast<const u32x4_t*>(vp + c * 16);
-            kf[c] = live ? x : z; vf[c] = live ? y : z;
-        }
-    }
+    const int mkey = live ? key : -1;      // (no span holds key -1)
     int pk[AX ? AX : 1];
 #pragma unroll
     for (int a = 0; a < AX; ++a) pk[a] = key < p.nk ? p.pos_k[b * p.pk_sb + (long)key * AX + a] : 0;
-    const float c1 = CAP ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E, c2 = p.cap * SPAN_LOG2E;
-    f32x16_t dk[D / 32], dv[D / 32];
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dk[c][r] = dv[c][r] = 0.f;
+    BwdForm<CAP, AX> F;
+    F.init(p);
 
     const int qtiles = (p.nq + BT - 1) / BT;
+    // the tile being fetched: entry f_at of the list, head f_h, stage f_st; its rows' numbers (lane = row of the 64, every wave the same; wave 0 writes them to LDS)
     float lsev = 0.f, delv = 0.f;
     int2 spv = make_int2(0, 0);
     int posv[AX ? AX : 1];
-    // the tile being fetched: entry f_at of the list, head f_h (its rows: lane = row of the 64, every wave the same; wave 0 writes them to LDS)
-    int f_at = 0, f_h = h0, f_stage = 0;
-    const uint16_t *f_q = p.q + b * p.q_s[0] + f_h * p.q_s[1], *f_g = p.dout + b * p.do_s[0] + f_h * p.do_s[1];
-#define SPAN_ISSUE()                                                                                                              \
-    {                                                                                                                             \
-        unsigned char* st_ = smem + f_stage * STAGE;                                                                              \
-        const int q0_ = __builtin_amdgcn_readfirstlane(list[f_at]) * BT, ok_ = min(BT, p.nq - q0_);                               \
-        T::template fill<4>(st_, f_q + (long)q0_ * p.q_s[2], ok_, (int)p.q_s[2], w, lane);                                        \
-        T::template fill<4>(st_ + T::BYTES, f_g + (long)q0_ * p.do_s[2], ok_, (int)p.do_s[2], w, lane);                           \
-        const int i_ = q0_ + lane;                                                                                                \
-        spv = make_int2(0, 0); lsev = 0.f; delv = 0.f;                                                                            \
-        if (i_ < p.nq) {                                                                                                          \
-            const long row_ = ((long)b * p.Hq + f_h) * p.nq + i_;                                                                 \
-            spv = row_span(p, b, f_h, i_);                                                                                        \
-            lsev = p.lse[row_] * SPAN_LOG2E; delv = p.delta[row_];                                                                \
-            _Pragma("unroll") for (int a = 0; a < AX; ++a) posv[a] = p.pos_q[b * p.pq_sb + (long)i_ * AX + a];                    \
-        }                                                                                                                         \
-    }
-#define SPAN_ROW_STORE()                                                                                     \
-    if (w == 0) {                                                                                            \
-        float* rw_ = reinterpret_cast<float*>(smem + f_stage * STAGE + 2 * T::BYTES);                        \
-        rw_[lane] = lsev; rw_[BT + lane] = delv;                                                             \
-        reinterpret_cast<int*>(rw_)[2 * BT + lane] = spv.x; reinterpret_cast<int*>(rw_)[3 * BT + lane] = spv.y; \
-        _Pragma("unroll") for (int a = 0; a < AX; ++a) reinterpret_cast<int*>(rw_)[(4 + a) * BT + lane] = posv[a]; \
-    }
-    for (int base = 0; base < qtiles; base += 256) {
-        // ---- the query tiles of this stretch that see keys of this tile, in order
-        __syncthreads();
-        int n_list;
+    float f_sl[AX ? AX : 1];
+    int n_list = 0, f_at = 0, f_h = h0, f_st = 0, f_rows = 0;
+    const auto fetch = [&]() {      // (nothing here waits: the rows' numbers are looked at in settle(), a tile later)
+        const int q0 = __builtin_amdgcn_readfirstlane(list[f_at]) * BT, i = min(q0 + lane, p.nq - 1);
+        const long row = ((long)b * p.Hq + f_h) * p.nq + i;
+        lsev = p.lse[row];
+        delv = p.delta[row];
+        spv = make_int2(0, p.nk);
+        if (p.spans) spv = reinterpret_cast<const int2*>(p.spans + b * p.spans_sb)[i];
+#pragma unroll
+        for (int a = 0; a < AX; ++a) { posv[a] = p.pos_q[b * p.pq_sb + (long)i * AX + a]; f_sl[a] = p.slopes[f_h * AX + a]; }
+        f_rows = p.nq - q0;
+        unsigned char* st = smem + f_st * STAGE;
+        const int ok = min(BT, f_rows);
+        T::template fill<NW>(st, p.q + b * p.q_s[0] + f_h * p.q_s[1] + (long)q0 * p.q_s[2], ok, (int)p.q_s[2], wave, lane);
+        T::template fill<NW>(st + T::BYTES, p.dout + b * p.do_s[0] + f_h * p.do_s[1] + (long)q0 * p.do_s[2], ok, (int)p.do_s[2], wave, lane);
+    };
+    // rows that are not there, see nothing or whose lse says so: an empty span; which of the 64 see a key of this tile
+    const auto settle = [&]() {
+        const bool out = lane >= f_rows || lsev == -INFINITY;
+        spv = out ? make_int2(0, 0) : make_int2(max(spv.x, 0), min(spv.y, p.nk));
+        const bool in = spv.x < t1 && spv.y > t0;
+        if (!in) spv = make_int2(0, 0);
+        lsev = in ? __builtin_fmaf(lsev, SPAN_LOG2E, -F.kb) : 0.f;
+        delv = in ? delv : 0.f;
+        return __ballot(in);
+    };
+    const auto store_rows = [&]() {
+        if (wave == 0) {
+            float* rw = reinterpret_cast<float*>(smem + f_st * STAGE + 2 * T::BYTES);
+            int* ri = reinterpret_cast<int*>(rw);
+            rw[lane] = lsev; rw[BT + lane] = delv;
+            ri[2 * BT + lane] = spv.x; ri[3 * BT + lane] = spv.y;
+#pragma unroll
+            for (int a = 0; a < AX; ++a) ri[(4 + a) * BT + lane] = posv[a];
+        }
+    };
+    const auto pass = [&](auto take_v, auto take_k) {      // the whole walk over the query tiles, for the gradients that this wave takes
+        constexpr bool DV = decltype(take_v)::value, DK = decltype(take_k)::value;
+        u32x4_t kf[D / 16], vf[DK ? D / 16 : 1];
         {
-            const int qt = base + t;
-            int4 a = make_int4(INT32_MAX, 0, INT32_MAX, 0), e = a;
-            if (qt < qtiles) {
-                const int4* hp = p.hulls + (long)b * p.hull_tiles + 2 * qt;
-                a = hp[0];
-                if (2 * qt + 1 < p.hull_tiles) e = hp[1];
+            const uint16_t* kp = p.k + b * p.k_s[0] + hk * p.k_s[1] + (long)(live ? key : 0) * p.k_s[2] + half * 8;
+            const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1] + (long)(live ? key : 0) * p.v_s[2] + half * 8;
+            const u32x4_t z = {0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                const u32x4_t x = *reinterpret_cast<const u32x4_t*>(kp + c * 16);
+                kf[c] = live ? x : z;
+                if constexpr (DK) { const u32x4_t y = *reinterpret_cast<const u32x4_t*>(vp + c * 16); vf[c] = live ? y : z; }
             }
-            const bool in = (a.x < t1 && a.y > t0) || (e.x < t1 && e.y > t0);
-            const unsigned long long m = __ballot(in);
-            if (lane == 0) cnt[w] = __popcll(m);
-            __syncthreads();
-            int to = __popcll(m & ((1ull << lane) - 1ull));
-            for (int x = 0; x < w; ++x) to += cnt[x];
-            n_list = __builtin_amdgcn_readfirstlane(cnt[0] + cnt[1] + cnt[2] + cnt[3]);
-            if (in) { list[to] = qt; hull[2 * to] = a; hull[2 * to + 1] = e; }
-            __syncthreads();
         }
-        if (n_list == 0) continue;
-        f_at = 0; f_h = h0; f_stage = 0;
-        f_q = p.q + b * p.q_s[0] + f_h * p.q_s[1]; f_g = p.dout + b * p.do_s[0] + f_h * p.do_s[1];
-        SPAN_ISSUE();
-        SPAN_ROW_STORE();
-        for (bool more = true; more;) {
-            const int at = f_at, stage = f_stage, h = f_h;
-            unsigned char* Qs = smem + stage * STAGE;
-            unsigned char* Gs = Qs + T::BYTES;
-            const float* rw = reinterpret_cast<const float*>(Gs + T::BYTES);
-            const int* ri = reinterpret_cast<const int*>(rw);
-            const unsigned long long keep = __ballot(spv.x < t1 && spv.y > t0);      // rows that see some key of the tile
-            float sl[AX ? AX : 1];
-#pragma unroll
-            for (int a = 0; a < AX; ++a) sl[a] = p.slopes[h * AX + a] * SPAN_LOG2E;
-            if (++f_at == n_list) { f_at = 0; ++f_h; f_q += p.q_s[1]; f_g += p.do_s[1]; }
-            more = f_h < h1;
-            f_stage ^= 1;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (more) SPAN_ISSUE();
-            if (keep != ~0ull) {      // the others' values take no part, whatever they hold (rows behind the last document)
-                T::clear_rows(Qs, keep, t, 256);
-                T::clear_rows(Gs, keep, t, 256);
-                __syncthreads();
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int4 hl = hull[2 * at + n];
-                if (!(hl.x < min(w0 + 32, t1) && hl.y > w0)) continue;
-                const bool masked = !all_live || !(hl.z <= w0 && hl.w >= w0 + 32) || (uint32_t)(keep >> (32 * n)) != 0xFFFFFFFFu;
-                f32x16_t s, g;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
-#pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    s = mfma32<false>(T::rows(Qs, c, n, lane), kf[c], s);
-                    g = mfma32<false>(T::rows(Gs, c, n, lane), vf[c], g);
-                }
-#pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4) {
-                    const int o4 = n * 32 + g4 * 8 + half * 4;
-                    const float4 ls = *reinterpret_cast<const float4*>(rw + o4), de = *reinterpret_cast<const float4*>(rw + BT + o4);
-                    int4 lo4 = make_int4(0, 0, 0, 0), hi4 = lo4;
-                    if (masked) { lo4 = *reinterpret_cast<const int4*>(ri + 2 * BT + o4); hi4 = *reinterpret_cast<const int4*>(ri + 3 * BT + o4); }
-                    int4 qq[AX ? AX : 1];
-#pragma unroll
-                    for (int a = 0; a < AX; ++a) qq[a] = *reinterpret_cast<const int4*>(ri + (4 + a) * BT + o4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = g4 * 4 + e;
-#define SPAN_E4(v_) (e == 0 ? v_.x : (e == 1 ? v_.y : (e == 2 ? v_.z : v_.w)))
-                        float x = s[r], slope = 1.f;
-                        if constexpr (CAP) { const float th = span_tanh(x, c1); slope = __builtin_fmaf(-th, th, 1.f); x = th * c2; }
-                        else x *= c1;
-#pragma unroll
-                        for (int a = 0; a < AX; ++a) x = __builtin_fmaf(-sl[a], fabsf((float)(SPAN_E4(qq[a]) - pk[a])), x);
-                        float pr = __builtin_amdgcn_exp2f(x - SPAN_E4(ls)), d = pr * (g[r] - SPAN_E4(de));
-                        if (masked && !(live && SPAN_E4(lo4) <= key && key < SPAN_E4(hi4))) { pr = 0.f; d = 0.f; }
-#undef SPAN_E4
-                        s[r] = pr;
-                        g[r] = CAP ? d * slope : d;
-                    }
-                    asm volatile("" ::: "memory");
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const u32x4_t pf = pack_slots<false>(s, x), df = pack_slots<false>(g, x);      // P and dS rounded to bf16: operands
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        dv[c] = mfma32<false>(T::cols(Gs, 2 * n + x, c, lane), pf, dv[c]);
-                        dk[c] = mfma32<false>(T::cols(Qs, 2 * n + x, c, lane), df, dk[c]);
-                    }
-                }
-            }
-            if (more) SPAN_ROW_STORE();
-        }
-    }
-#undef SPAN_ISSUE
-#undef SPAN_ROW_STORE
-    float bad = 0.f;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(dk[c][r], 0.f, __builtin_fmaf(dv[c][r], 0.f, bad));
-    bad = both_halves_sum(bad);
-    const bool redo = live && bad != 0.f;
-    const long prow = ((long)b * p.Hk + hk) * p.nk, pall = (long)p.B * p.Hk * p.nk;      // partial sums: [splits][dk, dv][rows][D]
-    if (p.splits > 1) {
-        if (key < p.nk && !redo) {
-            float* kp = p.part_o + ((long)part * 2 * pall + prow + key) * D + half * 4;
-            float* vp = kp + pall * D;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                    *reinterpret_cast<float4*>(kp + c * 32 + g * 8) = live ? make_float4(dk[c][4 * g], dk[c][4 * g + 1], dk[c][4 * g + 2], dk[c][4 * g + 3]) : z;
-                    *reinterpret_cast<float4*>(vp + c * 32 + g * 8) = live ? make_float4(dv[c][4 * g], dv[c][4 * g + 1], dv[c][4 * g + 2], dv[c][4 * g + 3]) : z;
-                }
-        }
-    } else if (key < p.nk && !redo) {
-        uint16_t* kp = p.dk + b * p.dk_s[0] + hk * p.dk_s[1] + (long)key * p.dk_s[2] + half * 4;
-        uint16_t* vp = p.dv + b * p.dv_s[0] + hk * p.dv_s[1] + (long)key * p.dv_s[2] + half * 4;
+        f32x16_t dk[DK ? D / 32 : 1], dv[DV ? D / 32 : 1];
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const uint2 x = make_uint2(pack_bf16x2(dk[c][4 * g] * p.scale, dk[c][4 * g + 1] * p.scale), pack_bf16x2(dk[c][4 * g + 2] * p.scale, dk[c][4 * g + 3] * p.scale));
-                const uint2 y = make_uint2(pack_bf16x2(dv[c][4 * g], dv[c][4 * g + 1]), pack_bf16x2(dv[c][4 * g + 2], dv[c][4 * g + 3]));
-                *reinterpret_cast<uint2*>(kp + c * 32 + g * 8) = live ? x : make_uint2(0, 0);
-                *reinterpret_cast<uint2*>(vp + c * 32 + g * 8) = live ? y : make_uint2(0, 0);
+            for (int r = 0; r < 16; ++r) {
+                if constexpr (DK) dk[c][r] = 0.f;
+                if constexpr (DV) dv[c][r] = 0.f;
             }
-    }
-    unsigned long long todo = __ballot(redo) & 0xFFFFFFFFull;
-#pragma nounroll
-    while (todo) {
-        const int r = __builtin_ctzll(todo);
-        todo &= todo - 1;
-        float a[2], c[2];
-        key_again<D, AX>(p, b, hk, h0, h1, w0 + r, lane, a, c);
-        if (p.splits > 1) {
-            float* kp = p.part_o + ((long)part * 2 * pall + prow + w0 + r) * D;
-            float* vp = kp + pall * D;
-            if (lane < D) { kp[lane] = a[0]; vp[lane] = c[0]; }
-            if (D > 64) { kp[lane + 64] = a[1]; vp[lane + 64] = c[1]; }
-            continue;
+        for (int base = 0; base < qtiles; base += 256) {
+            // ---- the query tiles of this stretch that see keys of this tile, in order
+            __syncthreads();
+            {
+                const int qt = base + t;
+                int4 x = make_int4(INT32_MAX, 0, INT32_MAX, 0), y = x;
+                if (t < 256 && qt < qtiles) {
+                    const int4* hp = p.hulls + (long)b * p.hull_tiles + 2 * qt;
+                    x = hp[0];
+                    if (2 * qt + 1 < p.hull_tiles) y = hp[1];
+                }
+                const bool in = (x.x < t1 && x.y > t0) || (y.x < t1 && y.y > t0);
+                const unsigned long long m = __ballot(in);
+                if (lane == 0 && wave < 4) cnt[wave] = __popcll(m);
+                __syncthreads();
+                int to = __popcll(m & ((1ull << lane) - 1ull));
+                for (int z = 0; z < min(wave, 4); ++z) to += cnt[z];
+                n_list = __builtin_amdgcn_readfirstlane(cnt[0] + cnt[1] + cnt[2] + cnt[3]);
+                if (in) { list[to] = qt; hull[2 * to] = x; hull[2 * to + 1] = y; }
+                __syncthreads();
+            }
+            if (n_list == 0) continue;
+            f_at = 0; f_h = h0; f_st = 0;
+            fetch();
+            for (bool more = true; more;) {
+                const int at = f_at, st = f_st;
+                float sl[AX ? AX : 1];
+#pragma unroll
+                for (int a = 0; a < AX; ++a) sl[a] = f_sl[a] * F.per;
+                const unsigned long long keep = settle();
+                store_rows();
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();      // the tile and its rows' numbers are there for every wave; every wave is done with the other stage
+                if (++f_at == n_list) { f_at = 0; ++f_h; }
+                f_st ^= 1;
+                more = f_h < h1;
+                if (more) fetch();
+                const unsigned char* Qs = smem + st * STAGE;
+                const unsigned char* Gs = Qs + T::BYTES;
+                if (keep != ~0ull) {      // rows that see no key of this tile take no part, whatever they hold (rows behind the last document)
+                    T::clear_rows(smem + st * STAGE, keep, t, NT);
+                    T::clear_rows(smem + st * STAGE + T::BYTES, keep, t, NT);
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const i32x4_t hl = lds_i4(hull + 2 * at + n);
+                    if (__builtin_amdgcn_readfirstlane((int)(hl[0] < min(w0 + 32, t1) && hl[1] > w0)) == 0) continue;
+                    const bool masked = !all_live || __builtin_amdgcn_readfirstlane((int)!(hl[2] <= w0 && hl[3] >= w0 + 32)) != 0 || (uint32_t)(keep >> (32 * n)) != 0xFFFFFFFFu;
+                    f32x16_t s, g;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+                    u32x4_t q0 = T::rows(Qs, 0, n, lane), q1 = T::rows(Qs, 1, n, lane), g0 = q0, g1 = q1;
+                    if constexpr (DK) { g0 = T::rows(Gs, 0, n, lane); g1 = T::rows(Gs, 1, n, lane); }
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) {
+                        const u32x4_t x = q0, y = g0;
+                        q0 = q1; g0 = g1;
+                        if (c + 2 < D / 16) {
+                            q1 = T::rows(Qs, c + 2, n, lane);
+                            if constexpr (DK) g1 = T::rows(Gs, c + 2, n, lane);
+                        }
+                        s = mfma32<false>(x, kf[c], s);
+                        if constexpr (DK) g = mfma32<false>(y, vf[c], g);
+                    }
+                    int rows = st * STAGE + 2 * T::BYTES + (n * 32 + half * 4) * 4;
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const f32x4_t l4 = lds_f4(smem + rows + g4 * 32);
+                        float y4[4], w4[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y4[e] = F.y(s[g4 * 4 + e], w4[e]);
+#pragma unroll
+                        for (int a = 0; a < AX; ++a) {
+                            const i32x4_t k4 = lds_i4(smem + rows + (4 + a) * BT * 4 + g4 * 32);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) y4[e] = __builtin_fmaf(-sl[a], fabsf((float)(k4[e] - pk[a])), y4[e]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y4[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(y4[e], F.ka, -l4[e]));
+                        if constexpr (DK) {
+                            const f32x4_t d4 = lds_f4(smem + rows + BT * 4 + g4 * 32);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float d = y4[e] * (g[g4 * 4 + e] - d4[e]);
+                                if constexpr (CAP) d *= w4[e];
+                                w4[e] = d;
+                            }
+                            asm volatile("" : "+v"(rows), "+v"(w4[0]), "+v"(w4[1]), "+v"(w4[2]), "+v"(w4[3]));      // (done with these four before the next are fetched)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) g[g4 * 4 + e] = w4[e];
+                        } else asm volatile("" : "+v"(rows), "+v"(y4[0]), "+v"(y4[1]), "+v"(y4[2]), "+v"(y4[3]));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[g4 * 4 + e] = y4[e];
+                    }
+                    if (masked) {
+                        const int* ri = reinterpret_cast<const int*>(Gs + T::BYTES) + 2 * BT + n * 32 + half * 4;
+#pragma unroll
+                        for (int g4 = 0; g4 < 4; ++g4) {
+                            const i32x4_t lo = lds_i4(ri + g4 * 8), hi = lds_i4(ri + BT + g4 * 8);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {      // all ones: the row sees this key (spans are 0 <= lo <= hi)
+                                const uint32_t z = (uint32_t)-(int)((uint32_t)(mkey - lo[e]) < (uint32_t)(hi[e] - lo[e]));
+                                s[g4 * 4 + e] = __uint_as_float(__float_as_uint(s[g4 * 4 + e]) & z);
+                                if constexpr (DK) g[g4 * 4 + e] = __uint_as_float(__float_as_uint(g[g4 * 4 + e]) & z);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const u32x4_t pf = pack_slots<false>(s, x), df = pack_slots<false>(g, x);      // P and dS rounded to bf16: operands
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            if constexpr (DV) dv[c] = mfma32<false>(T::cols(Gs, 2 * n + x, c, lane), pf, dv[c]);
+                            if constexpr (DK) dk[c] = mfma32<false>(T::cols(Qs, 2 * n + x, c, lane), df, dk[c]);
+                        }
+                    }
+                }
+            }
         }
-        uint16_t* kp = p.dk + b * p.dk_s[0] + hk * p.dk_s[1] + (long)(w0 + r) * p.dk_s[2];
-        uint16_t* vp = p.dv + b * p.dv_s[0] + hk * p.dv_s[1] + (long)(w0 + r) * p.dv_s[2];
-        if (lane < D) { kp[lane] = f32_to_bf16(a[0] * p.scale); vp[lane] = f32_to_bf16(c[0]); }
-        if (D > 64) { kp[lane + 64] = f32_to_bf16(a[1] * p.scale); vp[lane + 64] = f32_to_bf16(c[1]); }
-    }
+        // ---- out; a key whose gradient is not finite -- another key's infinity or NaN met its zero weight in the matrix instruction -- is computed again from its own rows
+        const long prow = ((long)b * p.Hk + hk) * p.nk, pall = (long)p.B * p.Hk * p.nk;      // partial sums: [splits][dk, dv][rows][D]
+        const auto put = [&](f32x16_t* acc, int which, float f) {
+            float bad = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(acc[c][r], 0.f, bad);
+            bad = both_halves_sum(bad);
+            const bool redo = live && bad != 0.f;
+            if (!live) f = 0.f;
+            if (key < p.nk && !redo) {
+                uint16_t* o = which ? p.dv + b * p.dv_s[0] + hk * p.dv_s[1] + (long)key * p.dv_s[2] : p.dk + b * p.dk_s[0] + hk * p.dk_s[1] + (long)key * p.dk_s[2];
+                float* po = p.part_o + (((long)part * 2 + which) * pall + prow + key) * D;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float4 v = live ? make_float4(acc[c][4 * g] * f, acc[c][4 * g + 1] * f, acc[c][4 * g + 2] * f, acc[c][4 * g + 3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (p.splits > 1) *reinterpret_cast<float4*>(po + c * 32 + g * 8 + half * 4) = v;
+                        else *reinterpret_cast<uint2*>(o + c * 32 + g * 8 + half * 4) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+                    }
+            }
+            unsigned long long todo = __ballot(redo) & 0xFFFFFFFFull;
+#pragma nounroll
+            while (todo) {
+                const int r = __builtin_ctzll(todo);
+                todo &= todo - 1;
+                float a[2], c[2];
+                key_again<D, AX>(p, b, hk, h0, h1, w0 + r, lane, a, c);
+                if (which) { a[0] = c[0]; a[1] = c[1]; }
+                else { a[0] *= p.scale; a[1] *= p.scale; }
+                if (p.splits > 1) {
+                    float* po = p.part_o + (((long)part * 2 + which) * pall + prow + w0 + r) * D;
+                    if (lane < D) po[lane] = a[0];
+                    if (D > 64) po[lane + 64] = a[1];
+                } else {
+                    uint16_t* o = which ? p.dv + b * p.dv_s[0] + hk * p.dv_s[1] + (long)(w0 + r) * p.dv_s[2] : p.dk + b * p.dk_s[0] + hk * p.dk_s[1] + (long)(w0 + r) * p.dk_s[2];
+                    if (lane < D) o[lane] = f32_to_bf16(a[0]);
+                    if (D > 64) o[lane + 64] = f32_to_bf16(a[1]);
+                }
+            }
+        };
+        if constexpr (DK) put(dk, 0, F.end);
+        if constexpr (DV) put(dv, 1, 1.f);
+    };
+    if constexpr (!ROLES) pass(Yes(), Yes());
+    else if (wave < 4) pass(Yes(), No());
+    else pass(No(), Yes());
 }
 
 // adds the head splits of a key row in split order; masked keys' parts are zeros.  4 elements a thread
@@ -554,9 +625,8 @@ __global__ __launch_bounds__(256) void span_bwd_join(const SpanArgs p) {
     const bool is_v = row >= pall;
     const long r = is_v ? row - pall : row;
     const int key = (int)(r % p.nk), hk = (int)(r / p.nk % p.Hk), b = (int)(r / p.nk / p.Hk);
-    const float f = is_v ? 1.f : p.scale;
     uint16_t* o = is_v ? p.dv + b * p.dv_s[0] + hk * p.dv_s[1] + (long)key * p.dv_s[2] : p.dk + b * p.dk_s[0] + hk * p.dk_s[1] + (long)key * p.dk_s[2];
-    *reinterpret_cast<uint2*>(o + c) = make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
+    *reinterpret_cast<uint2*>(o + c) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
 }
 
 // Query heads that share a key head go to workgroups of their own, fp32 partial sums joined in order, as far as that fills the card: the smallest divisor of the group
@@ -589,7 +659,7 @@ int launch_bwd(hipStream_t s, const SpanArgs& a) {
         static std::atomic<unsigned long long> lds{0};
         if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dkv<D, AX, CAP>), sm, lds))) return rc;
         const long total = (long)a.B * a.Hk * a.splits * ((a.nk + BK - 1) / BK);
-        hipLaunchKernelGGL((span_bwd_dkv<D, AX, CAP>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), sm, s, a);
+        hipLaunchKernelGGL((span_bwd_dkv<D, AX, CAP>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(D == 128 ? 512 : 256), sm, s, a);
         if ((rc = mm_check_launch("span_bwd_dkv"))) return rc;
         if (a.splits > 1) {
             const long work = 2L * a.B * a.Hk * a.nk * (D / 4);

@@ -29,6 +29,10 @@ namespace {
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short sp_v4i16_t __attribute__((ext_vector_type(4)));
+// reads of LDS beside a DMA in flight: through native vectors.  HIP's int4 / float4 carry no alias information, and without any the compiler waits for every DMA first
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4_t lds_i4(const void* p) { return *reinterpret_cast<const i32x4_t*>(p); }
+__device__ __forceinline__ f32x4_t lds_f4(const void* p) { return *reinterpret_cast<const f32x4_t*>(p); }
 
 constexpr float SPAN_LOG2E = 1.4426950408889634f, SPAN_LN2 = 0.6931471805599453f;
 constexpr float SPAN_LOW = -1.0e30f;      // start of a running maximum: finite, so that a masked score (-inf) minus it is -inf, not NaN
