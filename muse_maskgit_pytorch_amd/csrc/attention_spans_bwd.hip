@@ -313,6 +313,27 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
     }
 }
 
+// The order of LDS reads and matrix instructions of a product in the instruction stream: the operands of two steps ahead.  Left alone the compiler often reads one
+// operand, waits for it and multiplies, eight times over.  (0x100: LDS read, 0x008: matrix instruction)
+template <int PER, int STEPS>
+__device__ __forceinline__ void paced() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * PER, 0);
+#pragma unroll
+    for (int c = 0; c < STEPS; ++c) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+        if (c + 2 < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+    }
+}
+template <int STEPS>      // transposed operands: two reads each
+__device__ __forceinline__ void paced_cols() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+    for (int c = 0; c < STEPS; ++c) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (c + 3 < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+}
+
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
@@ -504,6 +525,7 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
                         s = mfma32<false>(x, kf[c], s);
                         if constexpr (DK) g = mfma32<false>(y, vf[c], g);
                     }
+                    paced<DK ? 2 : 1, D / 16>();
                     int rows = st * STAGE + 2 * T::BYTES + (n * 32 + half * 4) * 4;
 #pragma unroll
                     for (int g4 = 0; g4 < 4; ++g4) {
@@ -527,10 +549,10 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
                                 if constexpr (CAP) d *= w4[e];
                                 w4[e] = d;
                             }
-                            asm volatile("" : "+v"(rows), "+v"(w4[0]), "+v"(w4[1]), "+v"(w4[2]), "+v"(w4[3]));      // (done with these four before the next are fetched)
+                            if constexpr (AX > 0) asm volatile("" : "+v"(rows), "+v"(w4[0]), "+v"(w4[1]), "+v"(w4[2]), "+v"(w4[3]));      // (done with these four before the next are fetched)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) g[g4 * 4 + e] = w4[e];
-                        } else asm volatile("" : "+v"(rows), "+v"(y4[0]), "+v"(y4[1]), "+v"(y4[2]), "+v"(y4[3]));
+                        } else if constexpr (AX > 0) asm volatile("" : "+v"(rows), "+v"(y4[0]), "+v"(y4[1]), "+v"(y4[2]), "+v"(y4[3]));
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[g4 * 4 + e] = y4[e];
                     }
@@ -556,6 +578,7 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
                             if constexpr (DK) dk[c] = mfma32<false>(T::cols(Qs, 2 * n + x, c, lane), df, dk[c]);
                         }
                     }
+                    paced_cols<(DV ? D / 16 : 0) + (DK ? D / 16 : 0)>();
                 }
             }
         }
