@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr int WQ = 128, KT = 64;
+constexpr int WQ = SPAN_TILE, KT = 64;
 
 // sum over this row's visible keys in [k0, k1) of exp2(s - m) v, by one wave: lane = key for the scores, lane = element for the sum
 template <int D, bool F16, int AX>
@@ -551,48 +551,9 @@ __global__ __launch_bounds__(256) void span_attn_join(const SpanArgs p) {
     if (p.lse && c == 0) p.lse[((long)b * p.Hq + h) * p.nq + i] = L > 0.f ? (M + __builtin_amdgcn_logf(L)) * SPAN_LN2 : (L == 0.f ? -INFINITY : L);
 }
 
-// Tiles of 128 query rows, those that see the most keys first.  Documents differ in length: in their own order the long ones meet on some CUs and the others wait
-// (16300 rows of packed images, 8 heads: 67 us; prefix case: 137 us).  The length comes from four rows of a tile; it decides an order, no result.  One workgroup, a
-// counting sort in LDS, up to ORDER_MAX tiles.
-constexpr int ORDER_MAX = 4096;
-__global__ __launch_bounds__(1024) void span_order(const int32_t* __restrict__ spans, long sb, int B, int n, int nk, int tiles, int32_t* __restrict__ order) {
-    __shared__ int hist[1024], part[16];
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6, N = B * tiles;
-    hist[t] = 0;
-    __syncthreads();
-    int bucket[ORDER_MAX / 1024];
-#pragma unroll
-    for (int x = 0; x < ORDER_MAX / 1024; ++x) {
-        const int item = t + x * 1024;
-        bucket[x] = 0;
-        if (item >= N) continue;
-        const int2* sp = reinterpret_cast<const int2*>(spans + (item / tiles) * sb);
-        const int r0 = item % tiles * WQ;
-        int lo = INT32_MAX, hi = 0;
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-            const int2 v = sp[min(r0 + y * (WQ - 1) / 3, n - 1)];
-            const int a = max(v.x, 0), e = min(v.y, nk);
-            if (a < e) { lo = min(lo, a); hi = max(hi, e); }
-        }
-        const long len = hi > lo ? hi - lo : 0;
-        bucket[x] = 1023 - (int)(len * 1023 / max(nk, 1));
-        atomicAdd(&hist[bucket[x]], 1);
-    }
-    __syncthreads();
-    int v = hist[t];
-    const int own = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(v, o, 64); if (lane >= o) v += u; }
-    if (lane == 63) part[w] = v;
-    __syncthreads();
-    int base = 0;
-    for (int x = 0; x < w; ++x) base += part[x];
-    hist[t] = base + v - own;
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < ORDER_MAX / 1024; ++x)
-        if (t + x * 1024 < N) order[atomicAdd(&hist[bucket[x]], 1)] = t + x * 1024;
+__global__ __launch_bounds__(1024) void span_order(const int32_t* __restrict__ spans, long sb, int B, int n, int nk, int32_t* __restrict__ order) {
+    __shared__ SpanOrderLds m;
+    span_order_tiles<1024>(m, spans, sb, B, n, nk, order);
 }
 
 struct SpanPlan { bool narrow; int row_tiles, splits; };
@@ -665,19 +626,9 @@ void span_args(const mm_span_attn* a, SpanArgs& p) {
     p.dout = (const uint16_t*)a->dout; p.dq = (uint16_t*)a->dq; p.dk = (uint16_t*)a->dk; p.dv = (uint16_t*)a->dv;
 }
 
-// the order pays from two workgroups per CU on (below, all of them start at once)
-long span_order_tiles(const mm_span_attn* a) {
-    const long n = (long)a->batch * ((a->nq + WQ - 1) / WQ);
-    return a->spans && n <= ORDER_MAX && n * a->heads_q >= 512 ? n : 0;
-}
-int span_order_run(hipStream_t s, const mm_span_attn* a, int32_t* order) {
-    hipLaunchKernelGGL(span_order, dim3(1), dim3(1024), 0, s, a->spans, a->spans_sb, a->batch, a->nq, a->nk, (a->nq + WQ - 1) / WQ, order);
-    return mm_check_launch("span_order");
-}
-
 size_t k_span_attn_workspace_bytes(const mm_span_attn* a) {
     const SpanPlan pl = span_plan(a);
-    if (!pl.narrow) return (size_t)span_order_tiles(a) * sizeof(int32_t);
+    if (!pl.narrow) return (size_t)span_order_count(a) * sizeof(int32_t);
     if (pl.splits == 1) return 0;
     return (size_t)pl.splits * a->batch * a->heads_k * pl.row_tiles * 32 * (a->dim + 2) * sizeof(float);
 }
@@ -687,8 +638,9 @@ int k_span_attn(hipStream_t s, const mm_span_attn* a, void* ws) {
     span_args(a, p);
     const SpanPlan pl = span_plan(a);
     p.splits = pl.splits; p.row_tiles = pl.row_tiles;
-    if (!pl.narrow && span_order_tiles(a)) {
-        if (const int rc = span_order_run(s, a, (int32_t*)ws)) return rc;
+    if (!pl.narrow && span_order_count(a)) {
+        hipLaunchKernelGGL(span_order, dim3(1), dim3(1024), 0, s, a->spans, a->spans_sb, a->batch, a->nq, a->nk, (int32_t*)ws);
+        if (const int rc = mm_check_launch("span_order")) return rc;
         p.order = (const int32_t*)ws;
     }
     p.part_o = (float*)ws;

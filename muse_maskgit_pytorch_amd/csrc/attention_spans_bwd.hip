@@ -12,12 +12,10 @@
 #include "span_attn.h"
 
 void span_args(const mm_span_attn* a, SpanArgs& p);
-long span_order_tiles(const mm_span_attn* a);
-int span_order_run(hipStream_t s, const mm_span_attn* a, int32_t* order);
 
 namespace {
 
-constexpr int BQ = 128, BK = 128, BT = 64;
+constexpr int BQ = SPAN_TILE, BK = 128, BT = 64;
 
 __device__ __forceinline__ int2 row_span(const SpanArgs& p, int b, int h, int i) {      // empty where the row sees nothing or its lse says so
     int lo = 0, hi = p.nk;
@@ -29,12 +27,45 @@ __device__ __forceinline__ int2 row_span(const SpanArgs& p, int b, int h, int i)
     return make_int2(lo, hi);
 }
 
-// one wave per 64 / (D / 8) rows: D / 8 lanes a row, 16 bytes of out and of dout each
+// In one launch, all of it read by the other two:
+//   the first workgroup (where the order is wanted): the order of the query tiles
+//   then 8 blocks of 32 queries a workgroup: .x lowest, .y highest key bound (x >= y: nobody sees anything), .z / .w highest low and lowest high bound (a key tile
+//   inside them needs no mask).  By the spans alone: a row whose lse is -inf although its span is not empty (all of its keys masked) is found per tile
+//   then delta: D / 8 lanes a row, 16 bytes of out and of dout each
 template <int D>
 __global__ __launch_bounds__(256) void span_bwd_pre(const SpanArgs p) {
     constexpr int TPR = D / 8, RPB = 256 / TPR;
+    __shared__ SpanOrderLds m;
+    long block = blockIdx.x;
+    if (p.order_out) {
+        if (block == 0) { span_order_tiles<256>(m, p.spans, p.spans_sb, p.B, p.nq, p.nk, p.order_out); return; }
+        --block;
+    }
+    const long hull_blocks = ((long)p.B * p.hull_tiles + 7) / 8;
+    if (block < hull_blocks) {
+        const int lane = threadIdx.x & 63;
+        const long seg = (block * 256 + threadIdx.x) / 32, tiles = p.hull_tiles;
+        const int b = (int)(seg / tiles), i = (int)(seg % tiles) * 32 + (lane & 31);
+        int lo = INT32_MAX, hi = 0, lx = INT32_MAX, hn = 0;      // a row that is not there or sees nothing: no part of the hull, and no tile without a mask
+        if (b < p.B && i < p.nq) {
+            int a = 0, e = p.nk;
+            if (p.spans) {
+                const int2 sp = reinterpret_cast<const int2*>(p.spans + b * p.spans_sb)[i];
+                a = max(sp.x, 0); e = min(sp.y, p.nk);
+            }
+            if (a < e) { lo = lx = a; hi = hn = e; }
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            lo = min(lo, __shfl_xor(lo, o, 64)); hi = max(hi, __shfl_xor(hi, o, 64));
+            lx = max(lx, __shfl_xor(lx, o, 64)); hn = min(hn, __shfl_xor(hn, o, 64));
+        }
+        if (b < p.B && (lane & 31) == 0) p.hulls[seg] = make_int4(lo, hi, lx, hn);
+        return;
+    }
+    block -= hull_blocks;
     const int c = threadIdx.x % TPR;
-    const long row = (long)blockIdx.x * RPB + threadIdx.x / TPR, rows = (long)p.B * p.Hq * p.nq;
+    const long row = block * RPB + threadIdx.x / TPR, rows = (long)p.B * p.Hq * p.nq;
     if (row < rows) {
         const int i = (int)(row % p.nq), h = (int)(row / p.nq % p.Hq), b = (int)(row / p.nq / p.Hq);
         const u32x4_t x = *reinterpret_cast<const u32x4_t*>(p.out + b * p.o_s[0] + h * p.o_s[1] + (long)i * p.o_s[2] + c * 8);
@@ -48,28 +79,24 @@ __global__ __launch_bounds__(256) void span_bwd_pre(const SpanArgs p) {
     }
 }
 
-// per 32 queries: .x lowest, .y highest key bound (x >= y: nobody sees anything), .z / .w highest low and lowest high bound (a tile inside them needs no mask).  By the
-// spans alone: a row whose lse is -inf although its span is not empty (all of its keys masked) is found per key tile by the mask.
-__global__ __launch_bounds__(256) void span_bwd_hulls(const SpanArgs p) {
-    const int lane = threadIdx.x & 63;
-    const long seg = ((long)blockIdx.x * 256 + threadIdx.x) / 32;
-    const long tiles = (long)p.hull_tiles;
-    const int b = (int)(seg / tiles), i = (int)(seg % tiles) * 32 + (lane & 31);
-    int lo = INT32_MAX, hi = 0, lx = INT32_MAX, hn = 0;      // a row that is not there or sees nothing: no part of the hull, and no tile without a mask
-    if (b < p.B && i < p.nq) {
-        int a = 0, e = p.nk;
-        if (p.spans) {
-            const int2 sp = reinterpret_cast<const int2*>(p.spans + b * p.spans_sb)[i];
-            a = max(sp.x, 0); e = min(sp.y, p.nk);
+// the slopes' gradients: the parts of the query tiles (and rows of the batch) in 32 chains, the chains in order; one workgroup, launched with dk and dv
+__device__ __forceinline__ void sum_slope_parts(const SpanArgs& p, int threads, float* red) {
+    const int n = p.Hq * p.axes, t = threadIdx.x, lanes = threads / 32;      // threads / 32 columns at a time, 32 chains each
+    const long parts = (long)p.B * ((p.nq + BQ - 1) / BQ);
+    for (int c0 = 0; c0 < n; c0 += lanes) {
+        const int c = c0 + t % lanes, chain = t / lanes;
+        float v = 0.f;
+        if (c < n)
+            for (long x = chain; x < parts; x += 32) v += p.dsl_part[x * n + c];
+        __syncthreads();
+        red[chain * lanes + t % lanes] = v;
+        __syncthreads();
+        if (chain == 0 && c < n) {
+            v = 0.f;
+            for (int x = 0; x < 32; ++x) v += red[x * lanes + t];
+            p.dslopes[c] = v;
         }
-        if (a < e) { lo = lx = a; hi = hn = e; }
     }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        lo = min(lo, __shfl_xor(lo, o, 64)); hi = max(hi, __shfl_xor(hi, o, 64));
-        lx = max(lx, __shfl_xor(lx, o, 64)); hn = min(hn, __shfl_xor(hn, o, 64));
-    }
-    if (b < p.B && (lane & 31) == 0) p.hulls[seg] = make_int4(lo, hi, lx, hn);
 }
 
 // gradient of one query row from its own keys alone, by one wave (lane = key, then lane = element)
@@ -382,7 +409,11 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), w = ROLES ? wave & 3 : wave;
     const int tiles = (p.nk + BK - 1) / BK, total = p.B * p.Hk * p.splits * tiles, per = (total + 7) / 8;
     const int item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);      // (a contiguous part of (row, key head, split, tile) per XCD)
-    if ((int)(blockIdx.x >> 3) >= per || item >= total) return;
+    if ((int)(blockIdx.x >> 3) >= per) {
+        if (AX > 0 && p.dsl_part) sum_slope_parts(p, NT, reinterpret_cast<float*>(smem));      // (one workgroup more than there are tiles)
+        return;
+    }
+    if (item >= total) return;
     const int tile = item % tiles, part = (item / tiles) % p.splits, hk = (item / tiles / p.splits) % p.Hk, b = item / tiles / p.splits / p.Hk;
     const int heads = p.Hq / p.Hk / p.splits, h0 = (hk * p.splits + part) * heads, h1 = h0 + heads;      // the query heads of this workgroup
     const int t0 = tile * BK, t1 = min(t0 + BK, p.nk), w0 = t0 + w * 32;      // the wave's keys: w0 .. w0 + 31
@@ -666,25 +697,24 @@ template <int D, int AX, bool CAP>
 int launch_bwd(hipStream_t s, const SpanArgs& a) {
     int rc;
     if (a.nq > 0) {
-        const long rows = (long)a.B * a.Hq * a.nq;
-        hipLaunchKernelGGL(span_bwd_pre<D>, dim3((unsigned)((rows + 256 / (D / 8) - 1) / (256 / (D / 8)))), dim3(256), 0, s, a);
+        const long rows = (long)a.B * a.Hq * a.nq, rpb = 256 / (D / 8);
+        const long blocks = (a.order_out ? 1 : 0) + ((long)a.B * a.hull_tiles + 7) / 8 + (rows + rpb - 1) / rpb;
+        hipLaunchKernelGGL(span_bwd_pre<D>, dim3((unsigned)blocks), dim3(256), 0, s, a);
         if ((rc = mm_check_launch("span_bwd_pre"))) return rc;
-        hipLaunchKernelGGL(span_bwd_hulls, dim3((unsigned)(((long)a.B * a.hull_tiles + 7) / 8)), dim3(256), 0, s, a);
-        if ((rc = mm_check_launch("span_bwd_hulls"))) return rc;
         constexpr int sm = 2 * (2 * Tile<D, BT>::BYTES + AX * BT * 4) + 64;
         static std::atomic<unsigned long long> lds{0};
         if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dq<D, AX, CAP>), sm, lds))) return rc;
         hipLaunchKernelGGL((span_bwd_dq<D, AX, CAP>), dim3((unsigned)(a.B * a.Hq * ((a.nq + BQ - 1) / BQ))), dim3(256), sm, s, a);
         if ((rc = mm_check_launch("span_bwd_dq"))) return rc;
     }
-    if (a.nk > 0) {
+    if (a.nk > 0 || a.dsl_part) {      // (without keys: the slopes' gradients alone)
         constexpr int sm = 2 * (2 * Tile<D, BT>::BYTES + (4 + AX) * BT * 4) + 256 * 4 + 512 * 16 + 16;
         static std::atomic<unsigned long long> lds{0};
         if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dkv<D, AX, CAP>), sm, lds))) return rc;
         const long total = (long)a.B * a.Hk * a.splits * ((a.nk + BK - 1) / BK);
-        hipLaunchKernelGGL((span_bwd_dkv<D, AX, CAP>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(D == 128 ? 512 : 256), sm, s, a);
+        hipLaunchKernelGGL((span_bwd_dkv<D, AX, CAP>), dim3((unsigned)((total + 7) / 8 * 8 + (a.dsl_part ? 1 : 0))), dim3(D == 128 ? 512 : 256), sm, s, a);
         if ((rc = mm_check_launch("span_bwd_dkv"))) return rc;
-        if (a.splits > 1) {
+        if (a.splits > 1 && a.nk > 0) {
             const long work = 2L * a.B * a.Hk * a.nk * (D / 4);
             hipLaunchKernelGGL(span_bwd_join<D>, dim3((unsigned)((work + 255) / 256)), dim3(256), 0, s, a);
             if ((rc = mm_check_launch("span_bwd_join"))) return rc;
@@ -713,7 +743,7 @@ BwdLayout bwd_layout(const mm_span_attn* a) {
     size_t at = 0;
     r.hulls = at; at += (size_t)a->batch * r.hull_tiles * sizeof(int4);
     r.delta = at; at += ((size_t)a->batch * a->heads_q * a->nq * sizeof(float) + 15) / 16 * 16;
-    r.order = at; at += span_order_tiles(a) * sizeof(int32_t);
+    r.order = at; at += span_order_count(a) * sizeof(int32_t);
     r.slopes = at; at += (size_t)r.slope_parts * a->heads_q * a->axes * sizeof(float);
     at = (at + 15) / 16 * 16;
     r.splits = head_splits(a);
@@ -734,13 +764,11 @@ int k_span_attn_bwd(hipStream_t s, const mm_span_attn* a, void* ws) {
     p.hull_tiles = l.hull_tiles;
     p.delta = reinterpret_cast<float*>((char*)ws + l.delta);
     p.splits = l.splits;
-    if (span_order_tiles(a)) {
-        p.order = reinterpret_cast<int32_t*>((char*)ws + l.order);
-        if (const int rc = span_order_run(s, a, reinterpret_cast<int32_t*>((char*)ws + l.order))) return rc;
-    }
+    if (span_order_count(a)) p.order = p.order_out = reinterpret_cast<int32_t*>((char*)ws + l.order);
     p.part_o = reinterpret_cast<float*>((char*)ws + l.parts);
     p.dsl_part = l.slope_parts ? reinterpret_cast<float*>((char*)ws + l.slopes) : nullptr;
-    const int rc = a->dim == 32 ? launch_bwd_dim<32>(s, p) : (a->dim == 64 ? launch_bwd_dim<64>(s, p) : launch_bwd_dim<128>(s, p));
-    if (rc || !a->slopes || !a->dslopes) return rc;
-    return k_colsum(s, p.dsl_part, (int)l.slope_parts, (long)a->heads_q * a->axes, a->dslopes);      // (no rows: zeros)
+    p.dslopes = a->dslopes;
+    if (a->slopes && a->dslopes && !l.slope_parts)      // (no rows: zeros)
+        if (const int rc = k_colsum(s, a->dslopes, 0, (long)a->heads_q * a->axes, a->dslopes)) return rc;
+    return a->dim == 32 ? launch_bwd_dim<32>(s, p) : (a->dim == 64 ? launch_bwd_dim<64>(s, p) : launch_bwd_dim<128>(s, p));
 }

@@ -22,7 +22,7 @@ struct SpanArgs {
     // backward
     const uint16_t* dout; long do_s[3];
     uint16_t *dq, *dk, *dv; long dq_s[3], dk_s[3], dv_s[3];
-    float* delta; float* dsl_part; int4* hulls; int hull_tiles;
+    float* delta; float* dsl_part; float* dslopes; int4* hulls; int hull_tiles; int32_t* order_out;
 };
 
 namespace {
@@ -174,6 +174,61 @@ __device__ __forceinline__ float pair_score(const SpanArgs& p, const uint16_t* q
     for (int a = 0; a < AX; ++a)
         x -= p.slopes[h * AX + a] * SPAN_LOG2E * fabsf((float)(p.pos_q[b * p.pq_sb + (long)i * AX + a] - p.pos_k[b * p.pk_sb + (long)key * AX + a]));
     return x;
+}
+
+// Tiles of 128 query rows, those that see the most keys first.  Documents differ in length: in their own order the long ones meet on some CUs and the others wait
+// (16300 rows of packed images, 8 heads: 67 us, 60 so; long documents in order, 16 heads of 128: 137 and 107).  The length comes from four rows of a tile; it decides an
+// order, no result.  One workgroup, a counting sort in LDS, up to SPAN_ORDER_MAX tiles; ITEMS = SPAN_ORDER_MAX / threads.
+constexpr int SPAN_ORDER_MAX = 4096, SPAN_TILE = 128;
+struct SpanOrderLds { int hist[1024], part[16]; };
+template <int THREADS>
+__device__ __forceinline__ void span_order_tiles(SpanOrderLds& m, const int32_t* __restrict__ spans, long sb, int B, int n, int nk, int32_t* __restrict__ order) {
+    constexpr int ITEMS = SPAN_ORDER_MAX / THREADS, PER = 1024 / THREADS;
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, tiles = (n + SPAN_TILE - 1) / SPAN_TILE, N = B * tiles;
+#pragma unroll
+    for (int y = 0; y < PER; ++y) m.hist[t * PER + y] = 0;
+    __syncthreads();
+    int bucket[ITEMS];
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x) {
+        const int item = t + x * THREADS;
+        bucket[x] = 0;
+        if (item >= N) continue;
+        const int2* sp = reinterpret_cast<const int2*>(spans + (item / tiles) * sb);
+        const int r0 = item % tiles * SPAN_TILE;
+        int lo = INT32_MAX, hi = 0;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const int2 v = sp[min(r0 + y * (SPAN_TILE - 1) / 3, n - 1)];
+            const int a = max(v.x, 0), e = min(v.y, nk);
+            if (a < e) { lo = min(lo, a); hi = max(hi, e); }
+        }
+        const long len = hi > lo ? hi - lo : 0;
+        bucket[x] = 1023 - (int)(len * 1023 / max(nk, 1));
+        atomicAdd(&m.hist[bucket[x]], 1);
+    }
+    __syncthreads();
+    int own[PER], v = 0;
+#pragma unroll
+    for (int y = 0; y < PER; ++y) { own[y] = m.hist[t * PER + y]; v += own[y]; }
+    const int mine = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(v, o, 64); if (lane >= o) v += u; }
+    if (lane == 63) m.part[w] = v;
+    __syncthreads();
+    int base = v - mine;
+    for (int x = 0; x < w; ++x) base += m.part[x];
+#pragma unroll
+    for (int y = 0; y < PER; ++y) { m.hist[t * PER + y] = base; base += own[y]; }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x)
+        if (t + x * THREADS < N) order[atomicAdd(&m.hist[bucket[x]], 1)] = t + x * THREADS;
+}
+// the order pays from two workgroups per CU on (below, all of them start at once)
+inline long span_order_count(const mm_span_attn* a) {
+    const long n = (long)a->batch * ((a->nq + SPAN_TILE - 1) / SPAN_TILE);
+    return a->spans && n <= SPAN_ORDER_MAX && n * a->heads_q >= 512 ? n : 0;
 }
 
 // more than 64 KiB of dynamic LDS has to be allowed once per kernel and device (`done`: a bit per device)
