@@ -55,8 +55,9 @@ __global__ __launch_bounds__(256) void attention_spans_kernel(const int32_t* __r
 // Pair p of a head (p < P = sum of the sections) belongs to axis a(p) and turns by the angle  pos_a * freq_p:   a' = a cos - b sin,  b' = a sin + b cos,  with
 // (a, b) = elements (p, P + p), or (2p, 2p + 1) interleaved; elements from 2P on pass.  The gradient turns back.  The angle is formed in 64 bits and reduced to one
 // turn there (far positions: an fp32 product is 0.03 rad off at position 10^6), then sin / cos in fp32.
-// HBM-bound: one read + one write of every element (the backward with the norm reads two).  A token's angles serve all of its heads: a group of G lanes owns a
-// token, lane u of it VEC pairs, and walks over the heads of q and of k.  With few tokens the heads are split over blockIdx.y instead (angles computed again there).
+// HBM-bound: one read + one write of every element (the backward with the norm reads two).  A workgroup takes TB tokens: first their turns into LDS, one pair a thread
+// (the 64-bit products and sincospif of eight pairs side by side in a lane take 130 registers, and the loads need the occupancy), then their heads, G lanes a head, VEC
+// pairs a lane.
 struct RotT {      // one of q / k
     const void* x; long x_sb, x_sh, x_sn;      // forward: the input; backward: the forward's input (NORM only)
     const void* dy; long d_sb, d_sh, d_sn;     // backward: the gradient of the output
@@ -69,8 +70,8 @@ struct RotArgs {
     const int32_t* pos; long pos_sb; int A;
     const double* freq;
     int P, c1, c2, c3;                         // axis of pair p = (p >= c1) + (p >= c2) + (p >= c3)
-    int B, n, d, G, interleaved, heads_per_block;
-    float* part;                               // backward with the norm: [gridDim.x * gridDim.y][2][d]
+    int B, n, d, G, TB, interleaved;
+    float* part;                               // backward with the norm: [gridDim.x][2][d]
 };
 
 template <typename T> __device__ __forceinline__ float rot_ld(T v);
@@ -81,12 +82,6 @@ template <> __device__ __forceinline__ float rot_ld<__bf16>(__bf16 v) { return (
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC > 16 ? 16 : sizeof(T) * VEC) RotVec { T v[VEC]; };
 
 template <typename T, int VEC>
-__device__ __forceinline__ void rot_load(const T* p, float (&f)[VEC]) {
-    const RotVec<T, VEC> r = *reinterpret_cast<const RotVec<T, VEC>*>(p);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = rot_ld<T>(r.v[e]);
-}
-template <typename T, int VEC>
 __device__ __forceinline__ void rot_store(T* p, const float (&f)[VEC]) {
     RotVec<T, VEC> r;
 #pragma unroll
@@ -94,9 +89,9 @@ __device__ __forceinline__ void rot_store(T* p, const float (&f)[VEC]) {
     *reinterpret_cast<RotVec<T, VEC>*>(p) = r;
 }
 
-template <int VEC>
-__device__ __forceinline__ void rot_turn(float (&a)[VEC], float (&b)[VEC], const float (&c)[VEC], const float (&s)[VEC], bool interleaved) {
-    if (!interleaved || VEC == 1) {
+template <int VEC, bool INTER>
+__device__ __forceinline__ void rot_turn(float (&a)[VEC], float (&b)[VEC], const float (&c)[VEC], const float (&s)[VEC]) {
+    if constexpr (!INTER || VEC == 1) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const float x = a[e], y = b[e];
@@ -120,157 +115,180 @@ __device__ __forceinline__ float rot_group_sum(float v, int G) {
     return v;
 }
 
-template <typename T, int VEC, bool NORM, bool BWD>
+constexpr int ROT_TURNS = 2048;      // (cos, sin) pairs a workgroup holds: ROT_TURNS / (d / 2) tokens at most
+
+template <typename T, int VEC, bool NORM, bool BWD, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs p) {
-    const int G = p.G, u = threadIdx.x & (G - 1), slots = 256 / G, slot = threadIdx.x / G;
-    const int U = p.d / (2 * VEC);
-    const bool live = u < U;
-    const bool inter = p.interleaved != 0;
+    constexpr int HB = VEC == 8 && !(NORM && BWD) ? 2 : 1;      // heads whose loads go out together
+    __shared__ __attribute__((aligned(16))) float2 turns[ROT_TURNS];
+    const int G = p.G, u = threadIdx.x & (G - 1), slots = 256 / G, slot = threadIdx.x / G, pairs = p.d / 2;
+    const bool live = u < p.d / (2 * VEC);
     int offa, offb;
-    if (inter) { offa = 2 * VEC * u; offb = offa + VEC; }
+    if (INTER) { offa = 2 * VEC * u; offb = offa + VEC; }
     else if (u * VEC < p.P) { offa = u * VEC; offb = p.P + u * VEC; }
     else { offa = 2 * p.P + 2 * (u * VEC - p.P); offb = offa + VEC; }
-    const int h_all = p.t[0].H + p.t[1].H;
-    const int h0 = blockIdx.y * p.heads_per_block, h1 = min(h0 + p.heads_per_block, h_all);
     const long tokens = (long)p.B * p.n;
-    float acc[2][2][VEC];      // backward with the norm: gradient of the scale, [q / k][a / b]
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+    for (int w = 0; w < 2; ++w) {      // q, then k
+        const RotT& t = p.t[w];
+        float acc[2][VEC];             // backward with the norm: gradient of the scale
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[w][0][e] = acc[w][1][e] = 0.f;
-
-    for (long tok0 = (long)blockIdx.x * slots; tok0 < tokens; tok0 += (long)gridDim.x * slots) {
-        const long tok = tok0 + slot;
-        const bool ok = tok < tokens && live;
-        const int b = ok ? (int)(tok / p.n) : 0, i = ok ? (int)(tok % p.n) : 0;
-        float c[VEC], s[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int pr = u * VEC + e;
-            c[e] = 1.f; s[e] = 0.f;
-            if (ok && pr < p.P) {
-                const int ax = (pr >= p.c1) + (pr >= p.c2) + (pr >= p.c3);
-                const double turns = (double)p.pos[b * p.pos_sb + (long)i * p.A + ax] * p.freq[pr] * 0.15915494309189533577;      // / (2 pi)
-                const float half_turns = (float)(2.0 * (turns - rint(turns)));
-                sincospif(half_turns, &s[e], &c[e]);
-                if (BWD) s[e] = -s[e];
+        for (int e = 0; e < VEC; ++e) acc[0][e] = acc[1][e] = 0.f;
+        for (long tok0 = (long)blockIdx.x * p.TB; tok0 < tokens && t.H > 0; tok0 += (long)gridDim.x * p.TB) {
+            const int here = (int)min((long)p.TB, tokens - tok0);
+            if (w == 0 || p.t[0].H == 0 || (long)gridDim.x * p.TB < tokens) {      // (one group of tokens: k finds q's turns)
+                __syncthreads();
+#pragma nounroll
+                for (int x = threadIdx.x; x < here * pairs; x += 256) {
+                    const long tk = tok0 + x / pairs;
+                    const int pr = x % pairs;
+                    float2 cs = make_float2(1.f, 0.f);
+                    if (pr < p.P) {
+                        const int ax = (pr >= p.c1) + (pr >= p.c2) + (pr >= p.c3);
+                        const double turn = (double)p.pos[tk / p.n * p.pos_sb + tk % p.n * p.A + ax] * p.freq[pr] * 0.15915494309189533577;      // / (2 pi)
+                        sincospif((float)(2.0 * (turn - rint(turn))), &cs.y, &cs.x);
+                        if (BWD) cs.y = -cs.y;
+                    }
+                    turns[x] = cs;
+                }
+                __syncthreads();
             }
-        }
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {      // q, then k
-            const RotT& t = p.t[w];
-            const int f = w ? p.t[0].H : 0;
-            const int a0 = max(h0 - f, 0), a1 = min(h1 - f, t.H);
             float sa[VEC], sb[VEC];
             if constexpr (NORM) {
-                if (a0 < a1) {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) { sa[e] = live ? t.scale[offa + e] : 0.f; sb[e] = live ? t.scale[offb + e] : 0.f; }
-                }
+                for (int e = 0; e < VEC; ++e) { sa[e] = live ? t.scale[offa + e] : 0.f; sb[e] = live ? t.scale[offb + e] : 0.f; }
             }
-            for (int h = a0; h < a1; ++h) {
-                float xa[VEC], xb[VEC], ga[VEC], gb[VEC];
+            // heads of one token beside each other in the workgroup: its reads and writes are whole rows, token after token
+            const int all = here * t.H, qt = slots / t.H, rh = slots % t.H;
+            int tk = slot / t.H, h = slot % t.H;
+#pragma nounroll
+            for (int v0 = 0; v0 < all; v0 += slots * HB) {
+                RotVec<T, VEC> rx[HB][2], rd[HB][2];
+                int ti[HB], hi[HB];
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) xa[e] = xb[e] = ga[e] = gb[e] = 0.f;
-                if (ok) {
-                    if constexpr (!BWD || NORM) {
-                        const T* xp = reinterpret_cast<const T*>(t.x) + b * t.x_sb + (long)h * t.x_sh + (long)i * t.x_sn;
-                        rot_load<T, VEC>(xp + offa, xa); rot_load<T, VEC>(xp + offb, xb);
-                    }
-                    if constexpr (BWD) {
-                        const T* dp = reinterpret_cast<const T*>(t.dy) + b * t.d_sb + (long)h * t.d_sh + (long)i * t.d_sn;
-                        rot_load<T, VEC>(dp + offa, ga); rot_load<T, VEC>(dp + offb, gb);
-                    }
-                }
-                float inv = 1.f;
-                if constexpr (NORM) {
-                    float ss = 0.f;
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) ss = __builtin_fmaf(xa[e], xa[e], __builtin_fmaf(xb[e], xb[e], ss));
-                    ss = rot_group_sum(ss, G);
-                    inv = 1.f / fmaxf(sqrtf(ss), 1e-12f);      // F.normalize eps (mmp.py:41-42)
-                }
-                if constexpr (!BWD) {
-                    if constexpr (NORM) {
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) { xa[e] = xa[e] * inv * sa[e]; xb[e] = xb[e] * inv * sb[e]; }
-                    }
-                    rot_turn<VEC>(xa, xb, c, s, inter);
-                } else {
-                    rot_turn<VEC>(ga, gb, c, s, inter);
-                    if constexpr (NORM) {
-                        float dot = 0.f;
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            xa[e] *= inv; xb[e] *= inv;
-                            acc[w][0][e] = __builtin_fmaf(ga[e], xa[e], acc[w][0][e]);
-                            acc[w][1][e] = __builtin_fmaf(gb[e], xb[e], acc[w][1][e]);
-                            ga[e] *= sa[e]; gb[e] *= sb[e];
-                            dot = __builtin_fmaf(xa[e], ga[e], __builtin_fmaf(xb[e], gb[e], dot));
+                for (int y = 0; y < HB; ++y) {
+                    const bool ok = live && v0 + y * slots + slot < all;
+                    ti[y] = ok ? tk : -1; hi[y] = h;
+                    if (ok) {
+                        const long token = tok0 + tk;
+                        const int b = (int)(token / p.n), i = (int)(token - (long)b * p.n);
+                        if constexpr (!BWD || NORM) {
+                            const T* xp = reinterpret_cast<const T*>(t.x) + b * t.x_sb + (long)h * t.x_sh + (long)i * t.x_sn;
+                            rx[y][0] = *reinterpret_cast<const RotVec<T, VEC>*>(xp + offa); rx[y][1] = *reinterpret_cast<const RotVec<T, VEC>*>(xp + offb);
                         }
-                        dot = rot_group_sum(dot, G);
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) { xa[e] = __builtin_fmaf(-xa[e], dot, ga[e]) * inv; xb[e] = __builtin_fmaf(-xb[e], dot, gb[e]) * inv; }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) { xa[e] = ga[e]; xb[e] = gb[e]; }
+                        if constexpr (BWD) {
+                            const T* dp = reinterpret_cast<const T*>(t.dy) + b * t.d_sb + (long)h * t.d_sh + (long)i * t.d_sn;
+                            rd[y][0] = *reinterpret_cast<const RotVec<T, VEC>*>(dp + offa); rd[y][1] = *reinterpret_cast<const RotVec<T, VEC>*>(dp + offb);
+                        }
                     }
+                    h += rh; tk += qt;
+                    if (h >= t.H) { h -= t.H; ++tk; }
                 }
-                if (ok) {
-                    T* op = reinterpret_cast<T*>(t.out) + (tok * t.H + h) * p.d;
-                    rot_store<T, VEC>(op + offa, xa); rot_store<T, VEC>(op + offb, xb);
+#pragma unroll
+                for (int y = 0; y < HB; ++y) {
+                    const bool ok = ti[y] >= 0;
+                    float xa[VEC], xb[VEC], ga[VEC], gb[VEC], c[VEC], s[VEC];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        xa[e] = xb[e] = ga[e] = gb[e] = 0.f;
+                        const float2 cs = ok ? turns[ti[y] * pairs + u * VEC + e] : make_float2(1.f, 0.f);
+                        c[e] = cs.x; s[e] = cs.y;
+                        if (ok) {
+                            if constexpr (!BWD || NORM) { xa[e] = rot_ld<T>(rx[y][0].v[e]); xb[e] = rot_ld<T>(rx[y][1].v[e]); }
+                            if constexpr (BWD) { ga[e] = rot_ld<T>(rd[y][0].v[e]); gb[e] = rot_ld<T>(rd[y][1].v[e]); }
+                        }
+                    }
+                    float inv = 1.f;
+                    if constexpr (NORM) {
+                        float ss = 0.f;
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) ss = __builtin_fmaf(xa[e], xa[e], __builtin_fmaf(xb[e], xb[e], ss));
+                        ss = rot_group_sum(ss, G);
+                        inv = 1.f / fmaxf(sqrtf(ss), 1e-12f);      // F.normalize eps (mmp.py:41-42)
+                    }
+                    if constexpr (!BWD) {
+                        if constexpr (NORM) {
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) { xa[e] = xa[e] * inv * sa[e]; xb[e] = xb[e] * inv * sb[e]; }
+                        }
+                        rot_turn<VEC, INTER>(xa, xb, c, s);
+                    } else {
+                        rot_turn<VEC, INTER>(ga, gb, c, s);
+                        if constexpr (NORM) {
+                            float dot = 0.f;
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) {
+                                xa[e] *= inv; xb[e] *= inv;
+                                acc[0][e] = __builtin_fmaf(ga[e], xa[e], acc[0][e]);
+                                acc[1][e] = __builtin_fmaf(gb[e], xb[e], acc[1][e]);
+                                ga[e] *= sa[e]; gb[e] *= sb[e];
+                                dot = __builtin_fmaf(xa[e], ga[e], __builtin_fmaf(xb[e], gb[e], dot));
+                            }
+                            dot = rot_group_sum(dot, G);
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) { xa[e] = __builtin_fmaf(-xa[e], dot, ga[e]) * inv; xb[e] = __builtin_fmaf(-xb[e], dot, gb[e]) * inv; }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) { xa[e] = ga[e]; xb[e] = gb[e]; }
+                        }
+                    }
+                    if (ok) {
+                        T* op = reinterpret_cast<T*>(t.out) + ((tok0 + ti[y]) * t.H + hi[y]) * p.d;
+                        rot_store<T, VEC>(op + offa, xa); rot_store<T, VEC>(op + offb, xb);
+                    }
                 }
             }
         }
-    }
-    if constexpr (NORM && BWD) {      // the workgroup's part of the scales' gradients: its token slots added in slot order
-        extern __shared__ float sm[];      // [slots][2][d]
-        if (live) {
+        if constexpr (NORM && BWD) {      // the workgroup's part of the scale's gradient: its slots added in order
+            extern __shared__ float sm[];      // [slots][d]
+            if (w == 1) __syncthreads();
+            if (live) {
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    sm[(slot * 2 + w) * p.d + offa + e] = acc[w][0][e];
-                    sm[(slot * 2 + w) * p.d + offb + e] = acc[w][1][e];
-                }
-        }
-        __syncthreads();
-        float* part = p.part + (long)(blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.d;
-        for (int col = threadIdx.x; col < 2 * p.d; col += 256) {
-            float v = 0.f;
-            for (int sl = 0; sl < slots; ++sl) v += sm[sl * 2 * p.d + col];
-            part[col] = v;
+                for (int e = 0; e < VEC; ++e) { sm[slot * p.d + offa + e] = acc[0][e]; sm[slot * p.d + offb + e] = acc[1][e]; }
+            }
+            __syncthreads();
+            float* part = p.part + ((long)blockIdx.x * 2 + w) * p.d;
+            for (int col = threadIdx.x; col < p.d; col += 256) {
+                float v = 0.f;
+                for (int sl = 0; sl < slots; ++sl) v += sm[sl * p.d + col];
+                part[col] = v;
+            }
         }
     }
 }
 
-struct RotPlan { int vec, G, gx, gy, hpb; };
+struct RotPlan { int vec, G, TB, gx; };
 
-// VEC = 8 where rows and pairs allow 16-byte accesses, else one pair per lane.  Workgroups: every token slot once, up to 2048 (8 per CU; more only lengthen the
-// scales' reduction); with fewer than 512 of them the heads are split until the card has work (a step of a decoder: 32 tokens).
-RotPlan rot_plan(int B, int n, int H, int d, int vec) {
+// VEC = 8 where rows and pairs allow 16-byte accesses, else one pair per lane.  Tokens a workgroup: as many as leave four workgroups a CU, two where each has parts of the
+// scales' gradients to add up (32 x 1024 tokens, 16 heads of 64, forward: 36 us with two and 31 with four; gradient behind the norm: 53 and 59); one for a step of a
+// decoder, at most what the turns have room for.  Up to 2048 workgroups, which then take several such groups.
+RotPlan rot_plan(int B, int n, int d, int vec, bool sums) {
     RotPlan r;
     r.vec = vec;
     int g = 1;
     while (g < d / (2 * vec)) g *= 2;
     r.G = g;
-    const long blocks = ((long)B * n + 256 / g - 1) / (256 / g);
+    const long tokens = (long)B * n;
+    const long most = ROT_TURNS / (d / 2), tb = tokens / (sums ? 512 : 1024);
+    r.TB = (int)(tb < 1 ? 1 : (tb > most ? most : tb));
+    const long blocks = (tokens + r.TB - 1) / r.TB;
     r.gx = (int)(blocks < 2048 ? blocks : 2048);
-    int split = 1;
-    while ((long)r.gx * split * 2 <= 512 && split * 2 <= H) split *= 2;
-    r.hpb = (H + split - 1) / split;
-    r.gy = (H + r.hpb - 1) / r.hpb;
     return r;
 }
 
+template <typename T, int VEC, bool INTER>
+void rot_launch_pairs(hipStream_t s, const RotArgs& a, const RotPlan& pl, bool norm, bool bwd) {
+    const dim3 g(pl.gx), blk(256);
+    const size_t sm = norm && bwd ? (size_t)(256 / pl.G) * a.d * sizeof(float) : 0;
+    if (norm && bwd) hipLaunchKernelGGL((rotary_kernel<T, VEC, true, true, INTER>), g, blk, sm, s, a);
+    else if (bwd) hipLaunchKernelGGL((rotary_kernel<T, VEC, false, true, INTER>), g, blk, 0, s, a);
+    else if (norm) hipLaunchKernelGGL((rotary_kernel<T, VEC, true, false, INTER>), g, blk, 0, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, VEC, false, false, INTER>), g, blk, 0, s, a);
+}
 template <typename T, int VEC>
 void rot_launch(hipStream_t s, const RotArgs& a, const RotPlan& pl, bool norm, bool bwd) {
-    const dim3 g(pl.gx, pl.gy), blk(256);
-    const size_t sm = norm && bwd ? (size_t)(256 / pl.G) * 2 * a.d * sizeof(float) : 0;
-    if (norm && bwd) hipLaunchKernelGGL((rotary_kernel<T, VEC, true, true>), g, blk, sm, s, a);
-    else if (bwd) hipLaunchKernelGGL((rotary_kernel<T, VEC, false, true>), g, blk, 0, s, a);
-    else if (norm) hipLaunchKernelGGL((rotary_kernel<T, VEC, true, false>), g, blk, 0, s, a);
-    else hipLaunchKernelGGL((rotary_kernel<T, VEC, false, false>), g, blk, 0, s, a);
+    if (a.interleaved) rot_launch_pairs<T, VEC, true>(s, a, pl, norm, bwd);
+    else rot_launch_pairs<T, VEC, false>(s, a, pl, norm, bwd);
 }
 
 bool rot_wide(const mm_rotary* r) {
@@ -301,8 +319,8 @@ int k_attention_spans(hipStream_t s, const int32_t* cu_q, long q_sb, const int32
 // rows [2 dim] of the scales' partial gradients; -1: a head too long for one pair per lane (64 lanes) whose rows do not allow 16-byte accesses
 long k_rotary_parts(const mm_rotary* r) {
     if (r->dim > 128 && !rot_wide(r)) return -1;
-    const RotPlan pl = rot_plan(r->batch, r->n, r->q.heads + r->k.heads, r->dim, rot_wide(r) ? 8 : 1);
-    return (long)pl.gx * pl.gy;
+    const RotPlan pl = rot_plan(r->batch, r->n, r->dim, rot_wide(r) ? 8 : 1, true);
+    return pl.gx;
 }
 
 int k_rotary(hipStream_t s, const mm_rotary* r, bool bwd, float* ws, float* dscales) {
@@ -321,15 +339,15 @@ int k_rotary(hipStream_t s, const mm_rotary* r, bool bwd, float* ws, float* dsca
     a.P = P; a.c1 = cum[0]; a.c2 = cum[1]; a.c3 = cum[2];
     a.B = r->batch; a.n = r->n; a.d = r->dim; a.interleaved = r->interleaved;
     const bool wide = rot_wide(r);
-    const RotPlan pl = rot_plan(r->batch, r->n, r->q.heads + r->k.heads, r->dim, wide ? 8 : 1);
-    a.G = pl.G; a.heads_per_block = pl.hpb; a.part = ws;
     const bool norm = r->normalize != 0;
-    if (pl.gx > 0 && pl.gy > 0) {
+    const RotPlan pl = rot_plan(r->batch, r->n, r->dim, wide ? 8 : 1, norm && bwd);
+    a.G = pl.G; a.TB = pl.TB; a.part = ws;
+    if (pl.gx > 0 && r->q.heads + r->k.heads > 0) {
         if (r->dtype == MM_DT_F32) { if (wide) rot_launch<float, 8>(s, a, pl, norm, bwd); else rot_launch<float, 1>(s, a, pl, norm, bwd); }
         else if (r->dtype == MM_DT_F16) { if (wide) rot_launch<_Float16, 8>(s, a, pl, norm, bwd); else rot_launch<_Float16, 1>(s, a, pl, norm, bwd); }
         else { if (wide) rot_launch<__bf16, 8>(s, a, pl, norm, bwd); else rot_launch<__bf16, 1>(s, a, pl, norm, bwd); }
         const int rc = mm_check_launch("rotary_kernel");
         if (rc) return rc;
     }
-    return norm && bwd ? k_colsum(s, ws, pl.gx * pl.gy, 2 * r->dim, dscales) : MM_OK;      // (no rows: zeros)
+    return norm && bwd ? k_colsum(s, ws, pl.gx, 2 * r->dim, dscales) : MM_OK;      // (no rows: zeros)
 }
