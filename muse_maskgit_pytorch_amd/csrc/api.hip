@@ -468,7 +468,7 @@ int mm_attention_bwd(mm_stream_t stream, const void* q, int64_t q_sb, int64_t q_
 
 int mm_attention_spans(mm_stream_t stream, const int32_t* cu_q, int64_t q_sb, const int32_t* cu_k, int64_t k_sb, const int32_t* prefix, int64_t p_sb,
                        int B, int docs, int n, int j, int causal, int32_t* out) {
-    if (B < 0 || n < 0 || j < 0 || docs < 0 || B > 65535) return mm_set_error(MM_ERR_SHAPE, "attention_spans: sizes (batch <= 65535)");
+    if (B < 0 || n < 0 || j < 0 || docs < 0 || docs > (1 << 30) || n > (1 << 30) || B > 65535) return mm_set_error(MM_ERR_SHAPE, "attention_spans: sizes (batch <= 65535, 2^30 rows)");
     if (B == 0 || n == 0) return MM_OK;
     CHK_PTR(cu_q, "cu_q"); CHK_PTR(cu_k, "cu_k"); CHK_PTR(out, "out");
     if (((uintptr_t)out) & 7) return mm_set_error(MM_ERR_ALIGN, "attention_spans: out must be 8-byte aligned");
@@ -543,11 +543,12 @@ static int span_check(const mm_span_attn* a, bool bwd) {
     if (a->dim != 32 && a->dim != 64 && a->dim != 128) return mm_set_error(MM_ERR_UNSUPPORTED, "span attention: dim 32, 64 or 128");
     if (a->batch < 0 || a->nq < 0 || a->nk < 0 || a->heads_q < 1 || a->heads_k < 1 || a->heads_q % a->heads_k || a->heads_q > 1024)
         return mm_set_error(MM_ERR_SHAPE, "span attention: sizes (heads_k divides heads_q, at most 1024 heads)");
-    if (a->batch > (1 << 20) || a->nq > (1 << 28) || a->nk > (1 << 28) || (int64_t)a->batch * a->heads_q * ((a->nq + 31) / 32 + 1) > (1 << 28) ||
-        (int64_t)a->batch * a->heads_q * ((a->nk + 31) / 32 + 1) > (1 << 28))
+    // (a launch has less than 2^32 threads in a direction; the most are the backward's, 512 per 32 rows of a head)
+    const int64_t rows = (int64_t)a->batch * a->heads_q * ((a->nq + 31) / 32 + 1), keys = (int64_t)a->batch * a->heads_q * ((a->nk + 31) / 32 + 1);
+    if (a->batch > (1 << 20) || a->nq > (1 << 26) || a->nk > (1 << 26) || rows > (1 << 22) || (bwd && keys > (1 << 22)))
         return mm_set_error(MM_ERR_SHAPE, "span attention: too many rows for one call");
-    if (!(a->scale > 0.f) || a->scale > 1e30f) return mm_set_error(MM_ERR_SHAPE, "span attention: scale must be positive");
-    if (!(a->softcap >= 0.f) || a->softcap > 1e30f) return mm_set_error(MM_ERR_SHAPE, "span attention: softcap must be 0 (none) or positive");
+    if (!(a->scale >= 1e-20f) || a->scale > 1e20f) return mm_set_error(MM_ERR_SHAPE, "span attention: scale must be positive (1e-20 .. 1e20)");
+    if (a->softcap != 0.f && (!(a->softcap >= 1e-3f) || a->softcap > 1e4f)) return mm_set_error(MM_ERR_SHAPE, "span attention: softcap must be 0 (none) or 1e-3 .. 1e4");
     if (a->axes < 0 || a->axes > 3 || (a->slopes && a->axes == 0)) return mm_set_error(MM_ERR_SHAPE, "span attention: 1 to 3 axes for the distance bias");
     if (a->slopes && (!a->positions_q || !a->positions_k)) return mm_set_error(MM_ERR_SHAPE, "span attention: slopes need positions of queries and keys");
     if (a->spans && (((uintptr_t)a->spans) & 7)) return mm_set_error(MM_ERR_ALIGN, "span attention: spans must be 8-byte aligned");

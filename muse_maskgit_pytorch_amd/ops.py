@@ -897,11 +897,11 @@ def attention_spans(cu_q, n, cu_k=None, j=None, prefix=None, causal=False):
         if cu_k is not None:
             raise _Err('attention_spans: cu_k needs the number of keys j')
         j = n
-    if not (0 <= n < 2 ** 31 and 0 <= j < 2 ** 31):
-        raise _Err('attention_spans: n and j from 0 to 2^31 - 1')
+    if not (0 <= n <= 2 ** 30 and 0 <= j < 2 ** 31):
+        raise _Err('attention_spans: n from 0 to 2^30, j from 0 to 2^31 - 1')
     if prefix is not None and not causal:
         raise _Err('attention_spans: a prefix without causal order says nothing')
-    b, args, keep = 0, [], []
+    b, args, keep = None, [], []
     for t, width, what in ((cu_q, docs + 1, 'cu_q needs at least one bound'), (cu_q if cu_k is None else cu_k, docs + 1, 'cu_q and cu_k of one length'),
                            (prefix, docs, 'one prefix per document')):
         if t is None:
@@ -913,13 +913,13 @@ def attention_spans(cu_q, n, cu_k=None, j=None, prefix=None, causal=False):
         if s[-1] != width or docs < 0:
             raise _Err('attention_spans: ' + what)
         if len(s) == 2:
-            if b and s[0] != b:
+            if b is not None and s[0] != b:
                 raise _Err('attention_spans: tables of different batch sizes')
             b = s[0]
         t = t.contiguous()
         keep.append(t)
         args += (t.data_ptr(), width if len(s) == 2 else 0)
-    batched = any(t.dim() == 2 for t in keep)
+    batched = b is not None
     stream = _one_device(*keep)
     out = torch.empty((b, n, 2) if batched else (n, 2), dtype=torch.int32, device=cu_q.device)
     L.check(L.lib().mm_attention_spans(stream, *args, b if batched else 1, docs, n, j, int(causal), out.data_ptr()), 'mm_attention_spans')
@@ -1035,10 +1035,10 @@ def _span_args(q, k, v, spans, scale, softcap, slopes, positions, key_positions,
         raise _Err(f'attend_spans: width 32, 64 or 128, not {d}')
     if hk < 1 or hq < 1 or hq % hk:
         raise _Err(f'attend_spans: {hq} query heads over {hk} key heads')
-    if not 0 < scale < 1e30:
-        raise _Err(f'attend_spans: scale {scale} is not positive')
-    if not 0 <= softcap < 1e30:
-        raise _Err(f'attend_spans: softcap {softcap} is neither 0 nor positive')
+    if not 1e-20 <= scale <= 1e20:
+        raise _Err(f'attend_spans: scale {scale} is not positive (1e-20 .. 1e20)')
+    if softcap != 0 and not 1e-3 <= softcap <= 1e4:
+        raise _Err(f'attend_spans: softcap {softcap} is neither 0 nor 1e-3 .. 1e4')
     st = []
     for t in (q, k, v):
         z = t.stride()
@@ -1087,7 +1087,7 @@ def _span_args(q, k, v, spans, scale, softcap, slopes, positions, key_positions,
 def attend_spans(q, k, v, spans=None, scale=8.0, softcap=0.0, slopes=None, positions=None, key_positions=None, key_mask=None, return_lse=False, out_rows=False):
     """Attention of packed rows: q (b, hq, n, d), k / v (b, hk, j, d), bf16 or fp16, d = 32 / 64 / 128, hk a divisor of hq (shared key heads), strided views
     with 16-byte aligned rows.  A query sees the keys of its span (int32 (n, 2) or (b, n, 2), ops.attention_spans; None: all) that key_mask (b, j) keeps.
-    softcap > 0: scores are softcap * tanh(score / softcap).  slopes fp32 (hq, axes) and positions / key_positions int32 (n, axes) / (j, axes) (or (b, .., axes);
+    softcap > 0 (1e-3 .. 1e4; the score keeps the absolute precision of softcap in fp32): scores are softcap * tanh(score / softcap).  slopes fp32 (hq, axes) and positions / key_positions int32 (n, axes) / (j, axes) (or (b, .., axes);
     key_positions default: positions): sum over the axes of slope * |distance| is taken off the score; |position| < 2^30.  A row that sees nothing gives 0
     (lse -inf); what a row does not see never reaches it, infinities and NaN included.  Returns (b, hq, n, d) (a view of rows), out_rows: [b * n, hq * d], and with
     return_lse also the log of the sum of exp(score), fp32 (b, hq, n)."""

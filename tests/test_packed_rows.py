@@ -165,3 +165,28 @@ def test_plain_attention_gradients_are_autograds(cap, axes):
     got = R.attention(q, k, v, seen, 0.3, cap, slopes, pq, pk, dout=w, out=f['out'], lse=f['lse'])
     for name, want in zip(('dq', 'dk', 'dv', 'dslopes'), grads):
         assert torch.allclose(got[name], want, rtol=0, atol=1e-9), name
+
+
+@pytest.mark.parametrize('match,change', [('not positive', dict(scale=1e-30)), ('not positive', dict(scale=1e30)), ('softcap', dict(softcap=1e-9)), ('softcap', dict(softcap=1e6))])
+def test_attention_refuses_numbers_that_leave_32_bits(match, change):
+    refuses(match, ops.attend_spans, **att(**change))
+    lib = _lib.lib()
+    for f, v in change.items():
+        assert lib.mm_span_attention(None, _lib.C.byref(span_desc(**{f: v})), None, 0) == -1
+
+
+def test_spans_refuse_tables_of_no_rows_beside_tables_of_some():
+    cu, none = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(0, 4, dtype=torch.int32)
+    refuses('batch sizes', ops.attention_spans, none, 5, cu, 5)
+    refuses('batch sizes', ops.attention_spans, cu, 5, none, 5)
+    refuses('2\\^30', ops.attention_spans, cu, 2 ** 31 - 1)
+    assert _lib.lib().mm_attention_spans(None, 4096, 0, 4096, 0, None, 0, 1, 3, 2 ** 31 - 1, 5, 0, 4096) == -1
+
+
+def test_c_sizes_of_a_long_cache_are_taken_forward_alone():
+    """64 sequences of one new position over 2^22 keys: the blocks of 32 keys count only where a launch has threads for each (the backward)"""
+    lib = _lib.lib()
+    d = span_desc(batch=64, heads_q=32, heads_k=4, nq=1, nk=1 << 22)      # (256 workgroups: the keys are split in two)
+    assert lib.mm_span_attention_workspace_bytes(_lib.C.byref(d)) == 2 * 256 * 32 * (64 + 2) * 4
+    assert lib.mm_span_attention_bwd_workspace_bytes(_lib.C.byref(d)) == 0
+    assert lib.mm_span_attention_bwd(None, _lib.C.byref(d), None, 0) == -1
