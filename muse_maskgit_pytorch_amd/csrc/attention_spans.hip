@@ -24,18 +24,12 @@ __device__ __forceinline__ void row_again(const SpanArgs& p, int b, int h, int i
     const uint16_t* vb = p.v + b * p.v_s[0] + hk * p.v_s[1];
     o[0] = o[1] = 0.f;
 #pragma nounroll
-    for (int t0 = k0; t0 < k1; t0 += 64) {
+    for (int t0 = k0; t0 < k1 && !all_nan<D>(o, lane); t0 += 64) {
         const int key = t0 + lane;
+        const bool sees = key < k1 && (!p.kmask || p.kmask[b * p.km_sb + key]);
         float w = 0.f, unused;
-        if (key < k1 && (!p.kmask || p.kmask[b * p.km_sb + key])) w = __builtin_amdgcn_exp2f(pair_score<D, F16, AX>(p, q, kb + (long)key * p.k_s[2], b, h, i, key, &unused) - m);
-#pragma nounroll
-        for (int e = 0; e < min(64, k1 - t0); ++e) {
-            const float we = __shfl(w, e, 64);
-            if (p.kmask && !p.kmask[b * p.km_sb + t0 + e]) continue;
-            const uint16_t* v = vb + (long)(t0 + e) * p.v_s[2];
-            if (lane < D) o[0] = __builtin_fmaf(we, to_f32<F16>(v[lane]), o[0]);
-            if (D > 64) o[1] = __builtin_fmaf(we, to_f32<F16>(v[lane + 64]), o[1]);
-        }
+        if (sees) w = __builtin_amdgcn_exp2f(pair_score<D, F16, AX>(p, q, kb + (long)key * p.k_s[2], b, h, i, key, &unused) - m);
+        rows_add<D, F16>(o, __ballot(sees), w, vb + (long)t0 * p.v_s[2], p.v_s[2], min(64, k1 - t0), lane);
     }
 }
 

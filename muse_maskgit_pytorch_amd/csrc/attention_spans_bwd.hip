@@ -109,21 +109,15 @@ __device__ __forceinline__ void query_again(const SpanArgs& p, int b, int h, int
     const uint16_t* vb = p.v + b * p.v_s[0] + hk * p.v_s[1];
     o[0] = o[1] = 0.f;
 #pragma nounroll
-    for (int t0 = k0; t0 < k1; t0 += 64) {
+    for (int t0 = k0; t0 < k1 && !all_nan<D>(o, lane); t0 += 64) {
         const int key = t0 + lane;
+        const bool sees = key < k1 && (!p.kmask || p.kmask[b * p.km_sb + key]);
         float w = 0.f, slope;
-        if (key < k1 && (!p.kmask || p.kmask[b * p.km_sb + key])) {
+        if (sees) {
             const float s = pair_score<D, false, AX>(p, q, kb + (long)key * p.k_s[2], b, h, i, key, &slope);
             w = __builtin_amdgcn_exp2f(s - lse2) * (row_dot<D, false>(g, vb + (long)key * p.v_s[2]) - delta) * slope;
         }
-#pragma nounroll
-        for (int e = 0; e < min(64, k1 - t0); ++e) {
-            const float we = __shfl(w, e, 64);
-            if (p.kmask && !p.kmask[b * p.km_sb + t0 + e]) continue;
-            const uint16_t* k = kb + (long)(t0 + e) * p.k_s[2];
-            if (lane < D) o[0] = __builtin_fmaf(we, bf16_to_f32(k[lane]), o[0]);
-            if (D > 64) o[1] = __builtin_fmaf(we, bf16_to_f32(k[lane + 64]), o[1]);
-        }
+        rows_add<D, false>(o, __ballot(sees), w, kb + (long)t0 * p.k_s[2], p.k_s[2], min(64, k1 - t0), lane);
     }
 }
 
@@ -150,17 +144,11 @@ __device__ __forceinline__ void key_again(const SpanArgs& p, int b, int hk, int 
                 w = __builtin_amdgcn_exp2f(s - p.lse[row] * SPAN_LOG2E);
                 ds = w * (row_dot<D, false>(p.dout + b * p.do_s[0] + h * p.do_s[1] + (long)i * p.do_s[2], v) - p.delta[row]) * slope;
             }
-            unsigned long long todo = __ballot(sees);
-#pragma nounroll
-            while (todo) {
-                const int e = __builtin_ctzll(todo);
-                todo &= todo - 1;
-                const float we = __shfl(w, e, 64), de = __shfl(ds, e, 64);
-                const uint16_t* q = p.q + b * p.q_s[0] + h * p.q_s[1] + (long)(t0 + e) * p.q_s[2];
-                const uint16_t* g = p.dout + b * p.do_s[0] + h * p.do_s[1] + (long)(t0 + e) * p.do_s[2];
-                if (lane < D) { dk[0] = __builtin_fmaf(de, bf16_to_f32(q[lane]), dk[0]); dv[0] = __builtin_fmaf(we, bf16_to_f32(g[lane]), dv[0]); }
-                if (D > 64) { dk[1] = __builtin_fmaf(de, bf16_to_f32(q[lane + 64]), dk[1]); dv[1] = __builtin_fmaf(we, bf16_to_f32(g[lane + 64]), dv[1]); }
-            }
+            const unsigned long long seen = __ballot(sees);
+            if (!seen) continue;
+            rows_add<D, false>(dk, seen, ds, p.q + b * p.q_s[0] + h * p.q_s[1] + (long)t0 * p.q_s[2], p.q_s[2], min(64, p.nq - t0), lane);
+            rows_add<D, false>(dv, seen, w, p.dout + b * p.do_s[0] + h * p.do_s[1] + (long)t0 * p.do_s[2], p.do_s[2], min(64, p.nq - t0), lane);
+            if (all_nan<D>(dk, lane) && all_nan<D>(dv, lane)) return;
         }
 }
 

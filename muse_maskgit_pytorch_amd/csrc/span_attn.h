@@ -148,7 +148,7 @@ __device__ __forceinline__ float span_bias(const int (&pq)[AX ? AX : 1], const f
 template <int D, bool F16>
 __device__ __forceinline__ float row_dot(const uint16_t* x, const uint16_t* y) {
     float s = 0.f;
-#pragma nounroll
+#pragma unroll 4
     for (int c = 0; c < D; c += 8) {
         const u32x4_t a = *reinterpret_cast<const u32x4_t*>(x + c), b = *reinterpret_cast<const u32x4_t*>(y + c);
 #pragma unroll
@@ -159,6 +159,31 @@ __device__ __forceinline__ float row_dot(const uint16_t* x, const uint16_t* y) {
     }
     return s;
 }
+
+// o += sum over the set bits e of `sees` of w[lane e] * (row e of x)[lane], lane = element (o[1]: element lane + 64): eight rows' loads at a time.  Rows whose bit is clear
+// are read where they lie (below `rows`) but not added, whatever they hold
+template <int D, bool F16>
+__device__ __forceinline__ void rows_add(float (&o)[2], unsigned long long sees, float w, const uint16_t* x, long stride, int rows, int lane) {
+#pragma nounroll
+    for (int e0 = 0; e0 < rows; e0 += 8) {
+        if (((sees >> e0) & 0xFFull) == 0) continue;
+        float a[8], c[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            const uint16_t* r = x + (long)min(e0 + y, rows - 1) * stride;
+            a[y] = to_f32<F16>(r[D >= 64 ? lane : lane & (D - 1)]);
+            c[y] = D > 64 ? to_f32<F16>(r[lane + 64]) : 0.f;
+        }
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            const float we = __shfl(w, e0 + y, 64);      // (e0 + y <= 63)
+            if ((sees >> (e0 + y)) & 1ull) { o[0] = __builtin_fmaf(we, a[y], o[0]); o[1] = __builtin_fmaf(we, c[y], o[1]); }
+        }
+    }
+}
+// nothing finite can come back: every element of the sum is NaN
+template <int D>
+__device__ __forceinline__ bool all_nan(const float (&o)[2], int lane) { return __all((lane >= D || o[0] != o[0]) && (D <= 64 || o[1] != o[1])); }
 
 // score (log2 units) of one visible pair by one lane; *slope: derivative of the cap
 template <int D, bool F16, int AX>

@@ -492,3 +492,39 @@ def test_packed_rows_on_a_stream_of_their_own():
         got = ops.attend_spans_bwd(q, k, v, out, lse, q)
     side.synchronize()
     assert torch.equal(out, want) and torch.equal(lse, wl) and all(torch.equal(a, c) for a, c in zip(got[:3], wb[:3]))
+
+
+@pytest.mark.parametrize('d,cap,axes', [(32, 0.0, 1), (64, 0.0, 0), (128, 20.0, 2)])
+def test_one_broken_element_in_many_rows(d, cap, axes):
+    """one NaN in v, seen by all, and one in dout: every row and key is computed again on its own, and only what the formula reaches is NaN"""
+    x, out, lse, dout = bwd_inputs((1, 4, 2, 1100, 1100, d, 'bf16', 'none', cap, axes), 91)
+    want = {**plain(x), **plain(x, dout=dout, out=out, lse=lse)}
+    args, kw = on_gpu(x)
+    v = args[2].clone()
+    v[0, 1, 700, 3] = math.nan
+    got = ops.attend_spans(args[0], args[1], v, args[3], **kw)
+    assert got[:, 2:, :, 3].isnan().all() and got.isnan().sum() == 2 * 1100
+    clean = ~got.isnan().cpu()
+    R.check(got.cpu()[clean], want['out'][clean], want['out_tol'][clean], 'out')
+    g = dout.clone()
+    g[0, 3, 50, 5] = math.nan                                   # row 50 of head 3 (key head 1)
+    dq, dk, dv, ds = ops.attend_spans_bwd(*args[:3], out.to(DEV), lse.to(DEV), g.to(DEV), args[3], **kw)
+    assert dq[0, 3, 50].isnan().all() and dq.isnan().sum() == d
+    assert dk[0, 1].isnan().all() and dk.isnan().sum() == 1100 * d
+    assert dv[0, 1, :, 5].isnan().all() and dv.isnan().sum() == 1100
+    for name, t in (('dq', dq), ('dk', dk), ('dv', dv)):
+        clean = ~t.isnan().cpu()
+        R.check(t.cpu()[clean], want[name][clean], want[name + '_tol'][clean], name)
+    if axes:
+        assert ds[3].isnan().all() and ds.isnan().sum() == axes
+
+
+def test_everything_broken_ends_soon():
+    """a diverged step: all of dout NaN.  Rows and keys stop at their first NaN sum instead of walking every pair"""
+    g = gen(92)
+    q, k, v = (torch.randn(1, 4, 4096, 64, generator=g).to(torch.bfloat16).to(DEV) for _ in range(3))
+    out, lse = ops.attend_spans(q, k, v, return_lse=True)
+    dq, dk, dv, _ = ops.attend_spans_bwd(q, k, v, out, lse, torch.full_like(out, math.nan))
+    assert dq.isnan().all() and dk.isnan().all() and dv.isnan().all()
+    out, lse = ops.attend_spans(q, k, torch.full_like(v, math.nan), return_lse=True)
+    assert out.isnan().all() and lse.isfinite().all()
