@@ -52,8 +52,9 @@ struct Form {
         for (int a = 0; a < AX; ++a) sl[a] = CAP ? p.slopes[h * AX + a] * SPAN_LOG2E : p.slopes[h * AX + a] / p.scale;
     }
     float c2;
-    // 4 consecutive keys (pk: their positions, [axis][stride])
-    __device__ __forceinline__ void y4(f32x16_t& s, int r, const int (&pq)[AX ? AX : 1], const int* pk, int stride) const {
+    // 4 consecutive keys (k: their positions).  Positions are whole numbers below 2^24, exact in fp32 and so are their differences: a subtraction and a
+    // multiply-add with |.| an axis and score
+    __device__ __forceinline__ void y4(f32x16_t& s, int r, const float (&pq)[AX ? AX : 1], const f32x4_t (&k)[AX ? AX : 1]) const {
         float v[4] = {s[r], s[r + 1], s[r + 2], s[r + 3]};
         if constexpr (CAP) {
 #pragma unroll
@@ -64,11 +65,10 @@ struct Form {
         }
 #pragma unroll
         for (int a = 0; a < AX; ++a) {
-            const i32x4_t k = lds_i4(pk + a * stride);
-            v[0] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.x)), v[0]);
-            v[1] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.y)), v[1]);
-            v[2] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.z)), v[2]);
-            v[3] = __builtin_fmaf(-sl[a], fabsf((float)(pq[a] - k.w)), v[3]);
+            v[0] = __builtin_fmaf(-sl[a], fabsf(pq[a] - k[a].x), v[0]);
+            v[1] = __builtin_fmaf(-sl[a], fabsf(pq[a] - k[a].y), v[1]);
+            v[2] = __builtin_fmaf(-sl[a], fabsf(pq[a] - k[a].z), v[2]);
+            v[3] = __builtin_fmaf(-sl[a], fabsf(pq[a] - k[a].w), v[3]);
         }
         s[r] = v[0]; s[r + 1] = v[1]; s[r + 2] = v[2]; s[r + 3] = v[3];
     }
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int tiles = (p.nq + WQ - 1) / WQ;
     int rt, h;
-    if (!span_item(p.order, p.Hq, p.B * tiles, rt, h)) return;
+    if (!span_item(blockIdx.x, p.order, p.Hq, p.B * tiles, rt, h)) return;
     const int tile = rt % tiles, b = rt / tiles, hk = h / (p.Hq / p.Hk);
     const int i = tile * WQ + w * 32 + (lane & 31);
     const bool ok = i < p.nq;
@@ -154,9 +154,9 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) qf[c] = *reinterpret_cast<const u32x4_t*>(qp + c * 16);
     }
-    int pq[AX ? AX : 1];
+    float pq[AX ? AX : 1];
 #pragma unroll
-    for (int a = 0; a < AX; ++a) pq[a] = ok ? p.pos_q[b * p.pq_sb + (long)i * AX + a] : 0;
+    for (int a = 0; a < AX; ++a) pq[a] = ok ? (float)p.pos_q[b * p.pq_sb + (long)i * AX + a] : 0.f;
     Form<CAP, AX> F;
     F.init(p, h);
     __syncthreads();
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
     };
     const auto pos_store = [&](int it) {
         if constexpr (AX > 0) {
-            if (t < KT * AX) reinterpret_cast<int*>(smem + (it & 1) * STAGE + 2 * T::BYTES)[(t % AX) * KT + t / AX] = posv;
+            if (t < KT * AX) reinterpret_cast<float*>(smem + (it & 1) * STAGE + 2 * T::BYTES)[(t % AX) * KT + t / AX] = (float)posv;
         }
     };
     const auto sees = [&](int it) { return it < nt && __any(lo < k0 + it * KT + KT && hi > k0 + it * KT); };
@@ -200,6 +200,11 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
     const auto mix = [&](int it, f32x16_t (&s)[2], f32x16_t (&sn)[2], auto with_next, auto with_this) {
         const unsigned char* Kn = smem + ((it + 1) & 1) * STAGE;
         int pos = (it & 1) * STAGE + 2 * T::BYTES + half * 16;
+        // positions of this group of four keys and of the next (their read waits in the open otherwise: 2 x 16 heads of 4096 x 4096, 64 wide, two axes 279 us, 256 so)
+        f32x4_t pk[AX ? AX : 1], pn[AX ? AX : 1];
+        if constexpr (with_this.value && AX > 0)
+#pragma unroll
+            for (int a = 0; a < AX; ++a) pk[a] = lds_f4(smem + pos + a * KT * 4);
         u32x4_t f0, f1;
         if constexpr (with_next.value) {
 #pragma unroll
@@ -218,7 +223,11 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
 #pragma unroll
                 for (int x = 0; x < E; ++x) {
                     const int g = c * E + x;
-                    F.y4(s[g >> 2], (g & 3) * 4, pq, reinterpret_cast<const int*>(smem + pos) + (g >> 2) * 32 + (g & 3) * 8, KT);
+                    if constexpr (AX > 0)
+                        if (g < 7)
+#pragma unroll
+                            for (int a = 0; a < AX; ++a) pn[a] = lds_f4(smem + pos + a * KT * 4 + ((g + 1) >> 2) * 128 + ((g + 1) & 3) * 32);
+                    F.y4(s[g >> 2], (g & 3) * 4, pq, pk);
                     // y of these four now, the next group's positions behind it: left alone, the compiler moves three of the four behind the branch on the mask and keeps
                     // the positions of all 64 keys until then (32 registers an axis: a wave per SIMD)
                     if constexpr (AX > 0) {
@@ -227,6 +236,8 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
                         float y0 = y[r], y1 = y[r + 1], y2 = y[r + 2], y3 = y[r + 3];
                         asm volatile("" : "+v"(pos), "+v"(y0), "+v"(y1), "+v"(y2), "+v"(y3));
                         y[r] = y0; y[r + 1] = y1; y[r + 2] = y2; y[r + 3] = y3;
+#pragma unroll
+                        for (int a = 0; a < AX; ++a) pk[a] = pn[a];
                     }
                 }
             }
@@ -374,9 +385,9 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) qf[c] = *reinterpret_cast<const u32x4_t*>(qp + c * 16);
     }
-    int pq[AX ? AX : 1];
+    float pq[AX ? AX : 1];
 #pragma unroll
-    for (int a = 0; a < AX; ++a) pq[a] = p.pos_q[b * p.pq_sb + (long)i * AX + a];
+    for (int a = 0; a < AX; ++a) pq[a] = (float)p.pos_q[b * p.pq_sb + (long)i * AX + a];
     Form<CAP, AX> F;
     F.init(p, h);
     const uint16_t* kp = p.k + b * p.k_s[0] + hk * p.k_s[1];
@@ -404,11 +415,11 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
         const int t0 = k0 + tt * 32;
         unsigned char* Ks = mine + st * STAGE;
         unsigned char* Vs = Ks + T::BYTES;
-        int* pks = reinterpret_cast<int*>(Ks + 2 * T::BYTES);
+        float* pks = reinterpret_cast<float*>(Ks + 2 * T::BYTES);
         if constexpr (AX > 0) {
             if (lane < 32) {
 #pragma unroll
-                for (int a = 0; a < AX; ++a) pks[a * 32 + lane] = t0 + lane < k1 ? pkp[(long)(t0 + lane) * AX + a] : 0;
+                for (int a = 0; a < AX; ++a) pks[a * 32 + lane] = t0 + lane < k1 ? (float)pkp[(long)(t0 + lane) * AX + a] : 0.f;
             }
         }
         uint32_t keep = 0xFFFFFFFFu;
@@ -424,7 +435,12 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
         for (int c = 0; c < D / 16; ++c) s = mfma32<F16>(T::rows(Ks, c, 0, lane), qf[c], s);
         if constexpr (CAP || AX > 0)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) F.y4(s, g * 4, pq, pks + g * 8 + half * 4, 32);
+            for (int g = 0; g < 4; ++g) {
+                f32x4_t pk[AX ? AX : 1];
+#pragma unroll
+                for (int a = 0; a < AX; ++a) pk[a] = lds_f4(pks + a * 32 + g * 8 + half * 4);
+                F.y4(s, g * 4, pq, pk);
+            }
         if (keep != 0xFFFFFFFFu || !__all(lo <= t0 && hi >= t0 + 32)) F.hide(s, (uint32_t)((bit_range(lo - t0, hi - t0) & (unsigned long long)keep) >> (4 * half)));
         rescale<D>(F.score(F.extreme(s, Form<CAP, AX>::worst())), m, l, o);
         const float kbm = F.kb - m;
@@ -519,7 +535,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
 // joins the splits of a row in split order: D / 4 threads a row
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void span_attn_join(const SpanArgs p) {
-    constexpr int TPR = D / 4;
+    constexpr int TPR = D / 4, JOIN = 8;
     const long rows = (long)p.B * p.Hk * p.row_tiles * 32;
     const long r = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     const int c = threadIdx.x % TPR;
@@ -529,15 +545,31 @@ __global__ __launch_bounds__(256) void span_attn_join(const SpanArgs p) {
     if (in_head >= group * p.nq) return;
     const int hk = (int)(r / (p.row_tiles * 32)) % p.Hk, b = (int)(r / (p.row_tiles * 32) / p.Hk);
     const int h = hk * group + in_head / p.nq, i = in_head % p.nq;
-    float M = SPAN_LOW;
-    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[(s * rows + r) * 2]);
-    float L = 0.f;
+    float M = SPAN_LOW, L = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < p.splits; ++s) {
-        const float f = __builtin_amdgcn_exp2f(p.part_ml[(s * rows + r) * 2] - M);
-        L = __builtin_fmaf(p.part_ml[(s * rows + r) * 2 + 1], f, L);
-        const float4 y = *reinterpret_cast<const float4*>(p.part_o + (s * rows + r) * D + c * 4);
-        v.x = __builtin_fmaf(y.x, f, v.x); v.y = __builtin_fmaf(y.y, f, v.y); v.z = __builtin_fmaf(y.z, f, v.z); v.w = __builtin_fmaf(y.w, f, v.w);
+    for (int s0 = 0; s0 < p.splits; s0 += JOIN) {      // JOIN splits' reads go out together (one by one, each waits for the one before: 8 us for 8 splits of 64 x 4 rows, 5 so)
+        float2 ml[JOIN];
+        float4 y[JOIN];
+#pragma unroll
+        for (int x = 0; x < JOIN; ++x) {
+            const long at = min(s0 + x, p.splits - 1) * rows + r;
+            ml[x] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+            y[x] = *reinterpret_cast<const float4*>(p.part_o + at * D + c * 4);
+        }
+        float mn = M;
+#pragma unroll
+        for (int x = 0; x < JOIN; ++x) mn = fmaxf(mn, ml[x].x);
+        float f = __builtin_amdgcn_exp2f(M - mn);
+        M = mn;
+        L *= f;
+        v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+#pragma unroll
+        for (int x = 0; x < JOIN; ++x) {
+            if (s0 + x >= p.splits) break;
+            f = __builtin_amdgcn_exp2f(ml[x].x - M);
+            L = __builtin_fmaf(ml[x].y, f, L);
+            v.x = __builtin_fmaf(y[x].x, f, v.x); v.y = __builtin_fmaf(y[x].y, f, v.y); v.z = __builtin_fmaf(y[x].z, f, v.z); v.w = __builtin_fmaf(y[x].w, f, v.w);
+        }
     }
     const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
     *reinterpret_cast<uint2*>(p.out + b * p.o_s[0] + h * p.o_s[1] + (long)i * p.o_s[2] + c * 4) =

@@ -1,11 +1,12 @@
 // Attention of packed rows, backward, from q, k, v, out, lse and dout.  With p = exp(s - lse) and delta_i = sum_d dout_id out_id:
 //     dv = p^T dout,   ds = p (dout v^T - delta),   dslope_a = - sum ds |distance_a|,   dq = scale (ds cap') k,   dk = scale (ds cap')^T q
-// Three launches and no atomics, so every sum has one order:
-//   span_bwd_pre : delta per row (one read of out and dout) and, per 32 queries, the keys they see (lowest, highest bound; and whether all see the same whole range)
-//   span_bwd_dq  : 128 queries of a head (4 waves x 32), key tiles of 64: the forward's S^T form -- lse and delta belong to the lane; ds goes into dQ^T = K^T dS^T
-//   span_bwd_dkv : 128 keys of a key head (4 waves x 32), query tiles of 64 of every head that shares it: S = Q K^T puts a KEY into the lane's column, so dV^T = dO^T P
-//                  and dK^T = Q^T dS take P and dS from the accumulators as they are; only the query tiles whose keys meet this tile are visited
-// Recomputing S and dP in both kernels makes 7 products where 5 would do with atomic sums of dQ.  P and dS are rounded to bf16 as operands of the products; everything
+// Two launches (three where heads share keys), and every sum in one order:
+//   span_bwd_pre  : delta per row (one read of out and dout) and, per 32 queries, the keys they see (lowest, highest bound; and whether all see the same whole range)
+//   span_bwd_main : dq_tile,  128 queries of a head, key tiles of 64: the forward's S^T form -- lse and delta belong to the lane; ds goes into dQ^T = K^T dS^T
+//                   dkv_tile, 128 keys of a key head, query tiles of 64 of every head that shares it: S = Q K^T puts a KEY into the lane's column, so dV^T = dO^T P and
+//                   dK^T = Q^T dS take P and dS from the accumulators as they are; only the query tiles whose keys meet this tile are visited
+//   span_bwd_join : the parts of dk and dv of the heads that share a key head, in order
+// Recomputing S and dP in both makes 7 products where 5 would do with atomic sums of dQ.  P and dS are rounded to bf16 as operands of the products; everything
 // else (scores, exp, ds, delta, slopes' gradients) is fp32.
 #include <string.h>
 
@@ -27,7 +28,7 @@ __device__ __forceinline__ int2 row_span(const SpanArgs& p, int b, int h, int i)
     return make_int2(lo, hi);
 }
 
-// In one launch, all of it read by the other two:
+// In one launch, all of it read by the next:
 //   the first workgroup (where the order is wanted): the order of the query tiles
 //   then 8 blocks of 32 queries a workgroup: .x lowest, .y highest key bound (x >= y: nobody sees anything), .z / .w highest low and lowest high bound (a key tile
 //   inside them needs no mask).  By the spans alone: a row whose lse is -inf although its span is not empty (all of its keys masked) is found per tile
@@ -37,6 +38,7 @@ __global__ __launch_bounds__(256) void span_bwd_pre(const SpanArgs p) {
     constexpr int TPR = D / 8, RPB = 256 / TPR;
     __shared__ SpanOrderLds m;
     long block = blockIdx.x;
+    if (block == 0 && threadIdx.x == 0 && p.done) *p.done = 0;
     if (p.order_out) {
         if (block == 0) { span_order_tiles<256>(m, p.spans, p.spans_sb, p.B, p.nq, p.nk, p.order_out); return; }
         --block;
@@ -79,7 +81,7 @@ __global__ __launch_bounds__(256) void span_bwd_pre(const SpanArgs p) {
     }
 }
 
-// the slopes' gradients: the parts of the query tiles (and rows of the batch) in 32 chains, the chains in order; one workgroup, launched with dk and dv
+// the slopes' gradients: the parts of the query tiles (and rows of the batch) in 32 chains, the chains in order; by the workgroup of dq that is done last
 __device__ __forceinline__ void sum_slope_parts(const SpanArgs& p, int threads, float* red) {
     const int n = p.Hq * p.axes, t = threadIdx.x, lanes = threads / 32;      // threads / 32 columns at a time, 32 chains each
     const long parts = (long)p.B * ((p.nq + BQ - 1) / BQ);
@@ -152,17 +154,21 @@ __device__ __forceinline__ void key_again(const SpanArgs& p, int b, int hk, int 
         }
 }
 
-template <int D, int AX, bool CAP>
-__global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
+// GROUPS (two for 128 wide heads, where one workgroup fills a CU): waves 0 .. 3 take the even key tiles of the same 128 queries, waves 4 .. 7 the odd ones, joined at the end
+template <int D, int AX, int GROUPS>
+struct DqLds {
+    static constexpr int STAGE = 2 * Tile<D, BT>::BYTES + AX * BT * 4, BYTES = 2 * GROUPS * STAGE + 128;
+};
+template <int D, int AX, bool CAP, int GROUPS>
+__device__ __forceinline__ void dq_tile(const SpanArgs& p, unsigned id, unsigned char* smem) {
     typedef Tile<D, BT> T;
-    extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
-    constexpr int POS = AX * BT * 4, STAGE = 2 * T::BYTES + POS;
-    int* red = reinterpret_cast<int*>(smem + 2 * STAGE);
-    const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
-    const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+    constexpr int STAGE = DqLds<D, AX, GROUPS>::STAGE;
+    int* red = reinterpret_cast<int*>(smem + 2 * GROUPS * STAGE);
+    const int t = threadIdx.x & 255, lane = t & 63, half = lane >> 5;      // (t: of the 256 threads of a group)
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), w = wave & 3, grp = GROUPS > 1 ? wave >> 2 : 0;
     const int tiles = (p.nq + BQ - 1) / BQ;
     int rt, h;
-    if (!span_item(p.order, p.Hq, p.B * tiles, rt, h)) return;
+    if (!span_item(id, p.order, p.Hq, p.B * tiles, rt, h)) return;
     const int tile = rt % tiles, b = rt / tiles, hk = h / (p.Hq / p.Hk);
     const int i = tile * BQ + w * 32 + (lane & 31);
     const bool ok = i < p.nq;
@@ -185,17 +191,17 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) { qf[c] = *reinterpret_cast<const u32x4_t*>(qp + c * 16); gf[c] = *reinterpret_cast<const u32x4_t*>(gp + c * 16); }
     }
-    float sl[AX ? AX : 1], ds_sl[AX ? AX : 1]; int pq[AX ? AX : 1];
+    float sl[AX ? AX : 1], ds_sl[AX ? AX : 1], pq[AX ? AX : 1];
 #pragma unroll
     for (int a = 0; a < AX; ++a) {
         sl[a] = p.slopes[h * AX + a] * SPAN_LOG2E;
-        pq[a] = ok ? p.pos_q[b * p.pq_sb + (long)i * AX + a] : 0;
+        pq[a] = ok ? (float)p.pos_q[b * p.pq_sb + (long)i * AX + a] : 0.f;
         ds_sl[a] = 0.f;
     }
     __syncthreads();
     const int k0 = __builtin_amdgcn_readfirstlane(min(min(red[0], red[1]), min(red[2], red[3])));
     const int k1 = __builtin_amdgcn_readfirstlane(max(max(red[4], red[5]), max(red[6], red[7])));
-    const int nt = k1 > k0 ? (k1 - k0 + BT - 1) / BT : 0;
+    const int nt = k1 > k0 ? (k1 - k0 + GROUPS * BT - 1) / (GROUPS * BT) : 0;
     const uint16_t* kp = p.k + b * p.k_s[0] + hk * p.k_s[1];
     const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1];
     const uint8_t* km = p.kmask ? p.kmask + b * p.km_sb : nullptr;
@@ -204,15 +210,15 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
 
 #define SPAN_ISSUE(it_)                                                                                                \
     {                                                                                                                  \
-        const int t0_ = k0 + (it_) * BT;                                                                               \
-        unsigned char* st_ = smem + ((it_) & 1) * STAGE;                                                               \
+        const int t0_ = k0 + ((it_) * GROUPS + grp) * BT;                                                              \
+        unsigned char* st_ = smem + (((it_) & 1) * GROUPS + grp) * STAGE;                                              \
         T::template fill<4>(st_, kp + (long)t0_ * p.k_s[2], min(BT, k1 - t0_), (int)p.k_s[2], w, lane);                \
         T::template fill<4>(st_ + T::BYTES, vp + (long)t0_ * p.v_s[2], min(BT, k1 - t0_), (int)p.v_s[2], w, lane);     \
     }
 #define SPAN_POS_LOAD(it_) \
-    if constexpr (AX > 0) { if (t < BT * AX) { const int key_ = k0 + (it_) * BT + t / AX; posv = key_ < k1 ? pkp[(long)key_ * AX + t % AX] : 0; } }
+    if constexpr (AX > 0) { if (t < BT * AX) { const int key_ = k0 + ((it_) * GROUPS + grp) * BT + t / AX; posv = key_ < k1 ? pkp[(long)key_ * AX + t % AX] : 0; } }
 #define SPAN_POS_STORE(it_) \
-    if constexpr (AX > 0) { if (t < BT * AX) reinterpret_cast<int*>(smem + ((it_) & 1) * STAGE + 2 * T::BYTES)[(t % AX) * BT + t / AX] = posv; }
+    if constexpr (AX > 0) { if (t < BT * AX) reinterpret_cast<float*>(smem + (((it_) & 1) * GROUPS + grp) * STAGE + 2 * T::BYTES)[(t % AX) * BT + t / AX] = (float)posv; }
     f32x16_t dq[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
@@ -221,16 +227,21 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
     int posv = 0;
     if (nt > 0) { SPAN_ISSUE(0); SPAN_POS_LOAD(0); SPAN_POS_STORE(0); }
     for (int it = 0; it < nt; ++it) {
-        const int t0 = k0 + it * BT;
-        unsigned char* Ks = smem + (it & 1) * STAGE;
+        const int t0 = k0 + (it * GROUPS + grp) * BT;
+        unsigned char* Ks = smem + ((it & 1) * GROUPS + grp) * STAGE;
         unsigned char* Vs = Ks + T::BYTES;
-        const int* pks = reinterpret_cast<const int*>(Ks + 2 * T::BYTES);
-        unsigned long long keep = ~0ull;
-        if (km) keep = __ballot(t0 + lane < k1 && km[t0 + lane]);
+        unsigned long long keep = ~0ull, all = ~0ull;
+        if (km) {
+            keep = all = __ballot(t0 + lane < k1 && km[t0 + lane]);
+            if constexpr (GROUPS > 1) {      // (the same answer in every wave: there is a barrier behind it)
+                const int t1 = k0 + (it * GROUPS + 1 - grp) * BT;
+                all &= __ballot(t1 + lane < k1 && km[t1 + lane]);
+            }
+        }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (it + 1 < nt) { SPAN_ISSUE(it + 1); SPAN_POS_LOAD(it + 1); }
-        if (keep != ~0ull) {
+        if (all != ~0ull) {
             T::clear_rows(Ks, keep, t, 256);
             __syncthreads();
         }
@@ -248,30 +259,43 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
                     g = mfma32<false>(T::rows(Vs, c, n, lane), gf[c], g);
                 }
                 const uint32_t wb = (uint32_t)(bits >> (32 * n));
+                int pos = ((it & 1) * GROUPS + grp) * STAGE + 2 * T::BYTES + (n * 32 + half * 4) * 4;
+                f32x4_t kq[AX ? AX : 1], kn[AX ? AX : 1];      // positions of four keys, and of the next four
+#pragma unroll
+                for (int a = 0; a < AX; ++a) kq[a] = lds_f4(smem + pos + a * BT * 4);
 #pragma unroll
                 for (int g4 = 0; g4 < 4; ++g4) {
-                    i32x4_t kq[AX ? AX : 1];
+                    float d4[4], far[AX ? AX : 1][4], slope[4];
+                    if (g4 < 3)
 #pragma unroll
-                    for (int a = 0; a < AX; ++a) kq[a] = lds_i4(pks + a * BT + n * 32 + g4 * 8 + half * 4);
+                        for (int a = 0; a < AX; ++a) kn[a] = lds_f4(smem + pos + a * BT * 4 + (g4 + 1) * 32);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = g4 * 4 + e;
-                        float x = s[r], slope = 1.f, far[AX ? AX : 1];
-                        if constexpr (CAP) { const float th = span_tanh(x, c1); slope = __builtin_fmaf(-th, th, 1.f); x = th * c2; }
-                        else x *= c1;
+                        float x;
+                        if constexpr (CAP) { const float th = span_tanh(s[r], c1); slope[e] = __builtin_fmaf(-th, th, 1.f); x = __builtin_fmaf(th, c2, -lse2); }
+                        else x = __builtin_fmaf(s[r], c1, -lse2);
 #pragma unroll
                         for (int a = 0; a < AX; ++a) {
-                            const int kv = kq[a][e];
-                            far[a] = fabsf((float)(pq[a] - kv));
-                            x = __builtin_fmaf(-sl[a], far[a], x);
+                            far[a][e] = pq[a] - kq[a][e];
+                            x = __builtin_fmaf(-sl[a], fabsf(far[a][e]), x);
                         }
-                        float d = __builtin_amdgcn_exp2f(x - lse2) * (g[r] - delta);
-                        if (!(wb & (1u << (8 * g4 + e)))) d = 0.f;
-#pragma unroll
-                        for (int a = 0; a < AX; ++a) ds_sl[a] = __builtin_fmaf(d, far[a], ds_sl[a]);
-                        s[r] = CAP ? d * slope : d;
+                        d4[e] = __builtin_amdgcn_exp2f(x) * (g[r] - delta);
                     }
-                    asm volatile("" ::: "memory");      // (four scores at a time: all sixteen at once cost 60 registers more, and the second workgroup of a CU)
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) d4[e] = __uint_as_float(__float_as_uint(d4[e]) & (uint32_t)((int)(wb << (31 - (8 * g4 + e))) >> 31));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                        for (int a = 0; a < AX; ++a) ds_sl[a] = __builtin_fmaf(d4[e], fabsf(far[a][e]), ds_sl[a]);
+                        s[g4 * 4 + e] = CAP ? d4[e] * slope[e] : d4[e];
+                    }
+                    // (four scores at a time: all sixteen at once cost 60 registers more)
+                    asm volatile("" : "+v"(pos), "+v"(s[g4 * 4]), "+v"(s[g4 * 4 + 1]), "+v"(s[g4 * 4 + 2]), "+v"(s[g4 * 4 + 3]) :: "memory");
+#pragma unroll
+                    for (int a = 0; a < AX; ++a) { asm volatile("" : "+v"(ds_sl[a])); kq[a] = kn[a]; }
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -286,14 +310,31 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
 #undef SPAN_ISSUE
 #undef SPAN_POS_LOAD
 #undef SPAN_POS_STORE
+    if constexpr (GROUPS > 1) {      // the second group's sums to the first
+        float* sum = reinterpret_cast<float*>(smem);
+        __syncthreads();
+        if (grp == 1) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum[(c * 16 + r) * 256 + t] = dq[c][r];
+        }
+        __syncthreads();
+        if (grp == 0) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dq[c][r] += sum[(c * 16 + r) * 256 + t];
+        }
+    }
     float bad = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
         for (int r = 0; r < 16; ++r) bad = __builtin_fmaf(dq[c][r], 0.f, bad);
     bad = both_halves_sum(bad);
-    const bool redo = ok && bad != 0.f && (lse2 + delta) * 0.f == 0.f;      // (a row whose own numbers are not finite is what it is)
-    if (ok && !redo) {
+    const bool here = ok && grp == 0, redo = here && bad != 0.f && (lse2 + delta) * 0.f == 0.f;      // (a row whose own numbers are not finite is what it is)
+    if (here && !redo) {
         uint16_t* op = p.dq + b * p.dq_s[0] + h * p.dq_s[1] + (long)i * p.dq_s[2] + half * 4;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
@@ -314,16 +355,27 @@ __global__ __launch_bounds__(256, 2) void span_bwd_dq(const SpanArgs p) {
         if (D > 64) op[lane + 64] = f32_to_bf16(ro[1] * p.scale);
     }
     if constexpr (AX > 0) {
-        if (p.dsl_part) {      // the workgroup's part of the slopes' gradients: lanes in a fixed tree, then the waves in order
+        if (p.dsl_part) {      // the workgroup's part of the slopes' gradients: lanes in a fixed tree, then the waves in order; the last workgroup adds the parts
             float* fr = reinterpret_cast<float*>(red);
             __syncthreads();
 #pragma unroll
             for (int a = 0; a < AX; ++a) {
                 const float v = wave_sum(ds_sl[a]);
-                if (lane == 0) fr[w * 4 + a] = -v;
+                if (lane == 0) fr[wave * 4 + a] = -v;
             }
             __syncthreads();
-            if (t < AX) p.dsl_part[((long)b * tiles + tile) * p.Hq * AX + h * AX + t] = ((fr[t] + fr[4 + t]) + fr[8 + t]) + fr[12 + t];
+            if (threadIdx.x < AX) {
+                float v = ((fr[t] + fr[4 + t]) + fr[8 + t]) + fr[12 + t];
+                if constexpr (GROUPS > 1) v += ((fr[16 + t] + fr[20 + t]) + fr[24 + t]) + fr[28 + t];
+                p.dsl_part[((long)b * tiles + tile) * p.Hq * AX + h * AX + t] = v;
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) red[0] = __hip_atomic_fetch_add(p.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1u == (unsigned)(p.B * p.Hq * tiles);
+            __syncthreads();
+            if (red[0]) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+                sum_slope_parts(p, GROUPS * 256, reinterpret_cast<float*>(smem));
+            }
         }
     }
 }
@@ -381,26 +433,25 @@ struct BwdForm {
 
 // 128 keys of a key head against the query tiles that see them: a wave holds 32 keys as operands (K, V) and their gradients as accumulators.
 // ROLES (128 wide heads): 8 waves, the first four take dV, the others dK of the same keys -- both gradients and both operands are 192 registers, which leaves one wave
-// per SIMD and every latency in the open (942 us for 2 x 16 heads of 4096 x 4096, the matrix pipe busy a quarter of the time); S is computed in both for it, 5 products
+// per SIMD and every latency in the open (942 us for dk and dv of 2 x 16 heads of 4096 x 4096, and 695 so); S is computed in both for it, 5 products
 // for 4.  Narrower heads take both gradients in one wave, two or three of which fit a SIMD.
+template <int D, int AX>
+struct DkvLds {
+    static constexpr int STAGE = 2 * Tile<D, BT>::BYTES + (4 + AX) * BT * 4, BYTES = 2 * STAGE + 256 * 4 + 512 * 16 + 16;
+};
 template <int D, int AX, bool CAP>
-__global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bwd_dkv(const SpanArgs p) {
+__device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigned char* smem) {
     typedef Tile<D, BT> T;
     constexpr bool ROLES = D == 128;
     constexpr int NW = ROLES ? 8 : 4, NT = NW * 64;
-    extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
-    constexpr int ROWB = (4 + AX) * BT * 4, STAGE = 2 * T::BYTES + ROWB;      // Q, dO, then per row: lse', delta, lo, hi, positions
+    constexpr int STAGE = DkvLds<D, AX>::STAGE;      // Q, dO, then per row: lse', delta, lo, hi, positions
     int* list = reinterpret_cast<int*>(smem + 2 * STAGE);                     // [256] query tiles
     int4* hull = reinterpret_cast<int4*>(list + 256);                         // [256][2] bounds of their two 32-row halves
     int* cnt = reinterpret_cast<int*>(hull + 512);                            // [4]
     const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), w = ROLES ? wave & 3 : wave;
     const int tiles = (p.nk + BK - 1) / BK, total = p.B * p.Hk * p.splits * tiles, per = (total + 7) / 8;
-    const int item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);      // (a contiguous part of (row, key head, split, tile) per XCD)
-    if ((int)(blockIdx.x >> 3) >= per) {
-        if (AX > 0 && p.dsl_part) sum_slope_parts(p, NT, reinterpret_cast<float*>(smem));      // (one workgroup more than there are tiles)
-        return;
-    }
+    const int item = (id & 7) * per + (id >> 3);      // (a contiguous part of (row, key head, split, tile) per XCD)
     if (item >= total) return;
     const int tile = item % tiles, part = (item / tiles) % p.splits, hk = (item / tiles / p.splits) % p.Hk, b = item / tiles / p.splits / p.Hk;
     const int heads = p.Hq / p.Hk / p.splits, h0 = (hk * p.splits + part) * heads, h1 = h0 + heads;      // the query heads of this workgroup
@@ -409,9 +460,9 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
     const bool live = key < p.nk && (!p.kmask || p.kmask[b * p.km_sb + key]);      // a key that is not there or masked: zeros, no weight
     const bool all_live = __all(live);
     const int mkey = live ? key : -1;      // (no span holds key -1)
-    int pk[AX ? AX : 1];
+    float pk[AX ? AX : 1];
 #pragma unroll
-    for (int a = 0; a < AX; ++a) pk[a] = key < p.nk ? p.pos_k[b * p.pk_sb + (long)key * AX + a] : 0;
+    for (int a = 0; a < AX; ++a) pk[a] = key < p.nk ? (float)p.pos_k[b * p.pk_sb + (long)key * AX + a] : 0.f;
     BwdForm<CAP, AX> F;
     F.init(p);
 
@@ -454,7 +505,7 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
             rw[lane] = lsev; rw[BT + lane] = delv;
             ri[2 * BT + lane] = spv.x; ri[3 * BT + lane] = spv.y;
 #pragma unroll
-            for (int a = 0; a < AX; ++a) ri[(4 + a) * BT + lane] = posv[a];
+            for (int a = 0; a < AX; ++a) rw[(4 + a) * BT + lane] = (float)posv[a];
         }
     };
     const auto pass = [&](auto take_v, auto take_k) {      // the whole walk over the query tiles, for the gradients that this wave takes
@@ -479,6 +530,7 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
                 if constexpr (DK) dk[c][r] = 0.f;
                 if constexpr (DV) dv[c][r] = 0.f;
             }
+        bool any = false;      // does any query see this tile
         for (int base = 0; base < qtiles; base += 256) {
             // ---- the query tiles of this stretch that see keys of this tile, in order
             __syncthreads();
@@ -501,6 +553,7 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
                 __syncthreads();
             }
             if (n_list == 0) continue;
+            any = true;
             f_at = 0; f_h = h0; f_st = 0;
             fetch();
             for (bool more = true; more;) {
@@ -546,22 +599,31 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
                     }
                     paced<DK ? 2 : 1, D / 16>();
                     int rows = st * STAGE + 2 * T::BYTES + (n * 32 + half * 4) * 4;
+                    f32x4_t l4, d4, k4[AX ? AX : 1], ln, dn, kn[AX ? AX : 1];      // numbers of four rows, and of the next four
+                    l4 = ln = lds_f4(smem + rows);
+                    d4 = dn = l4;
+                    if constexpr (DK) d4 = lds_f4(smem + rows + BT * 4);
+#pragma unroll
+                    for (int a = 0; a < AX; ++a) k4[a] = kn[a] = lds_f4(smem + rows + (4 + a) * BT * 4);
 #pragma unroll
                     for (int g4 = 0; g4 < 4; ++g4) {
-                        const f32x4_t l4 = lds_f4(smem + rows + g4 * 32);
+                        if (g4 < 3) {
+                            ln = lds_f4(smem + rows + (g4 + 1) * 32);
+                            if constexpr (DK) dn = lds_f4(smem + rows + BT * 4 + (g4 + 1) * 32);
+#pragma unroll
+                            for (int a = 0; a < AX; ++a) kn[a] = lds_f4(smem + rows + (4 + a) * BT * 4 + (g4 + 1) * 32);
+                        }
                         float y4[4], w4[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) y4[e] = F.y(s[g4 * 4 + e], w4[e]);
 #pragma unroll
                         for (int a = 0; a < AX; ++a) {
-                            const i32x4_t k4 = lds_i4(smem + rows + (4 + a) * BT * 4 + g4 * 32);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) y4[e] = __builtin_fmaf(-sl[a], fabsf((float)(k4[e] - pk[a])), y4[e]);
+                            for (int e = 0; e < 4; ++e) y4[e] = __builtin_fmaf(-sl[a], fabsf(k4[a][e] - pk[a]), y4[e]);
                         }
 #pragma unroll
                         for (int e = 0; e < 4; ++e) y4[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(y4[e], F.ka, -l4[e]));
                         if constexpr (DK) {
-                            const f32x4_t d4 = lds_f4(smem + rows + BT * 4 + g4 * 32);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 float d = y4[e] * (g[g4 * 4 + e] - d4[e]);
@@ -574,6 +636,9 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
                         } else if constexpr (AX > 0) asm volatile("" : "+v"(rows), "+v"(y4[0]), "+v"(y4[1]), "+v"(y4[2]), "+v"(y4[3]));
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[g4 * 4 + e] = y4[e];
+                        l4 = ln; d4 = dn;
+#pragma unroll
+                        for (int a = 0; a < AX; ++a) k4[a] = kn[a];
                     }
                     if (masked) {
                         const int* ri = reinterpret_cast<const int*>(Gs + T::BYTES) + 2 * BT + n * 32 + half * 4;
@@ -603,6 +668,10 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
         }
         // ---- out; a key whose gradient is not finite -- another key's infinity or NaN met its zero weight in the matrix instruction -- is computed again from its own rows
         const long prow = ((long)b * p.Hk + hk) * p.nk, pall = (long)p.B * p.Hk * p.nk;      // partial sums: [splits][dk, dv][rows][D]
+        if (p.splits > 1) {      // (a tile that nothing sees has no parts)
+            if (t == 0) p.seen[b * tiles + tile] = any;
+            if (!any) return;
+        }
         const auto put = [&](f32x16_t* acc, int which, float f) {
             float bad = 0.f;
 #pragma unroll
@@ -652,21 +721,35 @@ __global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bw
     else pass(No(), Yes());
 }
 
-// adds the head splits of a key row in split order; masked keys' parts are zeros.  4 elements a thread
+// dq and dk / dv read the same and need nothing of each other: one launch, the key tiles first, so that the end of one fills up with the other (a launch each: 6100 rows
+// with one document of 2462, 16 / 4 heads of 128, capped: 256 us, 206 so; 8150 rows of packed images, 8 heads of 64, two axes: 114 and 91; 2 x 16 heads of 4096 x 4096,
+// where both fill the card by themselves: 1.11 ms and 1.10)
+template <int D, int AX, bool CAP>
+__global__ __launch_bounds__(D == 128 ? 512 : 256, D == 32 ? 3 : 2) void span_bwd_main(const SpanArgs p) {
+    extern __shared__ __attribute__((aligned(128))) unsigned char smem[];
+    const int keys = (p.B * p.Hk * p.splits * ((p.nk + BK - 1) / BK) + 7) / 8 * 8;
+    if ((int)blockIdx.x < keys) dkv_tile<D, AX, CAP>(p, blockIdx.x, smem);
+    else dq_tile<D, AX, CAP, D == 128 ? 2 : 1>(p, blockIdx.x - keys, smem);
+}
+
+// adds the head splits of a key row in split order; masked keys' parts are zeros, tiles that nothing sees have none.  4 elements a thread
 template <int D>
 __global__ __launch_bounds__(256) void span_bwd_join(const SpanArgs p) {
     const long pall = (long)p.B * p.Hk * p.nk, x = (long)blockIdx.x * 256 + threadIdx.x;
     const long row = x / (D / 4);
     const int c = (int)(x % (D / 4)) * 4;
     if (row >= 2 * pall) return;
-    float4 v = *reinterpret_cast<const float4*>(p.part_o + row * D + c);
-    for (int s = 1; s < p.splits; ++s) {
-        const float4 y = *reinterpret_cast<const float4*>(p.part_o + (s * 2 * pall + row) * D + c);
-        v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
-    }
     const bool is_v = row >= pall;
     const long r = is_v ? row - pall : row;
     const int key = (int)(r % p.nk), hk = (int)(r / p.nk % p.Hk), b = (int)(r / p.nk / p.Hk);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.seen[b * ((p.nk + BK - 1) / BK) + key / BK]) {
+        v = *reinterpret_cast<const float4*>(p.part_o + row * D + c);
+        for (int s = 1; s < p.splits; ++s) {
+            const float4 y = *reinterpret_cast<const float4*>(p.part_o + (s * 2 * pall + row) * D + c);
+            v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+        }
+    }
     uint16_t* o = is_v ? p.dv + b * p.dv_s[0] + hk * p.dv_s[1] + (long)key * p.dv_s[2] : p.dk + b * p.dk_s[0] + hk * p.dk_s[1] + (long)key * p.dk_s[2];
     *reinterpret_cast<uint2*>(o + c) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
 }
@@ -689,19 +772,14 @@ int launch_bwd(hipStream_t s, const SpanArgs& a) {
         const long blocks = (a.order_out ? 1 : 0) + ((long)a.B * a.hull_tiles + 7) / 8 + (rows + rpb - 1) / rpb;
         hipLaunchKernelGGL(span_bwd_pre<D>, dim3((unsigned)blocks), dim3(256), 0, s, a);
         if ((rc = mm_check_launch("span_bwd_pre"))) return rc;
-        constexpr int sm = 2 * (2 * Tile<D, BT>::BYTES + AX * BT * 4) + 64;
-        static std::atomic<unsigned long long> lds{0};
-        if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dq<D, AX, CAP>), sm, lds))) return rc;
-        hipLaunchKernelGGL((span_bwd_dq<D, AX, CAP>), dim3((unsigned)(a.B * a.Hq * ((a.nq + BQ - 1) / BQ))), dim3(256), sm, s, a);
-        if ((rc = mm_check_launch("span_bwd_dq"))) return rc;
     }
-    if (a.nk > 0 || a.dsl_part) {      // (without keys: the slopes' gradients alone)
-        constexpr int sm = 2 * (2 * Tile<D, BT>::BYTES + (4 + AX) * BT * 4) + 256 * 4 + 512 * 16 + 16;
+    if (a.nk > 0 || a.nq > 0) {
+        constexpr int dq = DqLds<D, AX, D == 128 ? 2 : 1>::BYTES, dkv = DkvLds<D, AX>::BYTES, sm = dq > dkv ? dq : dkv;
         static std::atomic<unsigned long long> lds{0};
-        if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_dkv<D, AX, CAP>), sm, lds))) return rc;
-        const long total = (long)a.B * a.Hk * a.splits * ((a.nk + BK - 1) / BK);
-        hipLaunchKernelGGL((span_bwd_dkv<D, AX, CAP>), dim3((unsigned)((total + 7) / 8 * 8 + (a.dsl_part ? 1 : 0))), dim3(D == 128 ? 512 : 256), sm, s, a);
-        if ((rc = mm_check_launch("span_bwd_dkv"))) return rc;
+        if ((rc = span_allow_lds(reinterpret_cast<const void*>(span_bwd_main<D, AX, CAP>), sm, lds))) return rc;
+        const long keys = ((long)a.B * a.Hk * a.splits * ((a.nk + BK - 1) / BK) + 7) / 8 * 8, rows = (long)a.B * a.Hq * ((a.nq + BQ - 1) / BQ);
+        hipLaunchKernelGGL((span_bwd_main<D, AX, CAP>), dim3((unsigned)(keys + rows)), dim3(D == 128 ? 512 : 256), sm, s, a);
+        if ((rc = mm_check_launch("span_bwd_main"))) return rc;
         if (a.splits > 1 && a.nk > 0) {
             const long work = 2L * a.B * a.Hk * a.nk * (D / 4);
             hipLaunchKernelGGL(span_bwd_join<D>, dim3((unsigned)((work + 255) / 256)), dim3(256), 0, s, a);
@@ -723,7 +801,7 @@ int launch_bwd_axes(hipStream_t s, const SpanArgs& a) {
 template <int D>
 int launch_bwd_dim(hipStream_t s, const SpanArgs& a) { return a.cap > 0.f ? launch_bwd_axes<D, true>(s, a) : launch_bwd_axes<D, false>(s, a); }
 
-struct BwdLayout { size_t hulls, delta, order, slopes, parts, bytes; int hull_tiles, splits; long slope_parts; };
+struct BwdLayout { size_t hulls, delta, done, seen, order, slopes, parts, bytes; int hull_tiles, splits; long slope_parts; };
 BwdLayout bwd_layout(const mm_span_attn* a) {
     BwdLayout r;
     r.hull_tiles = (a->nq + 31) / 32;
@@ -731,10 +809,12 @@ BwdLayout bwd_layout(const mm_span_attn* a) {
     size_t at = 0;
     r.hulls = at; at += (size_t)a->batch * r.hull_tiles * sizeof(int4);
     r.delta = at; at += ((size_t)a->batch * a->heads_q * a->nq * sizeof(float) + 15) / 16 * 16;
+    r.done = at; at += 16;
+    r.splits = head_splits(a);
+    r.seen = at; at += r.splits > 1 ? (size_t)a->batch * ((a->nk + BK - 1) / BK) * sizeof(int) : 0;
     r.order = at; at += span_order_count(a) * sizeof(int32_t);
     r.slopes = at; at += (size_t)r.slope_parts * a->heads_q * a->axes * sizeof(float);
     at = (at + 15) / 16 * 16;
-    r.splits = head_splits(a);
     r.parts = at; at += r.splits > 1 ? (size_t)r.splits * 2 * a->batch * a->heads_k * a->nk * a->dim * sizeof(float) : 0;
     r.bytes = at;
     return r;
@@ -755,6 +835,8 @@ int k_span_attn_bwd(hipStream_t s, const mm_span_attn* a, void* ws) {
     if (span_order_count(a)) p.order = p.order_out = reinterpret_cast<int32_t*>((char*)ws + l.order);
     p.part_o = reinterpret_cast<float*>((char*)ws + l.parts);
     p.dsl_part = l.slope_parts ? reinterpret_cast<float*>((char*)ws + l.slopes) : nullptr;
+    p.done = l.slope_parts ? reinterpret_cast<unsigned*>((char*)ws + l.done) : nullptr;
+    p.seen = reinterpret_cast<int*>((char*)ws + l.seen);
     p.dslopes = a->dslopes;
     if (a->slopes && a->dslopes && !l.slope_parts)      // (no rows: zeros)
         if (const int rc = k_colsum(s, a->dslopes, 0, (long)a->heads_q * a->axes, a->dslopes)) return rc;

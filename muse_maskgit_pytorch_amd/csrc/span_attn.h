@@ -22,7 +22,7 @@ struct SpanArgs {
     // backward
     const uint16_t* dout; long do_s[3];
     uint16_t *dq, *dk, *dv; long dq_s[3], dk_s[3], dv_s[3];
-    float* delta; float* dsl_part; float* dslopes; int4* hulls; int hull_tiles; int32_t* order_out;
+    float* delta; float* dsl_part; float* dslopes; unsigned* done; int* seen; int4* hulls; int hull_tiles; int32_t* order_out;
 };
 
 namespace {
@@ -112,8 +112,7 @@ struct Tile {
 
 // Which (tile, head) a workgroup takes.  Workgroups go to the 8 XCDs in turn: with a multiple of 8 heads each XCD keeps its own heads (their keys are read into one
 // L2), neighbours among them; otherwise heads in turn.  Tiles in the order of `order`, heads innermost, so the long ones of every head start first.
-__device__ __forceinline__ bool span_item(const int32_t* order, int heads, int rows, int& row_tile, int& head) {      // rows: tiles over the batch
-    const unsigned id = blockIdx.x;
+__device__ __forceinline__ bool span_item(unsigned id, const int32_t* order, int heads, int rows, int& row_tile, int& head) {      // rows: tiles over the batch
     int rank;
     if (heads % 8 == 0) {
         const unsigned own = heads / 8, slot = id >> 3;
@@ -134,14 +133,6 @@ __device__ __forceinline__ unsigned long long bit_range(int a, int e) {
 // rounding of cap.  c1 = scale * log2 e without a cap, 2 * scale * log2 e / cap with one; c2 = cap * log2 e.
 __device__ __forceinline__ float span_tanh(float x, float c1) {
     return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f), 1.f);
-}
-
-template <int AX>
-__device__ __forceinline__ float span_bias(const int (&pq)[AX ? AX : 1], const float (&sl)[AX ? AX : 1], const int* pk) {      // sum of slope (in log2 units) * distance
-    float v = 0.f;
-#pragma unroll
-    for (int a = 0; a < AX; ++a) v = __builtin_fmaf(sl[a], fabsf((float)(pq[a] - pk[a])), v);
-    return v;
 }
 
 // dot product of two rows by one lane
@@ -197,7 +188,7 @@ __device__ __forceinline__ float pair_score(const SpanArgs& p, const uint16_t* q
     } else x *= p.scale * SPAN_LOG2E;
 #pragma unroll
     for (int a = 0; a < AX; ++a)
-        x -= p.slopes[h * AX + a] * SPAN_LOG2E * fabsf((float)(p.pos_q[b * p.pq_sb + (long)i * AX + a] - p.pos_k[b * p.pk_sb + (long)key * AX + a]));
+        x -= p.slopes[h * AX + a] * SPAN_LOG2E * fabsf((float)p.pos_q[b * p.pq_sb + (long)i * AX + a] - (float)p.pos_k[b * p.pk_sb + (long)key * AX + a]);
     return x;
 }
 
