@@ -258,7 +258,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
         if (AHEAD && it + 2 < nt) fill_k(it + 2);
         if (keep != ~0ull) {
             T::clear_rows(Vs, keep, t, 256);
-            __syncthreads();
+            lds_barrier();
         }
         const bool now = sees(it);
         if constexpr (AHEAD) {

@@ -243,7 +243,7 @@ __device__ __forceinline__ void dq_tile(const SpanArgs& p, unsigned id, unsigned
         if (it + 1 < nt) { SPAN_ISSUE(it + 1); SPAN_POS_LOAD(it + 1); }
         if (all != ~0ull) {
             T::clear_rows(Ks, keep, t, 256);
-            __syncthreads();
+            lds_barrier();
         }
         if (__any(lo < t0 + BT && hi > t0)) {
             const bool masked = keep != ~0ull || !__all(lo <= t0 && hi >= t0 + BT);
@@ -437,15 +437,17 @@ struct BwdForm {
 // for 4.  Narrower heads take both gradients in one wave, two or three of which fit a SIMD.
 template <int D, int AX>
 struct DkvLds {
-    static constexpr int STAGE = 2 * Tile<D, BT>::BYTES + (4 + AX) * BT * 4, BYTES = 2 * STAGE + 256 * 4 + 512 * 16 + 16;
+    // [2] Q and per row: lse', delta, lo, hi, positions; [GS] dO; with roles [2] P of the four waves as operands; the list
+    static constexpr int T = Tile<D, BT>::BYTES, Q = T + (4 + AX) * BT * 4, GS = D == 128 ? 3 : 2, G = 2 * Q, P = G + GS * T, LIST = P + (D == 128 ? 2 * 4 * 4096 : 0);
+    static constexpr int BYTES = LIST + 256 * 4 + 512 * 16 + 16;
 };
 template <int D, int AX, bool CAP>
 __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigned char* smem) {
     typedef Tile<D, BT> T;
     constexpr bool ROLES = D == 128;
     constexpr int NW = ROLES ? 8 : 4, NT = NW * 64;
-    constexpr int STAGE = DkvLds<D, AX>::STAGE;      // Q, dO, then per row: lse', delta, lo, hi, positions
-    int* list = reinterpret_cast<int*>(smem + 2 * STAGE);                     // [256] query tiles
+    typedef DkvLds<D, AX> M;
+    int* list = reinterpret_cast<int*>(smem + M::LIST);                       // [256] query tiles
     int4* hull = reinterpret_cast<int4*>(list + 256);                         // [256][2] bounds of their two 32-row halves
     int* cnt = reinterpret_cast<int*>(hull + 512);                            // [4]
     const int t = threadIdx.x, lane = t & 63, half = lane >> 5;
@@ -467,12 +469,12 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
     F.init(p);
 
     const int qtiles = (p.nq + BT - 1) / BT;
-    // the tile being fetched: entry f_at of the list, head f_h, stage f_st; its rows' numbers (lane = row of the 64, every wave the same; wave 0 writes them to LDS)
+    // the tile being fetched: entry f_at of the list, head f_h, stages f_st and f_g (dO); its rows' numbers (lane = row of the 64, every wave the same; wave 0 writes them to LDS)
     float lsev = 0.f, delv = 0.f;
     int2 spv = make_int2(0, 0);
     int posv[AX ? AX : 1];
     float f_sl[AX ? AX : 1];
-    int n_list = 0, f_at = 0, f_h = h0, f_st = 0, f_rows = 0;
+    int n_list = 0, f_at = 0, f_h = h0, f_st = 0, f_g = 0, f_rows = 0;
     const auto fetch = [&]() {      // (nothing here waits: the rows' numbers are looked at in settle(), a tile later)
         const int q0 = __builtin_amdgcn_readfirstlane(list[f_at]) * BT, i = min(q0 + lane, p.nq - 1);
         const long row = ((long)b * p.Hq + f_h) * p.nq + i;
@@ -483,10 +485,9 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
 #pragma unroll
         for (int a = 0; a < AX; ++a) { posv[a] = p.pos_q[b * p.pq_sb + (long)i * AX + a]; f_sl[a] = p.slopes[f_h * AX + a]; }
         f_rows = p.nq - q0;
-        unsigned char* st = smem + f_st * STAGE;
         const int ok = min(BT, f_rows);
-        T::template fill<NW>(st, p.q + b * p.q_s[0] + f_h * p.q_s[1] + (long)q0 * p.q_s[2], ok, (int)p.q_s[2], wave, lane);
-        T::template fill<NW>(st + T::BYTES, p.dout + b * p.do_s[0] + f_h * p.do_s[1] + (long)q0 * p.do_s[2], ok, (int)p.do_s[2], wave, lane);
+        T::template fill<NW>(smem + f_st * M::Q, p.q + b * p.q_s[0] + f_h * p.q_s[1] + (long)q0 * p.q_s[2], ok, (int)p.q_s[2], wave, lane);
+        T::template fill<NW>(smem + M::G + f_g * M::T, p.dout + b * p.do_s[0] + f_h * p.do_s[1] + (long)q0 * p.do_s[2], ok, (int)p.do_s[2], wave, lane);
     };
     // rows that are not there, see nothing or whose lse says so: an empty span; which of the 64 see a key of this tile
     const auto settle = [&]() {
@@ -500,7 +501,7 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
     };
     const auto store_rows = [&]() {
         if (wave == 0) {
-            float* rw = reinterpret_cast<float*>(smem + f_st * STAGE + 2 * T::BYTES);
+            float* rw = reinterpret_cast<float*>(smem + f_st * M::Q + M::T);
             int* ri = reinterpret_cast<int*>(rw);
             rw[lane] = lsev; rw[BT + lane] = delv;
             ri[2 * BT + lane] = spv.x; ri[3 * BT + lane] = spv.y;
@@ -510,16 +511,17 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
     };
     const auto pass = [&](auto take_v, auto take_k) {      // the whole walk over the query tiles, for the gradients that this wave takes
         constexpr bool DV = decltype(take_v)::value, DK = decltype(take_k)::value;
-        u32x4_t kf[D / 16], vf[DK ? D / 16 : 1];
-        {
+        u32x4_t kf[DK ? D / 16 : 1], vf[DK ? D / 16 : 1];
+        if constexpr (DK) {
             const uint16_t* kp = p.k + b * p.k_s[0] + hk * p.k_s[1] + (long)(live ? key : 0) * p.k_s[2] + half * 8;
             const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1] + (long)(live ? key : 0) * p.v_s[2] + half * 8;
             const u32x4_t z = {0, 0, 0, 0};
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
                 const u32x4_t x = *reinterpret_cast<const u32x4_t*>(kp + c * 16);
+                const u32x4_t y = *reinterpret_cast<const u32x4_t*>(vp + c * 16);
                 kf[c] = live ? x : z;
-                if constexpr (DK) { const u32x4_t y = *reinterpret_cast<const u32x4_t*>(vp + c * 16); vf[c] = live ? y : z; }
+                vf[c] = live ? y : z;
             }
         }
         f32x16_t dk[DK ? D / 32 : 1], dv[DV ? D / 32 : 1];
@@ -554,10 +556,29 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
             }
             if (n_list == 0) continue;
             any = true;
-            f_at = 0; f_h = h0; f_st = 0;
+            f_at = 0; f_h = h0; f_st = 0; f_g = 0;
             fetch();
+            int p_at = -1, p_st = 0, p_g = 0;      // with roles: the tile whose P is in LDS
+            const auto take_dv = [&]() {
+                if constexpr (DV && !DK) {
+                    if (p_at < 0) return;
+                    const unsigned char* Gs = smem + M::G + p_g * M::T;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const i32x4_t hl = lds_i4(hull + 2 * p_at + n);
+                        if (__builtin_amdgcn_readfirstlane((int)(hl[0] < min(w0 + 32, t1) && hl[1] > w0)) == 0) continue;
+                        const unsigned char* ps = smem + M::P + ((p_st * 4 + w) * 2 + n) * 2048 + lane * 16;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const u32x4_t pf = *reinterpret_cast<const u32x4_t*>(ps + x * 1024);
+#pragma unroll
+                            for (int c = 0; c < D / 32; ++c) dv[c] = mfma32<false>(T::cols(Gs, 2 * n + x, c, lane), pf, dv[c]);
+                        }
+                    }
+                }
+            };
             for (bool more = true; more;) {
-                const int at = f_at, st = f_st;
+                const int at = f_at, st = f_st, gs = f_g;
                 float sl[AX ? AX : 1];
 #pragma unroll
                 for (int a = 0; a < AX; ++a) sl[a] = f_sl[a] * F.per;
@@ -567,15 +588,19 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
                 __syncthreads();      // the tile and its rows' numbers are there for every wave; every wave is done with the other stage
                 if (++f_at == n_list) { f_at = 0; ++f_h; }
                 f_st ^= 1;
+                f_g = f_g + 1 == M::GS ? 0 : f_g + 1;
                 more = f_h < h1;
                 if (more) fetch();
-                const unsigned char* Qs = smem + st * STAGE;
-                const unsigned char* Gs = Qs + T::BYTES;
+                const unsigned char* Qs = smem + st * M::Q;
+                const unsigned char* Gs = smem + M::G + gs * M::T;
                 if (keep != ~0ull) {      // rows that see no key of this tile take no part, whatever they hold (rows behind the last document)
-                    T::clear_rows(smem + st * STAGE, keep, t, NT);
-                    T::clear_rows(smem + st * STAGE + T::BYTES, keep, t, NT);
-                    __syncthreads();
+                    T::clear_rows(smem + st * M::Q, keep, t, NT);
+                    T::clear_rows(smem + M::G + gs * M::T, keep, t, NT);
+                    lds_barrier();
                 }
+                take_dv();
+                p_at = at; p_st = st; p_g = gs;
+                if constexpr (DK)
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const i32x4_t hl = lds_i4(hull + 2 * at + n);
@@ -584,32 +609,30 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
                     f32x16_t s, g;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
-                    u32x4_t q0 = T::rows(Qs, 0, n, lane), q1 = T::rows(Qs, 1, n, lane), g0 = q0, g1 = q1;
-                    if constexpr (DK) { g0 = T::rows(Gs, 0, n, lane); g1 = T::rows(Gs, 1, n, lane); }
+                    u32x4_t q0 = T::rows(Qs, 0, n, lane), q1 = T::rows(Qs, 1, n, lane), g0 = T::rows(Gs, 0, n, lane), g1 = T::rows(Gs, 1, n, lane);
 #pragma unroll
                     for (int c = 0; c < D / 16; ++c) {
                         const u32x4_t x = q0, y = g0;
                         q0 = q1; g0 = g1;
                         if (c + 2 < D / 16) {
                             q1 = T::rows(Qs, c + 2, n, lane);
-                            if constexpr (DK) g1 = T::rows(Gs, c + 2, n, lane);
+                            g1 = T::rows(Gs, c + 2, n, lane);
                         }
                         s = mfma32<false>(x, kf[c], s);
-                        if constexpr (DK) g = mfma32<false>(y, vf[c], g);
+                        g = mfma32<false>(y, vf[c], g);
                     }
-                    paced<DK ? 2 : 1, D / 16>();
-                    int rows = st * STAGE + 2 * T::BYTES + (n * 32 + half * 4) * 4;
+                    paced<2, D / 16>();
+                    int rows = st * M::Q + M::T + (n * 32 + half * 4) * 4;
                     f32x4_t l4, d4, k4[AX ? AX : 1], ln, dn, kn[AX ? AX : 1];      // numbers of four rows, and of the next four
                     l4 = ln = lds_f4(smem + rows);
-                    d4 = dn = l4;
-                    if constexpr (DK) d4 = lds_f4(smem + rows + BT * 4);
+                    d4 = dn = lds_f4(smem + rows + BT * 4);
 #pragma unroll
                     for (int a = 0; a < AX; ++a) k4[a] = kn[a] = lds_f4(smem + rows + (4 + a) * BT * 4);
 #pragma unroll
                     for (int g4 = 0; g4 < 4; ++g4) {
                         if (g4 < 3) {
                             ln = lds_f4(smem + rows + (g4 + 1) * 32);
-                            if constexpr (DK) dn = lds_f4(smem + rows + BT * 4 + (g4 + 1) * 32);
+                            dn = lds_f4(smem + rows + BT * 4 + (g4 + 1) * 32);
 #pragma unroll
                             for (int a = 0; a < AX; ++a) kn[a] = lds_f4(smem + rows + (4 + a) * BT * 4 + (g4 + 1) * 32);
                         }
@@ -623,17 +646,15 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
                         }
 #pragma unroll
                         for (int e = 0; e < 4; ++e) y4[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(y4[e], F.ka, -l4[e]));
-                        if constexpr (DK) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                float d = y4[e] * (g[g4 * 4 + e] - d4[e]);
-                                if constexpr (CAP) d *= w4[e];
-                                w4[e] = d;
-                            }
-                            if constexpr (AX > 0) asm volatile("" : "+v"(rows), "+v"(w4[0]), "+v"(w4[1]), "+v"(w4[2]), "+v"(w4[3]));      // (done with these four before the next are fetched)
+                        for (int e = 0; e < 4; ++e) {
+                            float d = y4[e] * (g[g4 * 4 + e] - d4[e]);
+                            if constexpr (CAP) d *= w4[e];
+                            w4[e] = d;
+                        }
+                        if constexpr (AX > 0) asm volatile("" : "+v"(rows), "+v"(w4[0]), "+v"(w4[1]), "+v"(w4[2]), "+v"(w4[3]));      // (done with these four before the next are fetched)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) g[g4 * 4 + e] = w4[e];
-                        } else if constexpr (AX > 0) asm volatile("" : "+v"(rows), "+v"(y4[0]), "+v"(y4[1]), "+v"(y4[2]), "+v"(y4[3]));
+                        for (int e = 0; e < 4; ++e) g[g4 * 4 + e] = w4[e];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[g4 * 4 + e] = y4[e];
                         l4 = ln; d4 = dn;
@@ -641,7 +662,7 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
                         for (int a = 0; a < AX; ++a) k4[a] = kn[a];
                     }
                     if (masked) {
-                        const int* ri = reinterpret_cast<const int*>(Gs + T::BYTES) + 2 * BT + n * 32 + half * 4;
+                        const int* ri = reinterpret_cast<const int*>(Qs + M::T) + 2 * BT + n * 32 + half * 4;
 #pragma unroll
                         for (int g4 = 0; g4 < 4; ++g4) {
                             const i32x4_t lo = lds_i4(ri + g4 * 8), hi = lds_i4(ri + BT + g4 * 8);
@@ -649,21 +670,26 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
                             for (int e = 0; e < 4; ++e) {      // all ones: the row sees this key (spans are 0 <= lo <= hi)
                                 const uint32_t z = (uint32_t)-(int)((uint32_t)(mkey - lo[e]) < (uint32_t)(hi[e] - lo[e]));
                                 s[g4 * 4 + e] = __uint_as_float(__float_as_uint(s[g4 * 4 + e]) & z);
-                                if constexpr (DK) g[g4 * 4 + e] = __uint_as_float(__float_as_uint(g[g4 * 4 + e]) & z);
+                                g[g4 * 4 + e] = __uint_as_float(__float_as_uint(g[g4 * 4 + e]) & z);
                             }
                         }
                     }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const u32x4_t pf = pack_slots<false>(s, x), df = pack_slots<false>(g, x);      // P and dS rounded to bf16: operands
+                        if constexpr (!DV) *reinterpret_cast<u32x4_t*>(smem + M::P + ((st * 4 + w) * 2 + n) * 2048 + x * 1024 + lane * 16) = pf;
 #pragma unroll
                         for (int c = 0; c < D / 32; ++c) {
                             if constexpr (DV) dv[c] = mfma32<false>(T::cols(Gs, 2 * n + x, c, lane), pf, dv[c]);
-                            if constexpr (DK) dk[c] = mfma32<false>(T::cols(Qs, 2 * n + x, c, lane), df, dk[c]);
+                            dk[c] = mfma32<false>(T::cols(Qs, 2 * n + x, c, lane), df, dk[c]);
                         }
                     }
-                    paced_cols<(DV ? D / 16 : 0) + (DK ? D / 16 : 0)>();
+                    paced_cols<(DV ? D / 16 : 0) + D / 16>();
                 }
+            }
+            if constexpr (ROLES) {
+                __syncthreads();
+                take_dv();
             }
         }
         // ---- out; a key whose gradient is not finite -- another key's infinity or NaN met its zero weight in the matrix instruction -- is computed again from its own rows

@@ -123,6 +123,13 @@ __device__ __forceinline__ bool span_item(unsigned id, const int32_t* order, int
     return true;
 }
 
+// a barrier for what was written to LDS alone (__syncthreads waits for the next tile's DMA too)
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // bits a .. e - 1 of 64, both clamped
 __device__ __forceinline__ unsigned long long bit_range(int a, int e) {
     a = max(a, 0); e = min(e, 64);
