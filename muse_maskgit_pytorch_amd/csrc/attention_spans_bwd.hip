@@ -437,8 +437,8 @@ struct BwdForm {
 // for 4.  Narrower heads take both gradients in one wave, two or three of which fit a SIMD.
 template <int D, int AX>
 struct DkvLds {
-    // [2] Q and per row: lse', delta, lo, hi, positions; [GS] dO; with roles [2] P of the four waves as operands; the list
-    static constexpr int T = Tile<D, BT>::BYTES, Q = T + (4 + AX) * BT * 4, GS = D == 128 ? 3 : 2, G = 2 * Q, P = G + GS * T, LIST = P + (D == 128 ? 2 * 4 * 4096 : 0);
+    // [ST] Q, [ST] dO, [2] per row: lse', delta, lo, hi, positions; with pairs [2] the operand that each of the eight waves has for its partner; the list
+    static constexpr int T = Tile<D, BT>::BYTES, ST = D == 128 ? 3 : 2, G = ST * T, R = 2 * ST * T, ROWB = (4 + AX) * BT * 4, X = R + 2 * ROWB, LIST = X + (D == 128 ? 2 * 8 * 2048 : 0);
     static constexpr int BYTES = LIST + 256 * 4 + 512 * 16 + 16;
 };
 template <int D, int AX, bool CAP>
@@ -469,7 +469,7 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
     F.init(p);
 
     const int qtiles = (p.nq + BT - 1) / BT;
-    // the tile being fetched: entry f_at of the list, head f_h, stages f_st and f_g (dO); its rows' numbers (lane = row of the 64, every wave the same; wave 0 writes them to LDS)
+    // the tile being fetched: entry f_at of the list, head f_h, stages f_g (Q, dO) and f_st (its rows' numbers); its rows' numbers (lane = row of the 64, every wave the same; wave 0 writes them to LDS)
     float lsev = 0.f, delv = 0.f;
     int2 spv = make_int2(0, 0);
     int posv[AX ? AX : 1];
@@ -486,7 +486,7 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
         for (int a = 0; a < AX; ++a) { posv[a] = p.pos_q[b * p.pq_sb + (long)i * AX + a]; f_sl[a] = p.slopes[f_h * AX + a]; }
         f_rows = p.nq - q0;
         const int ok = min(BT, f_rows);
-        T::template fill<NW>(smem + f_st * M::Q, p.q + b * p.q_s[0] + f_h * p.q_s[1] + (long)q0 * p.q_s[2], ok, (int)p.q_s[2], wave, lane);
+        T::template fill<NW>(smem + f_g * M::T, p.q + b * p.q_s[0] + f_h * p.q_s[1] + (long)q0 * p.q_s[2], ok, (int)p.q_s[2], wave, lane);
         T::template fill<NW>(smem + M::G + f_g * M::T, p.dout + b * p.do_s[0] + f_h * p.do_s[1] + (long)q0 * p.do_s[2], ok, (int)p.do_s[2], wave, lane);
     };
     // rows that are not there, see nothing or whose lse says so: an empty span; which of the 64 see a key of this tile
@@ -501,7 +501,7 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
     };
     const auto store_rows = [&]() {
         if (wave == 0) {
-            float* rw = reinterpret_cast<float*>(smem + f_st * M::Q + M::T);
+            float* rw = reinterpret_cast<float*>(smem + M::R + f_st * M::ROWB);
             int* ri = reinterpret_cast<int*>(rw);
             rw[lane] = lsev; rw[BT + lane] = delv;
             ri[2 * BT + lane] = spv.x; ri[3 * BT + lane] = spv.y;
@@ -511,8 +511,8 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
     };
     const auto pass = [&](auto take_v, auto take_k) {      // the whole walk over the query tiles, for the gradients that this wave takes
         constexpr bool DV = decltype(take_v)::value, DK = decltype(take_k)::value;
-        u32x4_t kf[DK ? D / 16 : 1], vf[DK ? D / 16 : 1];
-        if constexpr (DK) {
+        u32x4_t kf[D / 16], vf[D / 16], own[2];      // own: the operand that this wave made of the tile before, for its own product
+        {
             const uint16_t* kp = p.k + b * p.k_s[0] + hk * p.k_s[1] + (long)(live ? key : 0) * p.k_s[2] + half * 8;
             const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1] + (long)(live ? key : 0) * p.v_s[2] + half * 8;
             const u32x4_t z = {0, 0, 0, 0};
@@ -533,6 +533,10 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
                 if constexpr (DV) dv[c][r] = 0.f;
             }
         bool any = false;      // does any query see this tile
+        const auto meets = [&](int at, int n) {      // do rows 32 n .. + 31 of a listed tile see one of the wave's keys
+            const i32x4_t hl = lds_i4(hull + 2 * at + n);
+            return __builtin_amdgcn_readfirstlane((int)(hl[0] < min(w0 + 32, t1) && hl[1] > w0)) != 0;
+        };
         for (int base = 0; base < qtiles; base += 256) {
             // ---- the query tiles of this stretch that see keys of this tile, in order
             __syncthreads();
@@ -558,22 +562,25 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
             any = true;
             f_at = 0; f_h = h0; f_st = 0; f_g = 0;
             fetch();
-            int p_at = -1, p_st = 0, p_g = 0;      // with roles: the tile whose P is in LDS
-            const auto take_dv = [&]() {
-                if constexpr (DV && !DK) {
+            int p_at = -1, p_st = 0, p_g = 0;      // pairs: the tile whose operands are made
+            const auto product = [&]() {
+                if constexpr (ROLES) {
                     if (p_at < 0) return;
-                    const unsigned char* Gs = smem + M::G + p_g * M::T;
+                    const unsigned char* As = smem + p_g * M::T + (DV ? M::G : 0);
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        const i32x4_t hl = lds_i4(hull + 2 * p_at + n);
-                        if (__builtin_amdgcn_readfirstlane((int)(hl[0] < min(w0 + 32, t1) && hl[1] > w0)) == 0) continue;
-                        const unsigned char* ps = smem + M::P + ((p_st * 4 + w) * 2 + n) * 2048 + lane * 16;
+                        if (!meets(p_at, n)) continue;
+                        const unsigned char* xs = smem + M::X + ((p_st * 4 + w) * 2 + n) * 2048 + lane * 16;
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const u32x4_t pf = *reinterpret_cast<const u32x4_t*>(ps + x * 1024);
+                            const u32x4_t f = n == (DV ? 0 : 1) ? own[x] : *reinterpret_cast<const u32x4_t*>(xs + x * 1024);
 #pragma unroll
-                            for (int c = 0; c < D / 32; ++c) dv[c] = mfma32<false>(T::cols(Gs, 2 * n + x, c, lane), pf, dv[c]);
+                            for (int c = 0; c < D / 32; ++c) {
+                                if constexpr (DV) dv[c] = mfma32<false>(T::cols(As, 2 * n + x, c, lane), f, dv[c]);
+                                else dk[c] = mfma32<false>(T::cols(As, 2 * n + x, c, lane), f, dk[c]);
+                            }
                         }
+                        paced_cols<D / 16>();
                     }
                 }
             };
@@ -588,23 +595,22 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
                 __syncthreads();      // the tile and its rows' numbers are there for every wave; every wave is done with the other stage
                 if (++f_at == n_list) { f_at = 0; ++f_h; }
                 f_st ^= 1;
-                f_g = f_g + 1 == M::GS ? 0 : f_g + 1;
+                f_g = f_g + 1 == M::ST ? 0 : f_g + 1;
                 more = f_h < h1;
                 if (more) fetch();
-                const unsigned char* Qs = smem + st * M::Q;
+                const unsigned char* Qs = smem + gs * M::T;
                 const unsigned char* Gs = smem + M::G + gs * M::T;
                 if (keep != ~0ull) {      // rows that see no key of this tile take no part, whatever they hold (rows behind the last document)
-                    T::clear_rows(smem + st * M::Q, keep, t, NT);
+                    T::clear_rows(smem + gs * M::T, keep, t, NT);
                     T::clear_rows(smem + M::G + gs * M::T, keep, t, NT);
                     lds_barrier();
                 }
-                take_dv();
-                p_at = at; p_st = st; p_g = gs;
-                if constexpr (DK)
+                if constexpr (DV) product();      // (dV's wave first, dK's behind its scores: one has the matrix pipe while the other has the vector pipe)
+                u32x4_t made[2];
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
+                for (int n = ROLES ? (DV ? 0 : 1) : 0; n < (ROLES ? (DV ? 1 : 2) : 2); ++n) {
+                    if (!meets(at, n)) continue;
                     const i32x4_t hl = lds_i4(hull + 2 * at + n);
-                    if (__builtin_amdgcn_readfirstlane((int)(hl[0] < min(w0 + 32, t1) && hl[1] > w0)) == 0) continue;
                     const bool masked = !all_live || __builtin_amdgcn_readfirstlane((int)!(hl[2] <= w0 && hl[3] >= w0 + 32)) != 0 || (uint32_t)(keep >> (32 * n)) != 0xFFFFFFFFu;
                     f32x16_t s, g;
 #pragma unroll
@@ -622,7 +628,7 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
                         g = mfma32<false>(y, vf[c], g);
                     }
                     paced<2, D / 16>();
-                    int rows = st * M::Q + M::T + (n * 32 + half * 4) * 4;
+                    int rows = M::R + st * M::ROWB + (n * 32 + half * 4) * 4;
                     f32x4_t l4, d4, k4[AX ? AX : 1], ln, dn, kn[AX ? AX : 1];      // numbers of four rows, and of the next four
                     l4 = ln = lds_f4(smem + rows);
                     d4 = dn = lds_f4(smem + rows + BT * 4);
@@ -662,7 +668,7 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
                         for (int a = 0; a < AX; ++a) k4[a] = kn[a];
                     }
                     if (masked) {
-                        const int* ri = reinterpret_cast<const int*>(Qs + M::T) + 2 * BT + n * 32 + half * 4;
+                        const int* ri = reinterpret_cast<const int*>(smem + M::R + st * M::ROWB) + 2 * BT + n * 32 + half * 4;
 #pragma unroll
                         for (int g4 = 0; g4 < 4; ++g4) {
                             const i32x4_t lo = lds_i4(ri + g4 * 8), hi = lds_i4(ri + BT + g4 * 8);
@@ -677,19 +683,28 @@ __device__ __forceinline__ void dkv_tile(const SpanArgs& p, unsigned id, unsigne
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const u32x4_t pf = pack_slots<false>(s, x), df = pack_slots<false>(g, x);      // P and dS rounded to bf16: operands
-                        if constexpr (!DV) *reinterpret_cast<u32x4_t*>(smem + M::P + ((st * 4 + w) * 2 + n) * 2048 + x * 1024 + lane * 16) = pf;
+                        if constexpr (ROLES) {
+                            made[x] = DV ? pf : df;
+                            *reinterpret_cast<u32x4_t*>(smem + M::X + ((st * 4 + w) * 2 + n) * 2048 + x * 1024 + lane * 16) = DV ? df : pf;
+                        } else {
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            if constexpr (DV) dv[c] = mfma32<false>(T::cols(Gs, 2 * n + x, c, lane), pf, dv[c]);
-                            dk[c] = mfma32<false>(T::cols(Qs, 2 * n + x, c, lane), df, dk[c]);
+                            for (int c = 0; c < D / 32; ++c) {
+                                dv[c] = mfma32<false>(T::cols(Gs, 2 * n + x, c, lane), pf, dv[c]);
+                                dk[c] = mfma32<false>(T::cols(Qs, 2 * n + x, c, lane), df, dk[c]);
+                            }
                         }
                     }
-                    paced_cols<(DV ? D / 16 : 0) + D / 16>();
+                    if constexpr (!ROLES) paced_cols<D / 8>();
+                }
+                if constexpr (!DV) product();
+                if constexpr (ROLES) {
+                    own[0] = made[0]; own[1] = made[1];
+                    p_at = at; p_st = st; p_g = gs;
                 }
             }
             if constexpr (ROLES) {
                 __syncthreads();
-                take_dv();
+                product();
             }
         }
         // ---- out; a key whose gradient is not finite -- another key's infinity or NaN met its zero weight in the matrix instruction -- is computed again from its own rows
