@@ -550,7 +550,7 @@ static int span_check(const mm_span_attn* a, bool bwd) {
     if (!(a->scale >= 1e-20f) || a->scale > 1e20f) return mm_set_error(MM_ERR_SHAPE, "span attention: scale must be positive (1e-20 .. 1e20)");
     if (a->softcap != 0.f && (!(a->softcap >= 1e-3f) || a->softcap > 1e4f)) return mm_set_error(MM_ERR_SHAPE, "span attention: softcap must be 0 (none) or 1e-3 .. 1e4");
     if (a->axes < 0 || a->axes > 3 || (a->slopes && a->axes == 0)) return mm_set_error(MM_ERR_SHAPE, "span attention: 1 to 3 axes for the distance bias");
-    if (a->slopes && (!a->positions_q || !a->positions_k)) return mm_set_error(MM_ERR_SHAPE, "span attention: slopes need positions of queries and keys");
+    if (a->slopes && ((a->nq > 0 && !a->positions_q) || (a->nk > 0 && !a->positions_k))) return mm_set_error(MM_ERR_SHAPE, "span attention: slopes need positions of queries and keys");
     if (a->spans && (((uintptr_t)a->spans) & 7)) return mm_set_error(MM_ERR_ALIGN, "span attention: spans must be 8-byte aligned");
     if (a->spans && a->spans_sb % 2) return mm_set_error(MM_ERR_ALIGN, "span attention: spans batch stride must be even");
     if (a->batch == 0) return MM_OK;

@@ -585,7 +585,7 @@ __global__ __launch_bounds__(1024) void span_order(const int32_t* __restrict__ s
 struct SpanPlan { bool narrow; int row_tiles, splits; };
 
 // The narrow form where the wide one would leave CUs without a workgroup (< 256 of them) or most of a workgroup's 128 rows empty (up to 32 queries: 16 new positions
-// over caches of 16384 keys, 16 / 4 heads of 128: 505 us wide).  There: 2 workgroups' worth of splits per CU, at least 256 keys each (two tiles a wave).
+// over caches of 16384 keys, 16 / 4 heads of 128: 505 us wide, 105 narrow).  There: 2 workgroups' worth of splits per CU, at least 256 keys each (two tiles a wave).
 SpanPlan span_plan(const mm_span_attn* a) {
     SpanPlan r;
     const long wide = (long)a->batch * a->heads_q * ((a->nq + WQ - 1) / WQ);

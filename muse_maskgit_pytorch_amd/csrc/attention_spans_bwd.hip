@@ -433,8 +433,10 @@ struct BwdForm {
 
 // 128 keys of a key head against the query tiles that see them: a wave holds 32 keys as operands (K, V) and their gradients as accumulators.
 // ROLES (128 wide heads): 8 waves, the first four take dV, the others dK of the same keys -- both gradients and both operands are 192 registers, which leaves one wave
-// per SIMD and every latency in the open (942 us for dk and dv of 2 x 16 heads of 4096 x 4096, and 695 so); S is computed in both for it, 5 products
-// for 4.  Narrower heads take both gradients in one wave, two or three of which fit a SIMD.
+// per SIMD and every latency in the open.  The two waves of 32 keys make the scores, P and dS of half a query tile's rows each; what the other one multiplies by goes
+// through LDS and is taken a tile later, dV's wave in front of its next scores, dK's behind them (Q and dO have three stages for it).  2 x 16 heads of 4096 x 4096, dq, dk
+// and dv: S twice in waves of their own 1.10 ms (dk and dv alone 695 us; both in one wave 942), P handed over 1.05, scores shared 1.00 (capped, where the scores cost more:
+// 1.31, 1.23 and 1.15).  Narrower heads take both gradients in one wave, two or three of which fit a SIMD.
 template <int D, int AX>
 struct DkvLds {
     // [ST] Q, [ST] dO, [2] per row: lse', delta, lo, hi, positions; with pairs [2] the operand that each of the eight waves has for its partner; the list

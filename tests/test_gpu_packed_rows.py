@@ -528,3 +528,45 @@ def test_everything_broken_ends_soon():
     assert dq.isnan().all() and dk.isnan().all() and dv.isnan().all()
     out, lse = ops.attend_spans(q, k, torch.full_like(v, math.nan), return_lse=True)
     assert out.isnan().all() and lse.isfinite().all()
+
+
+@pytest.mark.parametrize('hq,hk,d', [(8, 1, 128), (4, 2, 64)])
+def test_rows_behind_the_last_document_on_a_poisoned_workspace(hq, hk, d):
+    """300 rows of documents in 900: whole key tiles that nothing sees get zeros from every split, whatever the workspace and those rows held"""
+    g = gen(93)
+    n = 900
+    q = torch.randn(1, n, hq, d, generator=g).to(torch.bfloat16).to(DEV).transpose(1, 2)
+    k, v = (torch.randn(1, n, hk, d, generator=g).to(torch.bfloat16).to(DEV).transpose(1, 2) for _ in range(2))
+    spans = ops.attention_spans(torch.tensor([0, 120, 300], dtype=torch.int32, device=DEV), n, causal=True)
+    s, pos = torch.rand(hq, 1, generator=g).to(DEV), torch.arange(n, dtype=torch.int32, device=DEV)[:, None]
+    kw = dict(scale=d ** -0.5, slopes=s, positions=pos)
+    out, lse = ops.attend_spans(q, k, v, spans, return_lse=True, **kw)
+    dout = torch.randn(out.shape, generator=g).to(torch.bfloat16).to(DEV)
+    short = [t[:, :, :300] for t in (q, k, v, out, lse, dout)]
+    want = ops.attend_spans_bwd(*short, spans[:300], scale=d ** -0.5, slopes=s, positions=pos[:300])
+    for t in (q, k, v, dout):
+        t[:, :, 300:] = math.nan
+    for _ in range(3):
+        held = [torch.full((1 << 23,), math.nan, device=DEV) for _ in range(2)]
+        torch.cuda.synchronize()
+        del held
+        got = ops.attend_spans_bwd(q, k, v, out, lse, dout, spans, **kw)
+        for a, b in zip(got[:3], want[:3]):
+            assert (a[:, :, 300:] == 0).all()
+            # other splits and tiles than the short call's: the sums' order, one rounding to bf16 apart, and that of the terms' sizes
+            torch.testing.assert_close(a[:, :, :300].float(), b.float(), rtol=2 ** -7, atol=2 ** -7 * float(b.float().abs().max()))
+        torch.testing.assert_close(got[3], want[3], rtol=1e-4, atol=1e-4 * float(want[3].abs().max()))
+
+
+@pytest.mark.parametrize('n,j', [(0, 50), (50, 0), (0, 0)])
+def test_attention_of_nothing(n, j):
+    q = torch.ones(2, 4, n, 64, dtype=torch.bfloat16, device=DEV)
+    k, v = (torch.ones(2, 2, j, 64, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    pq, pk = (torch.zeros(x, 2, dtype=torch.int32, device=DEV) for x in (n, j))
+    kw = dict(slopes=torch.ones(4, 2, device=DEV), positions=pq, key_positions=pk)
+    out, lse = ops.attend_spans(q, k, v, return_lse=True, **kw)
+    assert out.shape == q.shape and (out == 0).all() and (lse == -math.inf).all()
+    dq, dk, dv, ds = ops.attend_spans_bwd(q, k, v, out, lse, q, **kw)
+    assert dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape
+    for t in (dq, dk, dv, ds):
+        assert (t == 0).all()
