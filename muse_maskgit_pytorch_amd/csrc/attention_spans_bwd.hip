@@ -89,7 +89,7 @@ __device__ __forceinline__ void sum_slope_parts(const SpanArgs& p, int threads, 
         const int c = c0 + t % lanes, chain = t / lanes;
         float v = 0.f;
         if (c < n)
-            for (long x = chain; x < parts; x += 32) v += p.dsl_part[x * n + c];
+            for (long x = chain; x < parts; x += 32) v += __hip_atomic_load(&p.dsl_part[x * n + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         red[chain * lanes + t % lanes] = v;
         __syncthreads();
@@ -174,12 +174,17 @@ __device__ __forceinline__ void dq_tile(const SpanArgs& p, unsigned id, unsigned
     const bool ok = i < p.nq;
     int lo = 0, hi = 0;
     float lse2 = 0.f, delta = 0.f;
-    if (ok) {
-        const int2 sp = row_span(p, b, h, i);
-        lo = sp.x; hi = sp.y;
+    if (ok) {      // (all of a row's numbers at once: they come one memory latency later, not three)
         const long row = ((long)b * p.Hq + h) * p.nq + i;
-        lse2 = hi > lo ? p.lse[row] * SPAN_LOG2E : 0.f;
-        delta = hi > lo ? p.delta[row] : 0.f;      // (a row that sees nothing may hold anything)
+        const float l = p.lse[row], dl = p.delta[row];
+        lo = 0; hi = p.nk;
+        if (p.spans) {
+            const int2 sp = reinterpret_cast<const int2*>(p.spans + b * p.spans_sb)[i];
+            lo = max(sp.x, 0); hi = min(sp.y, p.nk);
+        }
+        if (lo >= hi || l == -INFINITY) lo = hi = 0;
+        lse2 = hi > lo ? l * SPAN_LOG2E : 0.f;
+        delta = hi > lo ? dl : 0.f;      // (a row that sees nothing may hold anything)
     }
     int h0 = hi > lo ? lo : INT32_MAX, h1 = hi;
     for (int o = 16; o > 0; o >>= 1) { h0 = min(h0, __shfl_xor(h0, o, 64)); h1 = max(h1, __shfl_xor(h1, o, 64)); }
@@ -367,13 +372,15 @@ __device__ __forceinline__ void dq_tile(const SpanArgs& p, unsigned id, unsigned
             if (threadIdx.x < AX) {
                 float v = ((fr[t] + fr[4 + t]) + fr[8 + t]) + fr[12 + t];
                 if constexpr (GROUPS > 1) v += ((fr[16 + t] + fr[20 + t]) + fr[24 + t]) + fr[28 + t];
-                p.dsl_part[((long)b * tiles + tile) * p.Hq * AX + h * AX + t] = v;
+                __hip_atomic_store(&p.dsl_part[((long)b * tiles + tile) * p.Hq * AX + h * AX + t], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
+            // the parts are stored and loaded at the scope of the card (past the XCD's L2), so that the count only has to wait until its workgroup's are there; a release
+            // would write back the whole L2, once a workgroup
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (threadIdx.x == 0) red[0] = __hip_atomic_fetch_add(p.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1u == (unsigned)(p.B * p.Hq * tiles);
+            if (threadIdx.x == 0) red[0] = __hip_atomic_fetch_add(p.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == (unsigned)(p.B * p.Hq * tiles);
             __syncthreads();
             if (red[0]) {
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
                 sum_slope_parts(p, GROUPS * 256, reinterpret_cast<float*>(smem));
             }
         }
