@@ -585,17 +585,24 @@ __global__ __launch_bounds__(1024) void span_order(const int32_t* __restrict__ s
 struct SpanPlan { bool narrow; int row_tiles, splits; };
 
 // The narrow form where the wide one would leave CUs without a workgroup (< 256 of them) or most of a workgroup's 128 rows empty (up to 32 queries: 16 new positions
-// over caches of 16384 keys, 16 / 4 heads of 128: 505 us wide, 105 narrow).  There: 2 workgroups' worth of splits per CU, at least 256 keys each (two tiles a wave).
+// over caches of 16384 keys, 16 / 4 heads of 128: 505 us wide, 105 narrow).  There the keys are split for one to four rounds of the workgroups that the card holds (one a CU
+// 128 wide, two narrower: their LDS), at least 256 keys each (two tiles a wave), whichever is least in keys a workgroup passes over, its start and the join counted as 512 each.
+// (8 heads of 1089 x 1089, 128 wide: 32 us whole, 37 in two splits and a round more; 8 key heads of 60000 keys, one position: 55 us in one round, 64 in two; 130 positions
+// of 2 x 16 / 4 heads over 5000 keys: 47 in three splits, two rounds, 52 whole on half the CUs)
 SpanPlan span_plan(const mm_span_attn* a) {
     SpanPlan r;
     const long wide = (long)a->batch * a->heads_q * ((a->nq + WQ - 1) / WQ);
     const long rows = (long)(a->heads_q / a->heads_k) * a->nq;
     r.row_tiles = (int)((rows + 31) / 32);
     r.narrow = wide < 256 || a->nq <= 32;
-    const long wgs = (long)a->batch * a->heads_k * r.row_tiles;
-    long s = (512 + wgs - 1) / wgs;
-    const long most = (a->nk + 255) / 256;
-    r.splits = r.narrow ? (int)(s < 1 ? 1 : (s > most ? (most < 1 ? 1 : most) : s)) : 1;
+    r.splits = 1;
+    if (!r.narrow) return r;
+    const long wgs = (long)a->batch * a->heads_k * r.row_tiles, slots = a->dim == 128 ? 256 : 512, most = (a->nk + 255) / 256;
+    const auto cost = [&](long s) { return (wgs * s + slots - 1) / slots * ((a->nk + s - 1) / s + 512) + (s > 1 ? 512 : 0); };
+    for (long rounds = 1; rounds <= 4; ++rounds) {
+        const long s = rounds * slots / wgs < most ? rounds * slots / wgs : most;
+        if (s > 1 && cost(s) < cost(r.splits)) r.splits = (int)s;
+    }
     return r;
 }
 
