@@ -570,3 +570,54 @@ def test_attention_of_nothing(n, j):
     assert dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape
     for t in (dq, dk, dv, ds):
         assert (t == 0).all()
+
+
+@pytest.mark.parametrize('n', [1, 600])
+def test_a_cache_whose_offsets_pass_32_bits(n):
+    """the last 700 of 2^19 rows, 4608 elements apart: byte offsets above 2^32, element offsets above 2^31; the rows before hold NaN and are not seen"""
+    g = gen(94)
+    j, seen, hq, d = 1 << 19, 700, 64, 128
+    rows = torch.full((1, j, 4608), math.nan, dtype=torch.bfloat16, device=DEV)
+    kv = torch.randn(1, seen, 2, d, generator=g).to(torch.bfloat16).to(DEV)
+    rows[:, -seen:, :d], rows[:, -seen:, 4352:4352 + d] = kv[:, :, 0], kv[:, :, 1]
+    k, v = rows[:, None, :, :d], rows[:, None, :, 4352:4352 + d]
+    q, dout = (torch.randn(1, hq, n, d, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    at = torch.arange(n, dtype=torch.int32, device=DEV)
+    near = torch.stack([at * 0, at + seen - n + 1], 1).to(torch.int32)
+    far = near + (j - seen)
+    kw = dict(scale=d ** -0.5, softcap=20.0)
+    close = lambda a, b: torch.testing.assert_close(a.float(), b.float(), rtol=2 ** -7, atol=2 ** -7 * float(b.float().abs().max()))      # (one rounding to bf16 each, and that of P)
+    kc, vc = kv[:, None, :, 0].contiguous(), kv[:, None, :, 1].contiguous()
+    out, lse = ops.attend_spans(q, k, v, far, return_lse=True, **kw)
+    want, want_lse = ops.attend_spans(q, kc, vc, near, return_lse=True, **kw)
+    close(out, want)
+    torch.testing.assert_close(lse, want_lse, rtol=1e-5, atol=1e-5)
+    dq, dk, dv, _ = ops.attend_spans_bwd(q, k, v, want, want_lse, dout, far, **kw)
+    wq, wk, wv, _ = ops.attend_spans_bwd(q, kc, vc, want, want_lse, dout, near, **kw)
+    close(dq, wq)
+    close(dk[:, :, -seen:], wk)
+    close(dv[:, :, -seen:], wv)
+    assert (dk[:, :, :-seen] == 0).all() and (dv[:, :, :-seen] == 0).all()
+
+
+def test_two_streams_at_once():
+    """gradients with slopes on two streams side by side, over and over: each call's workspace and counts are its own"""
+    g = gen(95)
+    n, h, d = 1500, 8, 64
+    s, pos = torch.rand(h, 2, generator=g).to(DEV), torch.stack([torch.arange(n) // 40, torch.arange(n) % 40], 1).to(torch.int32).to(DEV)
+    spans = ops.attention_spans(torch.tensor([0, 500, 1300], dtype=torch.int32, device=DEV), n)
+    kw = dict(slopes=s, positions=pos)
+    sets = []
+    for _ in range(2):
+        q, k, v, w = (torch.randn(1, n, h, d, generator=g).to(torch.bfloat16).to(DEV).transpose(1, 2) for _ in range(4))
+        out, lse = ops.attend_spans(q, k, v, spans, return_lse=True, **kw)
+        sets.append(((q, k, v, out, lse, w, spans), ops.attend_spans_bwd(q, k, v, out, lse, w, spans, **kw), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for a, _, stream in sets:
+            with torch.cuda.stream(stream):
+                got.append(ops.attend_spans_bwd(*a, **kw))
+        torch.cuda.synchronize()
+        for (_, want, _), x in zip(sets, got):
+            assert all(torch.equal(c, e) for c, e in zip(x, want))
