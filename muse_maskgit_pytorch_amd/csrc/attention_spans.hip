@@ -585,7 +585,7 @@ __global__ __launch_bounds__(1024) void span_order(const int32_t* __restrict__ s
 struct SpanPlan { bool narrow; int row_tiles, splits; };
 
 // The narrow form where the wide one would leave CUs without a workgroup (< 256 of them) or most of a workgroup's 128 rows empty (up to 32 queries: 16 new positions
-// over caches of 16384 keys, 16 / 4 heads of 128: 505 us wide, 105 narrow).  There the keys are split for one to four rounds of the workgroups that the card holds (one a CU
+// over caches of 16384 keys, 16 / 4 heads of 128: 505 us wide, 99 narrow).  There the keys are split for one to four rounds of the workgroups that the card holds (one a CU
 // 128 wide, two narrower: their LDS), at least 256 keys each (two tiles a wave), whichever is least in keys a workgroup passes over, its start and the join counted as 512 each.
 // (8 heads of 1089 x 1089, 128 wide: 32 us whole, 37 in two splits and a round more; 8 key heads of 60000 keys, one position: 55 us in one round, 64 in two; 130 positions
 // of 2 x 16 / 4 heads over 5000 keys: 47 in three splits, two rounds, 52 whole on half the CUs)
