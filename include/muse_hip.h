@@ -275,8 +275,9 @@ int mm_qk_norm_bwd(mm_stream_t stream, const void* x, int64_t ldx, const float* 
 
 /* Which keys a query row sees, as one interval per row: out int32 [B][n][2] = (lo, hi), keys lo <= k < hi of a key row of j keys.  Document doc owns the query rows
  * cu_q[doc] <= i < cu_q[doc + 1] and the keys cu_k[doc] <= k < cu_k[doc + 1] (int32 [docs + 1], not decreasing; q_sb / k_sb / p_sb: batch strides in elements, 0 = one
- * table for all rows; bounds outside [0, j] are clamped).  causal != 0: query i of lq sees the first i + 1 + lk - lq of its document's lk keys, and at least the first
- * prefix[doc] of them (optional int32 [docs]).  Rows of no document see nothing: (0, 0). */
+ * table for all rows).  causal != 0: query i of lq sees the first i + 1 + lk - lq of its document's lk keys, and at least the first prefix[doc] of them (optional int32
+ * [docs]).  Bounds may lie in front of or behind the n rows and j keys (a document that is cut off): lengths and order go by the bounds as they are, then keys outside
+ * [0, j) are cut off.  Rows of no document see nothing: (0, 0). */
 int mm_attention_spans(mm_stream_t stream, const int32_t* cu_q, int64_t q_sb, const int32_t* cu_k, int64_t k_sb, const int32_t* prefix, int64_t p_sb,
                        int B, int docs, int n, int j, int causal, int32_t* out);
 

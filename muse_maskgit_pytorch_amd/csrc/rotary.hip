@@ -37,16 +37,16 @@ __global__ __launch_bounds__(256) void attention_spans_kernel(const int32_t* __r
     int2 r = make_int2(0, 0);
     const int doc = a - 1;
     if (doc >= 0 && doc < docs) {
-        const int q0 = cq[doc], q1 = cq[doc + 1];
-        const int k0 = min(max(ck[doc], 0), j), k1 = min(max(ck[doc + 1], k0), j);
-        const int lk = k1 - k0;
-        int seen = lk;
+        // by the document's own lengths, in 64 bits (bounds may be any int32); what lies outside the j keys is cut off at the end: cut first, a document that goes on
+        // behind the row would lose keys but no queries, and its causal diagonal would move
+        const long k0 = ck[doc], lk = max((long)ck[doc + 1] - k0, 0L);
+        long seen = lk;
         if (causal) {
-            seen = i - q0 + 1 + lk - (q1 - q0);      // the last row of a document sees all of its keys
-            if (prefix) seen = max(seen, prefix[b * p_sb + doc]);
-            seen = min(max(seen, 0), lk);
+            seen = i + 1 + lk - cq[doc + 1];      // the last row of a document sees all of its keys
+            if (prefix) seen = max(seen, (long)prefix[b * p_sb + doc]);
+            seen = min(max(seen, 0L), lk);
         }
-        r = make_int2(k0, k0 + seen);
+        r = make_int2((int)min(max(k0, 0L), (long)j), (int)min(max(k0 + seen, 0L), (long)j));
     }
     out[(long)b * n + i] = r;
 }

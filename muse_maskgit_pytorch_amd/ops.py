@@ -891,7 +891,8 @@ def attention_spans(cu_q, n, cu_k=None, j=None, prefix=None, causal=False):
     cu_q[doc] <= i < cu_q[doc + 1]; cu_k (default cu_q) and j (default n): the same of the keys (j key rows).  causal: query i of a document with lq
     queries and lk keys sees the first i + 1 + lk - lq keys, and at least the first prefix[doc] (int32 [docs], needs causal).  [b, docs + 1] tables
     (and [b, docs] prefixes) give [b, n, 2].  Rows of no document see nothing: (0, 0).  What the bounds hold is not checked (they are on the GPU):
-    they must not decrease; what lies outside the j keys is cut off."""
+    they must not decrease.  A document may begin in front of the rows and keys or go on behind them: causal order and prefix go by the whole document,
+    then what lies outside the j keys is cut off."""
     docs = cu_q.shape[-1] - 1 if cu_q.dim() else -1
     if j is None:
         if cu_k is not None:

@@ -51,6 +51,38 @@ def test_spans_of_a_batch_and_of_bounds_that_do_not_start_at_zero():
     assert got.cpu().tolist() == [[0, 4]] * 4 + [[4, 10]] * 4
 
 
+CUT = [  # cu_q, cu_k, prefix, n, j: bounds behind the rows and keys or in front of them (a window of a longer packing), the last document cut off inside
+    ([0, 4, 20], None, None, 8, 8), ([0, 4, 20], None, None, 10, 10), ([0, 4, 20], None, [0, 3], 10, 10), ([0, 4, 20], None, [2, 9], 10, 7), ([-5, 3, 6], None, None, 9, 9),
+    ([-5, 3, 6], None, [4, 2], 9, 9), ([0, 3, 9], [0, 5, 40], None, 9, 12), ([0, 3, 9], [-4, 5, 40], [3, 20], 9, 12), ([0, 3, 9], [-4, -2, 6], [1, 1], 9, 12),
+    ([0, 3, 9], [14, 20, 30], None, 9, 12), ([0, 6, 2 ** 31 - 1], None, None, 300, 290), ([-2 ** 31, 6, 2 ** 31 - 1], None, [5, 7], 300, 300)]
+
+
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('case', CUT, ids=lambda c: f'{c[0]}-{c[1]}-{c[2]}-{c[3]}-{c[4]}')
+def test_spans_of_documents_that_are_cut_off(case, causal):
+    """what a row sees goes by the whole document; then what lies outside the j keys is cut off"""
+    cu_q, cu_k, prefix, n, j = case
+    if prefix is not None and not causal:
+        prefix = None
+    ck = cu_q if cu_k is None else cu_k
+    want = []
+    for i in range(n):
+        doc = max((d for d in range(len(cu_q)) if cu_q[d] <= i), default=-1)
+        if not 0 <= doc < len(cu_q) - 1:
+            want.append([0, 0])
+            continue
+        lq, lk = cu_q[doc + 1] - cu_q[doc], ck[doc + 1] - ck[doc]
+        seen = lk
+        if causal:
+            seen = min(lk, max(0, i - cu_q[doc] + 1 + lk - lq, prefix[doc] if prefix else 0))
+        want.append([min(max(ck[doc], 0), j), min(max(ck[doc] + seen, 0), j)])
+    t = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device=DEV)
+    got = ops.attention_spans(t(cu_q), n, cu_k=t(cu_k), j=j, prefix=t(prefix), causal=causal)
+    assert got.tolist() == want
+    two = lambda x: None if x is None else torch.stack([t(x)] * 2)
+    assert ops.attention_spans(two(cu_q), n, cu_k=two(cu_k), j=j, prefix=two(prefix), causal=causal).tolist() == [want] * 2
+
+
 # ------------------------------------------------------------------------------------------------ rotary
 ROT = [  # b, n, hq, hk, d, sections, interleaved
     (1, 1, 1, 1, 32, [16], False), (2, 37, 8, 8, 64, [16, 16], False), (3, 65, 4, 1, 128, [8, 20, 20], False), (2, 19, 6, 2, 64, [8, 8, 8], True),
