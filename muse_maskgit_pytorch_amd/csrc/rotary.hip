@@ -89,24 +89,19 @@ __device__ __forceinline__ void rot_store(T* p, const float (&f)[VEC]) {
     *reinterpret_cast<RotVec<T, VEC>*>(p) = r;
 }
 
+// the lane's pairs from `turned` on lie behind the P that turn: they pass as they are (a turn by 0 would not do: 0 times a neighbour's infinity is NaN)
 template <int VEC, bool INTER>
-__device__ __forceinline__ void rot_turn(float (&a)[VEC], float (&b)[VEC], const float (&c)[VEC], const float (&s)[VEC]) {
-    if constexpr (!INTER || VEC == 1) {
+__device__ __forceinline__ void rot_turn(float (&a)[VEC], float (&b)[VEC], const float (&c)[VEC], const float (&s)[VEC], int turned) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float x = a[e], y = b[e];
-            a[e] = __builtin_fmaf(x, c[e], -(y * s[e]));
-            b[e] = __builtin_fmaf(x, s[e], y * c[e]);
-        }
-    } else {      // the unit's 2 VEC consecutive elements hold its VEC pairs: (a0 a1) (a2 a3) .. (b0 b1) ..
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float& x_ = 2 * e < VEC ? a[(2 * e) % VEC] : b[(2 * e) % VEC];
-            float& y_ = 2 * e < VEC ? a[(2 * e + 1) % VEC] : b[(2 * e + 1) % VEC];
-            const float x = x_, y = y_;
-            x_ = __builtin_fmaf(x, c[e], -(y * s[e]));
-            y_ = __builtin_fmaf(x, s[e], y * c[e]);
-        }
+    for (int e = 0; e < VEC; ++e) {
+        // interleaved: the unit's 2 VEC consecutive elements hold its VEC pairs, (a0 a1) (a2 a3) .. (b0 b1) ..
+        constexpr bool beside = INTER && VEC > 1;
+        float& x_ = !beside ? a[e] : (2 * e < VEC ? a[(2 * e) % VEC] : b[(2 * e) % VEC]);
+        float& y_ = !beside ? b[e] : (2 * e < VEC ? a[(2 * e + 1) % VEC] : b[(2 * e + 1) % VEC]);
+        const float x = x_, y = y_;
+        const bool on = (beside ? e : 0) < turned;
+        x_ = on ? __builtin_fmaf(x, c[e], -(y * s[e])) : x;
+        y_ = on ? __builtin_fmaf(x, s[e], y * c[e]) : y;
     }
 }
 
@@ -123,6 +118,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs p) {
     __shared__ __attribute__((aligned(16))) float2 turns[ROT_TURNS];
     const int G = p.G, u = threadIdx.x & (G - 1), slots = 256 / G, slot = threadIdx.x / G, pairs = p.d / 2;
     const bool live = u < p.d / (2 * VEC);
+    const int turned = p.P - u * VEC;      // how many of the lane's pairs turn (none or all of them unless interleaved)
     int offa, offb;
     if (INTER) { offa = 2 * VEC * u; offb = offa + VEC; }
     else if (u * VEC < p.P) { offa = u * VEC; offb = p.P + u * VEC; }
@@ -211,9 +207,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs p) {
 #pragma unroll
                             for (int e = 0; e < VEC; ++e) { xa[e] = xa[e] * inv * sa[e]; xb[e] = xb[e] * inv * sb[e]; }
                         }
-                        rot_turn<VEC, INTER>(xa, xb, c, s);
+                        rot_turn<VEC, INTER>(xa, xb, c, s, turned);
                     } else {
-                        rot_turn<VEC, INTER>(ga, gb, c, s);
+                        rot_turn<VEC, INTER>(ga, gb, c, s, turned);
                         if constexpr (NORM) {
                             float dot = 0.f;
 #pragma unroll

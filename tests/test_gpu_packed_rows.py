@@ -162,6 +162,31 @@ def test_rotary_bwd(shape, norm, dtype):
         assert x is None and y is None or torch.equal(x, y)
 
 
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('shape', [(2, 37, 3, 1, 128, [8, 20, 20], False), (2, 33, 3, 3, 20, [3, 2], False), (1, 40, 4, 2, 64, [8, 8, 7], True), (1, 9, 2, 1, 24, [1, 2, 3, 4], True),
+                                   (1, 6, 2, 1, 64, [0, 0], False)], ids=str)
+def test_rotary_elements_behind_the_pairs_pass_as_they_are(shape, dtype):
+    """infinities, NaN and zeros of either sign behind the pairs, alone and beside each other: bit for bit the same in both directions, and the pairs in front know nothing of them"""
+    b, n, hq, hk, d, sections, inter = shape
+    rows, q, k, pos, freqs, _, _, g = rot_inputs(*shape[:6], dtype, 13)
+    P = sum(sections)
+    odd = torch.tensor([math.inf, -math.inf, math.nan, 0.0, -0.0, 3.0, -2.0], dtype=rows.dtype)
+    rows[..., 2 * P:] = odd[torch.randint(0, 7, rows[..., 2 * P:].shape, generator=g)]
+    r = rows.to(DEV)
+    bits = {2: torch.int16, 4: torch.int32}[rows.element_size()]
+    a, c = r[:, :, :hq].transpose(1, 2), r[:, :, hq:hq + hk].transpose(1, 2)
+    fwd = ops.rotary_axes(a, c, pos.to(DEV), freqs.to(DEV), sections, interleaved=inter)
+    bwd = ops.rotary_axes_bwd(a, c, pos.to(DEV), freqs.to(DEV), sections, interleaved=inter)
+    for back, got in ((False, fwd), (True, bwd[:2])):
+        for x, y in ((q, got[0]), (k, got[1])):
+            y = y.cpu()
+            same = y[..., 2 * P:].contiguous().view(bits) == x[..., 2 * P:].contiguous().view(bits)
+            assert (same | (x[..., 2 * P:].isnan() & y[..., 2 * P:].isnan())).all()
+            z = x.double()[..., :2 * P]
+            want = R.turn(z, pos, freqs, sections, inter, back=back)
+            R.check(y[..., :2 * P], want, rot_tol(want, pair_size(z, sections, inter), R.HALF[x.dtype]), 'pairs')
+
+
 def test_rotary_far_positions_keep_their_angle():
     n, d = 64, 64
     pos = (2 ** 30 - 1 - 977 * torch.arange(n)).to(torch.int32)[:, None]
