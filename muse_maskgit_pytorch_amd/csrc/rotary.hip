@@ -338,12 +338,13 @@ int k_rotary(hipStream_t s, const mm_rotary* r, bool bwd, float* ws, float* dsca
     const bool norm = r->normalize != 0;
     const RotPlan pl = rot_plan(r->batch, r->n, r->dim, wide ? 8 : 1, norm && bwd);
     a.G = pl.G; a.TB = pl.TB; a.part = ws;
-    if (pl.gx > 0 && r->q.heads + r->k.heads > 0) {
+    const bool any = pl.gx > 0 && r->q.heads + r->k.heads > 0;
+    if (any) {
         if (r->dtype == MM_DT_F32) { if (wide) rot_launch<float, 8>(s, a, pl, norm, bwd); else rot_launch<float, 1>(s, a, pl, norm, bwd); }
         else if (r->dtype == MM_DT_F16) { if (wide) rot_launch<_Float16, 8>(s, a, pl, norm, bwd); else rot_launch<_Float16, 1>(s, a, pl, norm, bwd); }
         else { if (wide) rot_launch<__bf16, 8>(s, a, pl, norm, bwd); else rot_launch<__bf16, 1>(s, a, pl, norm, bwd); }
         const int rc = mm_check_launch("rotary_kernel");
         if (rc) return rc;
     }
-    return norm && bwd ? k_colsum(s, ws, pl.gx, 2 * r->dim, dscales) : MM_OK;      // (no rows: zeros)
+    return norm && bwd ? k_colsum(s, ws, any ? pl.gx : 0, 2 * r->dim, dscales) : MM_OK;      // (no rows or no heads: zeros)
 }

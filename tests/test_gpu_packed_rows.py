@@ -230,6 +230,21 @@ def test_rotary_of_nothing_and_of_a_zero_row():
     assert torch.equal(y, x)
 
 
+def test_rotary_gradient_of_no_heads():
+    """scales whose q or k has no heads: their gradients are zeros, whatever the workspace held"""
+    freqs, pos, s = torch.ones(16, dtype=torch.float64, device=DEV), torch.zeros(700, 1, dtype=torch.int32, device=DEV), torch.ones(32, device=DEV)
+    none, some = torch.zeros(1, 0, 700, 32, device=DEV), torch.randn(1, 2, 700, 32, generator=gen(14)).to(DEV)
+    want = ops.rotary_axes_bwd(some, None, pos, freqs, [16], q=some, q_scale=s)[2]
+    for q, k in ((none, None), (none, none), (none, some), (some, none)):
+        held = [torch.full((1 << 18,), math.nan, device=DEV) for _ in range(4)]
+        torch.cuda.synchronize()
+        del held
+        dq, dk, ds, dks = ops.rotary_axes_bwd(q, k, pos, freqs, [16], q=q, k=k, q_scale=s, k_scale=None if k is None else s)
+        assert dq.shape == q.shape and (k is None or dk.shape == k.shape)
+        for x, y in ((q, ds), (k, dks)):
+            assert y is None and x is None or torch.equal(y, want if x is some else torch.zeros_like(s))
+
+
 # ------------------------------------------------------------------------------------------------ attention
 def att_inputs(b, hq, hk, n, j, d, dtype, mask, cap, axes, seed, unit=None):
     """operands on the CPU, spans, key mask, positions; the key rows are views of wider rows, as a projection leaves them"""
