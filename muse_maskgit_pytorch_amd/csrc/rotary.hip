@@ -195,12 +195,15 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs p) {
                         }
                     }
                     float inv = 1.f;
+                    bool below = false;      // the row is divided by the constant, whose derivative is 0: no projection in its gradient
                     if constexpr (NORM) {
                         float ss = 0.f;
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) ss = __builtin_fmaf(xa[e], xa[e], __builtin_fmaf(xb[e], xb[e], ss));
                         ss = rot_group_sum(ss, G);
-                        inv = 1.f / fmaxf(sqrtf(ss), 1e-12f);      // F.normalize eps (mmp.py:41-42)
+                        const float len = sqrtf(ss);
+                        below = len < 1e-12f;
+                        inv = 1.f / fmaxf(len, 1e-12f);      // F.normalize eps (mmp.py:41-42)
                     }
                     if constexpr (!BWD) {
                         if constexpr (NORM) {
@@ -221,6 +224,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs p) {
                                 dot = __builtin_fmaf(xa[e], ga[e], __builtin_fmaf(xb[e], gb[e], dot));
                             }
                             dot = rot_group_sum(dot, G);
+                            if (below) dot = 0.f;
 #pragma unroll
                             for (int e = 0; e < VEC; ++e) { xa[e] = __builtin_fmaf(-xa[e], dot, ga[e]) * inv; xb[e] = __builtin_fmaf(-xb[e], dot, gb[e]) * inv; }
                         } else {

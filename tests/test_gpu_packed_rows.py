@@ -245,6 +245,29 @@ def test_rotary_gradient_of_no_heads():
             assert y is None and x is None or torch.equal(y, want if x is some else torch.zeros_like(s))
 
 
+@pytest.mark.parametrize('dtype', ['bf16', 'fp32'])
+@pytest.mark.parametrize('d,sections,inter', [(64, [16, 16], False), (20, [3, 2], False), (64, [8, 8, 7], True)])
+def test_rotary_gradient_of_rows_below_the_norms_floor(d, sections, inter, dtype):
+    """rows shorter than 1e-12 are divided by that constant: no projection in their gradient; against autograd of the formula in 64 bits"""
+    sizes = torch.tensor([0.0, 1e-20, 1e-14, 3e-13, 8e-13, 9.8e-13, 1.03e-12, 3e-12, 1.0])
+    n, g = len(sizes), gen(15)
+    x = torch.randn(1, 2, n, d, generator=g)
+    x = (x / x.norm(dim=-1, keepdim=True) * sizes[:, None]).to(DT[dtype])
+    dy = torch.randn(1, 2, n, d, generator=g).to(DT[dtype])
+    pos = torch.randint(0, 50, (n, len(sections)), generator=g).to(torch.int32)
+    freqs = torch.cat([100.0 ** (-torch.arange(s, dtype=torch.float64) / s) for s in sections])
+    s = 1 + 0.3 * torch.randn(d, generator=g)
+    dx, _, ds, _ = ops.rotary_axes_bwd(dy.to(DEV), None, pos.to(DEV), freqs.to(DEV), sections, q=x.to(DEV), q_scale=s.to(DEV), interleaved=inter)
+    leaf, scale = x.double().requires_grad_(), s.double().requires_grad_()
+    ln = leaf.norm(dim=-1, keepdim=True).clamp(min=1e-12)
+    gr = R.turn(dy.double(), pos[None], freqs, sections, inter, back=True)
+    want, want_s = torch.autograd.grad((leaf / ln * scale * gr).sum(), (leaf, scale))
+    ln, xh, size = ln.detach(), (leaf / ln).detach().abs(), pair_size(dy.double(), sections, inter)
+    mag = (size * s.double().abs() + xh * (xh * size * s.double().abs()).sum(-1, keepdim=True)) / ln
+    R.check(dx, want, rot_tol(want, mag * d / 8, R.HALF[x.dtype]), 'dx')
+    R.check(ds[None], want_s[None], (R.F32 * (24 + d + 2 * math.sqrt(2 * n)) * (size * xh).sum((0, 1, 2)))[None], 'scale')
+
+
 # ------------------------------------------------------------------------------------------------ attention
 def att_inputs(b, hq, hk, n, j, d, dtype, mask, cap, axes, seed, unit=None):
     """operands on the CPU, spans, key mask, positions; the key rows are views of wider rows, as a projection leaves them"""
