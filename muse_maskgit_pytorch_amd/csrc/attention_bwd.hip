@@ -374,12 +374,13 @@ __global__ __launch_bounds__(256) void qk_norm_bwd_kernel(const bf16_t* __restri
         float ss = (xv[0] * xv[0] + xv[1] * xv[1]) + (xv[2] * xv[2] + xv[3] * xv[3]);
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) ss += __shfl_xor(ss, o, 64);
-        const float inv = 1.f / fmaxf(sqrtf(ss), 1e-12f);
+        const float len = sqrtf(ss), inv = 1.f / fmaxf(len, 1e-12f);
         float xh[4], g[4], dotv = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) { xh[j] = xv[j] * inv; g[j] = gy[j] * sc[j]; dotv += xh[j] * g[j]; acc[j] += gy[j] * xh[j]; }
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) dotv += __shfl_xor(dotv, o, 64);
+        if (len < 1e-12f) dotv = 0.f;      // (divided by the constant, whose derivative is 0: no projection)
         float o4[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) o4[j] = (g[j] - xh[j] * dotv) * inv;

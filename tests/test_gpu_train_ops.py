@@ -265,3 +265,36 @@ def test_ce_bwd_on_long_rows_reads_every_row_once(ops, R, V):
     assert torch.equal(a, b)
     assert (a.float().cpu() - logits.grad).abs().max() < 2 ** -8 * logits.grad.abs().max()      # (bf16 output: half an ulp of the label's (p - 1) / R entry)
     assert abs(a.float().sum(dim=1).cpu()).max() < 2 ** -7 / R          # rows of softmax - onehot sum to ~0 (bf16 rounding of 65536 entries)
+
+
+def test_qk_norm_bwd_of_rows_below_the_norms_floor(ops):
+    """rows shorter than 1e-12 are divided by that constant (F.normalize's eps, mmp.py:41-42): no projection in their gradient; against autograd in 64 bits, both forms"""
+    g = torch.Generator().manual_seed(31)
+    sizes = torch.tensor([0.0, 1e-20, 1e-14, 3e-13, 8e-13, 9.8e-13, 1.03e-12, 3e-12, 1.0])
+    H, n = 2, len(sizes)
+    x = torch.randn(n, H, 64, generator=g)
+    x = (x / x.norm(dim=-1, keepdim=True) * sizes[:, None, None]).to(torch.bfloat16)
+    scale = 1 + 0.3 * torch.randn(64, generator=g)
+
+    def want(x, dy):
+        leaf, s = x.double().requires_grad_(), scale.double().requires_grad_()
+        y = leaf / leaf.norm(dim=-1, keepdim=True).clamp(min=1e-12) * s
+        dx, ds = torch.autograd.grad((y * dy.double()).sum(), (leaf, s))
+        ln = x.double().norm(dim=-1, keepdim=True).clamp(min=1e-12)
+        xh, gs = (x.double() / ln).abs(), (dy.double() * scale.double()).abs()
+        # fp32: sums of 64 products (norm and dot), half a dozen roundings; of the terms' sizes
+        return dx, ds, 2.0 ** -24 * (64 + 16) * (gs + xh * (xh * gs).sum(-1, keepdim=True)) / ln, 2.0 ** -24 * (64 + 16 + dy[..., 0].numel()) * (dy.double().abs() * xh).sum((0, 1))
+
+    def check(got, ref, tol):
+        assert ((got.cpu().double() - ref).abs() <= tol).all(), float(((got.cpu().double() - ref).abs() / tol.clamp(min=1e-300)).max())
+    dy = torch.randn(n, H, 64, generator=g).to(torch.bfloat16)
+    dx, ds = ops.qk_norm_bwd(x.reshape(n, H * 64).to(DEV), dy.reshape(n, H * 64).to(DEV), scale.to(DEV), H)
+    ref, ref_s, tol, tol_s = want(x, dy)
+    check(dx.reshape(n, H, 64), ref, tol + 2.0 ** -8 * 1.01 * ref.abs() + 1e-30)
+    check(ds, ref_s, tol_s)
+    xf = x.reshape(n * H, 64).float()                         # the null key's form: one fp32 vector a head, gradients of every row of the batch
+    dyf = torch.randn(3 * n * H, 64, generator=g)
+    dx, ds = ops.qk_norm_bwd(None, None, scale.to(DEV), n * H, x_f32=xf.to(DEV), dy_f32=dyf.to(DEV))
+    ref, ref_s, tol, tol_s = want(xf.repeat(3, 1)[:, None], dyf[:, None])
+    check(dx[:, None], ref, tol + 2.0 ** -24 * ref.abs() + 1e-30)
+    check(ds, ref_s, tol_s)
