@@ -187,6 +187,26 @@ def test_rotary_elements_behind_the_pairs_pass_as_they_are(shape, dtype):
             R.check(y[..., :2 * P], want, rot_tol(want, pair_size(z, sections, inter), R.HALF[x.dtype]), 'pairs')
 
 
+LONG_ROT = [  # several tokens a workgroup (tokens / 1024, in the gradient behind the norm / 512), a ragged last group, groups over two rows of the batch
+    (1, 5003, 3, 2, 64, [16, 16], False), (3, 1671, 2, 3, 32, [5, 7], True), (1, 5003, 3, 2, 20, [3, 2], False), (1, 2100, 70, 1, 64, [8, 24], False), (2, 1300, 1, 70, 24, [1, 2, 3, 4], True),
+    # more tokens than 2048 workgroups hold at a time: k makes its turns again
+    (1, 33001, 1, 1, 256, [32, 32, 64], False), (2, 33001, 1, 2, 128, [9, 20, 20], False)]
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp32'])
+@pytest.mark.parametrize('norm', [False, True])
+@pytest.mark.parametrize('shape', LONG_ROT, ids=str)
+def test_rotary_of_several_tokens_a_workgroup(shape, norm, dtype):
+    test_rotary(shape, norm, dtype)
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp32'])
+@pytest.mark.parametrize('norm', [False, True])
+@pytest.mark.parametrize('shape', LONG_ROT, ids=str)
+def test_rotary_bwd_of_several_tokens_a_workgroup(shape, norm, dtype):
+    test_rotary_bwd(shape, norm, dtype)
+
+
 def test_rotary_far_positions_keep_their_angle():
     n, d = 64, 64
     pos = (2 ** 30 - 1 - 977 * torch.arange(n)).to(torch.int32)[:, None]
@@ -716,3 +736,43 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
         for (_, want, _), x in zip(sets, got):
             assert all(torch.equal(c, e) for c, e in zip(x, want))
+
+
+MANY = [  # tiles sorted longest first (batch x tiles x heads >= 512 with spans), too many of them to sort (more than 4096), documents that end inside tiles
+    (16, 16, 4, 257, 257, 64, 'bf16', 'docs', 0.0, 2), (16, 16, 4, 257, 257, 128, 'bf16', 'docs', 30.0, 1), (16, 16, 16, 150, 150, 64, 'bf16', 'docs', 0.0, 2),
+    (8, 32, 8, 300, 300, 32, 'bf16', 'prefix', 0.0, 0), (16, 16, 16, 260, 90, 64, 'bf16', 'any', 20.0, 0), (2100, 1, 1, 130, 130, 32, 'bf16', 'any', 0.0, 0)]
+
+
+@pytest.mark.parametrize('case', MANY, ids=lambda c: '-'.join(map(str, c)))
+def test_attend_spans_of_many_tiles(case):
+    test_attend_spans(case)
+
+
+MANY_BWD = MANY + [
+    # heads that share a key head: two workgroups of two heads each, one of all four, three of two (batch x key heads x key tiles against 512)
+    (8, 16, 4, 70, 1100, 64, 'bf16', 'none', 0.0, 2), (8, 16, 4, 70, 1100, 128, 'bf16', 'both', 30.0, 1), (16, 16, 4, 50, 1100, 128, 'bf16', 'any', 0.0, 0),
+    (16, 16, 4, 50, 1100, 32, 'bf16', 'keys', 0.0, 1), (9, 24, 4, 40, 700, 64, 'bf16', 'any', 20.0, 3),
+    # more than 256 tiles of 64 queries: the list of a key tile in two stretches
+    (1, 2, 2, 16500, 40, 128, 'bf16', 'none', 0.0, 0), (1, 2, 1, 16500, 140, 128, 'bf16', 'any', 20.0, 2), (1, 2, 2, 16500, 200, 64, 'bf16', 'docs', 0.0, 1)]
+
+
+@pytest.mark.parametrize('case', MANY_BWD, ids=lambda c: '-'.join(map(str, c)))
+def test_attend_spans_bwd_of_many_tiles(case):
+    test_attend_spans_bwd(case)
+
+
+def test_everything_broken_in_bounded_time():
+    """a diverged step of 4096 x 4096, gradients and forward: every row and key is looked at again, each until its first sum that is not finite -- milliseconds; a walk over all
+    of its pairs would take each 64 times as long and the call seconds"""
+    g = gen(92)
+    q, k, v = (torch.randn(1, 4, 4096, 64, generator=g).to(torch.bfloat16).to(DEV) for _ in range(3))
+    out, lse = ops.attend_spans(q, k, v, return_lse=True)
+    bad = torch.full_like(out, math.nan)
+    for call in (lambda: ops.attend_spans(q, k, bad), lambda: ops.attend_spans_bwd(q, k, v, out, lse, bad)):
+        call()
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        assert a.elapsed_time(b) < 200, 'ms'
