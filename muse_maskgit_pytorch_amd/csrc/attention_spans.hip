@@ -89,12 +89,15 @@ struct Form {
     __device__ __forceinline__ float score(float y) const { return __builtin_fmaf(y, ka, kb); }
 };
 
-// the running maximum moves only when some row's grows by more than 2^8: P stays below 2^8, exact enough in 16 bits, and most tiles rescale nothing
-template <int D>
+// The weights' reference m follows the running maximum: it moves only when some row's maximum passes m + TOP, and then to UP below it.  Most tiles rescale nothing.
+// bf16: P stays below 2^8.  fp16 has no exponents to spare: weights below 2^-24 would vanish as operands, though a long cache of them counts (131072 keys of 2^-25 beside one
+// key of 1: 0 for 0.003), and those below 2^-14 lose bits.  There P lies between 2^10 and 2^14 at a row's maximum, so that weights down to 2^-24 of it keep all their bits.
+template <int D, bool F16>
 __device__ __forceinline__ void rescale(float tmax, float& m, float& l, f32x16_t (&o)[D / 32]) {
+    constexpr float UP = F16 ? 10.f : 0.f, TOP = F16 ? 14.f : 8.f;
     tmax = both_halves_max(tmax);
-    if (__any(tmax > m + 8.f)) {
-        const float mn = fmaxf(m, tmax), f = __builtin_amdgcn_exp2f(m - mn);
+    if (__any(tmax > m + TOP)) {
+        const float mn = fmaxf(m, tmax - UP), f = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         l *= f;
 #pragma unroll
@@ -276,7 +279,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
                 F.hide(s[0], (uint32_t)bits);
                 F.hide(s[1], (uint32_t)(bits >> 32));
             }
-            rescale<D>(F.score(F.extreme(s[1], F.extreme(s[0], Form<CAP, AX>::worst()))), m, l, o);
+            rescale<D, F16>(F.score(F.extreme(s[1], F.extreme(s[0], Form<CAP, AX>::worst()))), m, l, o);
             const float kbm = F.kb - m;
             u32x4_t pf = probs<F16>(s[0], 0, F.ka, kbm, l);
 #pragma unroll
@@ -442,7 +445,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
                 F.y4(s, g * 4, pq, pk);
             }
         if (keep != 0xFFFFFFFFu || !__all(lo <= t0 && hi >= t0 + 32)) F.hide(s, (uint32_t)((bit_range(lo - t0, hi - t0) & (unsigned long long)keep) >> (4 * half)));
-        rescale<D>(F.score(F.extreme(s, Form<CAP, AX>::worst())), m, l, o);
+        rescale<D, F16>(F.score(F.extreme(s, Form<CAP, AX>::worst())), m, l, o);
         const float kbm = F.kb - m;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {

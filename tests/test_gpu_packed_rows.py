@@ -394,6 +394,39 @@ def test_attend_spans_what_is_hidden_stays_out(case, value, where):
         assert not out.cpu()[rest].isfinite().all(-1).any()
 
 
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+@pytest.mark.parametrize('hq,n,j,drop', [(1, 1, 1 << 19, 17.6), (1, 1, 1 << 19, 20.0), (8, 1, 1 << 16, 15.0), (1, 40, 1 << 17, 17.6), (128, 129, 1 << 17, 17.6), (128, 129, 1 << 13, 14.0)])
+def test_a_long_tail_of_small_weights(hq, n, j, drop, dtype):
+    """one key that takes nearly everything before a long cache of keys whose weights are each below the smallest fp16 number (2^-24 of it) but together some
+    thousandths: they count, in the narrow and the wide form"""
+    d, t = 32, DT[dtype]
+    q, k, v = torch.zeros(1, hq, n, d, dtype=t), torch.zeros(1, 1, j, d, dtype=t), torch.ones(1, 1, j, d, dtype=t)
+    q[..., 0] = 1.0
+    v[:, :, 5, ::2] = 0.0                                     # the one key's value: 0 in the even elements, 1 in the odd ones
+    k[:, :, 5, 0] = drop
+    k, v, q = k.to(DEV), v.to(DEV), q.to(DEV)
+    out, lse = ops.attend_spans(q, k, v, scale=1.0, return_lse=True)
+    top = float(torch.tensor(drop, dtype=t))
+    tail = (j - 1) * math.exp(-top)
+    want = torch.full(out.shape, tail / (1 + tail), dtype=torch.float64)
+    want[..., 1::2] = 1.0
+    # P and the result rounded once each; the sum in 32 bits: a lane has every other group of 4 keys, half of them, and adds them 8 at a time, so j / 16 additions to
+    # a sum of about 1, each off by at most 2^-24 of it
+    tol = want * (2.04 * R.HALF[t] + R.F32 * (64 + j / 16)) + 2.0 ** -24
+    R.check(out, want, tol, 'out')
+    R.check(lse, torch.full(lse.shape, top + math.log1p(tail), dtype=torch.float64), torch.full(lse.shape, R.F32 * (64 + j / 16 + 8 * top), dtype=torch.float64), 'lse')
+
+
+@pytest.mark.parametrize('hq,n', [(2, 3), (128, 129)])
+def test_subnormal_fp16_values_count(hq, n):
+    """values below 2^-14 in fp16, as they are"""
+    v = (torch.randint(-1000, 1001, (1, 1, 300, 64), generator=gen(97)) * 2.0 ** -24).to(torch.float16)
+    q, k = torch.zeros(1, hq, n, 64, dtype=torch.float16), torch.zeros(1, 1, 300, 64, dtype=torch.float16)
+    out = ops.attend_spans(q.to(DEV), k.to(DEV), v.to(DEV), scale=1.0)
+    want = v.double().mean(2, keepdim=True).expand(1, hq, n, 64)
+    R.check(out, want, 2.0 ** -25 * 1.01 + want.abs() * (2.0 ** -11 + 64 * R.F32), 'out')      # (P is 1: the result's rounding alone, to whole 2^-24)
+
+
 def test_attend_spans_sees_through_strides_and_expanded_operands():
     """keys shared by a batch (batch stride 0), token-major and head-major operands, a slice of a longer cache"""
     g = gen(9)
