@@ -52,8 +52,8 @@ struct Form {
         for (int a = 0; a < AX; ++a) sl[a] = CAP ? p.slopes[h * AX + a] * SPAN_LOG2E : p.slopes[h * AX + a] / p.scale;
     }
     float c2;
-    // 4 consecutive keys (k: their positions).  Positions are whole numbers below 2^24, exact in fp32 and so are their differences: a subtraction and a
-    // multiply-add with |.| an axis and score
+    // 4 consecutive keys (k: their positions).  Positions are whole numbers below 2^24 in size, exact in fp32; a distance is too up to 2^24, and rounded once above (signs
+    // apart): a subtraction and a multiply-add with |.| an axis and score
     __device__ __forceinline__ void y4(f32x16_t& s, int r, const float (&pq)[AX ? AX : 1], const f32x4_t (&k)[AX ? AX : 1]) const {
         float v[4] = {s[r], s[r + 1], s[r + 2], s[r + 3]};
         if constexpr (CAP) {

@@ -56,7 +56,6 @@ template <bool F16> __device__ __forceinline__ float to_f32(uint16_t v) {
 template <bool F16> __device__ __forceinline__ u32x4_t pack_slots(const f32x16_t& c, int s) {      // (s: a constant after unrolling)
     return u32x4_t{pack2<F16>(c[8 * s], c[8 * s + 1]), pack2<F16>(c[8 * s + 2], c[8 * s + 3]), pack2<F16>(c[8 * s + 4], c[8 * s + 5]), pack2<F16>(c[8 * s + 6], c[8 * s + 7])};
 }
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 __device__ __forceinline__ float both_halves_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));

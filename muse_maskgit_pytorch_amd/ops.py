@@ -847,7 +847,8 @@ def cfg_mix(emb_cond, emb_null, cond_scale, D, products=None):
 
 # ------------------------------------------------------------------------------------------------ packed rows: spans, rotary positions, attention
 # These calls are short (a few microseconds of GPU time for a small batch), so their host side is kept lean: one plain test per rule, the descriptor packed in one go
-# (mm_rotary / mm_span_attn: no padding between their fields), the stream handle without a Stream object.
+# (mm_rotary / mm_span_attn: no padding between their fields), the stream handle without a Stream object.  Like all operators here they record no autograd graph: a
+# result has no grad_fn whatever its inputs require, gradients come from the _bwd calls.
 _DT = {torch.bfloat16: L.MM_DT_BF16, torch.float16: L.MM_DT_F16, torch.float32: L.MM_DT_F32}
 _ROTARY = struct.Struct('=10q2i10q2i3q12i')
 _SPAN = struct.Struct('=26q8i2f17q')
@@ -997,7 +998,7 @@ def rotary_axes(q, k, positions, freqs, sections, q_scale=None, k_scale=None, in
     (elements of a head contiguous).  positions int32 (n, axes) or (b, n, axes); sections: how many pairs turn with each axis, in order; freqs float64 [their sum]:
     radians per unit of position.  Pairs are elements (p, P + p), interleaved: (2p, 2p + 1); the elements behind the pairs pass.  With q_scale / k_scale fp32 [d]
     the heads are l2-normalised and scaled first (mmp.py:151-153).  d even, up to 128 (256 where rows are 16-byte aligned and the sections add up to a multiple of
-    8 with a rest of whole 16 elements).  Returns (q', k') as (b, h, n, d) views of [b, n, h, d] rows."""
+    8 with a rest of whole 16 elements).  Returns (q', k') as (b, h, n, d) views of [b, n, h, d] rows.  No autograd graph: rotary_axes_bwd has the gradients."""
     desc, outs, stream, keep = _rotary(q, k, positions, freqs, sections, q_scale, k_scale, interleaved, False)
     L.check(L.lib().mm_rotary_axes(stream, desc), 'mm_rotary_axes')
     return tuple(outs)
@@ -1089,7 +1090,8 @@ def attend_spans(q, k, v, spans=None, scale=8.0, softcap=0.0, slopes=None, posit
     """Attention of packed rows: q (b, hq, n, d), k / v (b, hk, j, d), bf16 or fp16, d = 32 / 64 / 128, hk a divisor of hq (shared key heads), strided views
     with 16-byte aligned rows.  A query sees the keys of its span (int32 (n, 2) or (b, n, 2), ops.attention_spans; None: all) that key_mask (b, j) keeps.
     softcap > 0 (1e-3 .. 1e4; the score keeps the absolute precision of softcap in fp32): scores are softcap * tanh(score / softcap).  slopes fp32 (hq, axes) and positions / key_positions int32 (n, axes) / (j, axes) (or (b, .., axes);
-    key_positions default: positions): sum over the axes of slope * |distance| is taken off the score; |position| < 2^24.  A row that sees nothing gives 0
+    key_positions default: positions): sum over the axes of slope * |distance| is taken off the score; |position| < 2^24.  Scores are fp32, up to 1e7 in size (beyond,
+    32 bits do not tell one from the next).  No autograd graph: attend_spans_bwd has the gradients.  A row that sees nothing gives 0
     (lse -inf); what a row does not see never reaches it, infinities and NaN included.  Returns (b, hq, n, d) (a view of rows), out_rows: [b * n, hq * d], and with
     return_lse also the log of the sum of exp(score), fp32 (b, hq, n)."""
     head, sizes, stream, keep = _span_args(q, k, v, spans, scale, softcap, slopes, positions, key_positions, key_mask, ())
@@ -1112,7 +1114,7 @@ _NO_GRADS = (0,) * 17
 def attend_spans_bwd(q, k, v, out, lse, dout, spans=None, scale=8.0, softcap=0.0, slopes=None, positions=None, key_positions=None, key_mask=None):
     """Gradients of attend_spans (bf16) from its inputs, its out (b, hq, n, d) and lse, and dout, the gradient of out: (dq, dk, dv, dslopes) -- dq (b, hq, n, d),
     dk / dv (b, hk, j, d) as views of rows, dslopes fp32 (hq, axes) or None without slopes.  dk and dv are summed over the heads that share a key head.  Rows that
-    see nothing (lse -inf) and keys that nothing sees get and give 0, whatever they hold.  No atomics: the same bits every time."""
+    see nothing (lse -inf) and keys that nothing sees get and give 0, whatever they hold.  Every sum has one order: the same bits every time."""
     for name, t in (('out', out), ('dout', dout)):
         if t.shape != q.shape or t.dtype != q.dtype:
             raise _Err(f'attend_spans_bwd: {name} {t.dtype} {tuple(t.shape)} beside q {q.dtype} {tuple(q.shape)}')

@@ -427,6 +427,29 @@ def test_subnormal_fp16_values_count(hq, n):
     R.check(out, want, 2.0 ** -25 * 1.01 + want.abs() * (2.0 ** -11 + 64 * R.F32), 'out')      # (P is 1: the result's rounding alone, to whole 2^-24)
 
 
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+@pytest.mark.parametrize('hq,n', [(2, 3), (128, 129)])
+@pytest.mark.parametrize('sign', [1.0, -1.0])
+def test_scores_of_1e7(sign, hq, n, dtype):
+    """the largest scores that are taken: 63 keys of the same score of 9e6 in size and 64 far below them; the weights are 1 / 63, whatever the score's last bit is worth"""
+    t = DT[dtype]
+    q, k = torch.zeros(1, hq, n, 32, dtype=t), torch.zeros(1, 1, 127, 32, dtype=t)
+    q[..., 3], q[..., 7] = 3008.0, 256.0
+    k[..., 3] = 3008.0 * sign
+    k[:, :, 1::2, 7] = -2.0                                     # scores 512 lower: products of 8 bits each, exact in fp32
+    v = torch.randn(1, 1, 127, 32, generator=gen(98)).to(t)
+    k[:, :, 0, 7] = -2.0
+    out, lse = ops.attend_spans(q.to(DEV), k.to(DEV), v.to(DEV), scale=1.0, return_lse=True)
+    best = k[0, 0, :, 7] == 0
+    assert int(best.sum()) == 63
+    w = v[0, 0, best].double()
+    want = w.mean(0).expand(out.shape)
+    # P is the same number for all of them (2^0 .. 2^16, one rounding), and so is the sum's share; the result's rounding
+    R.check(out, want, w.abs().mean(0).expand(out.shape) * (2.04 * R.HALF[t] + 64 * R.F32), 'out')
+    top = 3008.0 ** 2 * sign
+    R.check(lse, torch.full(lse.shape, top + math.log(63), dtype=torch.float64), torch.full(lse.shape, 4 * R.F32 * abs(top), dtype=torch.float64), 'lse')
+
+
 def test_attend_spans_sees_through_strides_and_expanded_operands():
     """keys shared by a batch (batch stride 0), token-major and head-major operands, a slice of a longer cache"""
     g = gen(9)

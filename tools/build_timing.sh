@@ -5,7 +5,7 @@
 set -e
 P=muse_maskgit_pytorch_amd
 mkdir -p tools/build/t
-FL="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-fast-math -ffp-contract=off -DMM_GEMM_TIMING -DMM_TOOLS_PP -I$P/csrc"
+FL="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-fast-math -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops -DMM_GEMM_TIMING -DMM_TOOLS_PP -I$P/csrc"
 /opt/rocm/bin/hipcc $FL -c tools/experiments/gemm_pp.hip -o tools/build/t/gemm_pp.o &
 /opt/rocm/bin/hipcc $FL -c $P/csrc/gemm_wide.hip -o tools/build/t/gemm_wide.o &
 wait
