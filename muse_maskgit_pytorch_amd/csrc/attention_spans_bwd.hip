@@ -211,7 +211,8 @@ __device__ __forceinline__ void dq_tile(const SpanArgs& p, unsigned id, unsigned
     const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1];
     const uint8_t* km = p.kmask ? p.kmask + b * p.km_sb : nullptr;
     const int* pkp = AX ? p.pos_k + b * p.pk_sb : nullptr;
-    const float c1 = CAP ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E, c2 = p.cap * SPAN_LOG2E;
+    constexpr bool SLOPES = CAP && AX > 0;      // fp32 gradients of slopes behind a cap: span_tanh_block
+    const float c1 = SLOPES ? p.scale / p.cap : (CAP ? 2.f * p.scale * SPAN_LOG2E / p.cap : p.scale * SPAN_LOG2E), c2 = p.cap * SPAN_LOG2E;
 
 #define SPAN_ISSUE(it_)                                                                                                \
     {                                                                                                                  \
@@ -263,6 +264,8 @@ __device__ __forceinline__ void dq_tile(const SpanArgs& p, unsigned id, unsigned
                     s = mfma32<false>(T::rows(Ks, c, n, lane), qf[c], s);
                     g = mfma32<false>(T::rows(Vs, c, n, lane), gf[c], g);
                 }
+                SpanTanh tanh;
+                if constexpr (SLOPES) tanh = span_tanh_block(s, c1);
                 const uint32_t wb = (uint32_t)(bits >> (32 * n));
                 int pos = ((it & 1) * GROUPS + grp) * STAGE + 2 * T::BYTES + (n * 32 + half * 4) * 4;
                 f32x4_t kq[AX ? AX : 1], kn[AX ? AX : 1];      // positions of four keys, and of the next four
@@ -278,7 +281,7 @@ __device__ __forceinline__ void dq_tile(const SpanArgs& p, unsigned id, unsigned
                     for (int e = 0; e < 4; ++e) {
                         const int r = g4 * 4 + e;
                         float x;
-                        if constexpr (CAP) { const float th = span_tanh(s[r], c1); slope[e] = __builtin_fmaf(-th, th, 1.f); x = __builtin_fmaf(th, c2, -lse2); }
+                        if constexpr (CAP) { const float th = SLOPES ? span_tanh_poly(s[r] * tanh.k, tanh.c) : span_tanh(s[r], c1); slope[e] = __builtin_fmaf(-th, th, 1.f); x = __builtin_fmaf(th, c2, -lse2); }
                         else x = __builtin_fmaf(s[r], c1, -lse2);
 #pragma unroll
                         for (int a = 0; a < AX; ++a) {

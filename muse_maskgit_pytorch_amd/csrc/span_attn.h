@@ -136,9 +136,42 @@ __device__ __forceinline__ unsigned long long bit_range(int a, int e) {
 }
 
 // s in units of log2: cap(scale q.k) * log2 e.  cap tanh(x / cap) = cap (1 - 2 / (exp(2 x / cap) + 1)): one exp2 and one reciprocal; the absolute error is an fp32
-// rounding of cap.  c1 = scale * log2 e without a cap, 2 * scale * log2 e / cap with one; c2 = cap * log2 e.
+// rounding of cap, enough in front of weights that are rounded to 16 bits (in 2 x 16 heads of 4096 x 4096 the forward takes 338 us with it, 128 wide, and 353 with the polynomial
+// below; long documents 99 and 109).  c1 = scale * log2 e without a cap, 2 * scale * log2 e / cap with one; c2 = cap * log2 e.
 __device__ __forceinline__ float span_tanh(float x, float c1) {
     return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f), 1.f);
+}
+
+// tanh(u) to a few fp32 roundings of its own size, for the slopes' gradient: that is fp32, and a score that is off by a rounding of its cap leaves it 3 - 15 times as far from the
+// 64-bit form as a plain fp32 form is (scores of a few units under caps of 30 and 50).  |u| <= 1/2: u times a polynomial in u^2 (the minimax of the relative error, 1.5e-8, with 1 in
+// front; Remez's exchange); beyond, the exponential.  A wave whose scores are all below takes the polynomial alone; otherwise the scores become their tanh first and the polynomial
+// leaves them as they are (its coefficients are 0): one code for both, and a score's value is the same either way, whatever stands beside it.
+struct SpanTanh { float k, c[4]; };
+__device__ __forceinline__ float span_tanh_poly(float u, const float (&c)[4]) {
+    const float v = u * u;
+    float t = __builtin_fmaf(c[3], v, c[2]);
+    t = __builtin_fmaf(t, v, c[1]);
+    t = __builtin_fmaf(t, v, c[0]);
+    return u * __builtin_fmaf(t, v, 1.f);
+}
+// a block of raw scores in front of span_tanh_poly(raw * .k, .c) = tanh(raw k)
+__device__ __forceinline__ SpanTanh span_tanh_block(f32x16_t& s, float k) {
+    constexpr float C[4] = {-0.333331436f, 0.133258790f, -0.0530454926f, 0.0172414910f};
+    float m[4] = {0.f, 0.f, 0.f, 0.f};      // (a NaN is passed over: the polynomial keeps it)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m[r & 3] = fmaxf(m[r & 3], fabsf(s[r]));
+    const bool near = __all(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * k <= 0.5f);
+    if (!near)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float u = s[r] * k, far = span_tanh(u, 2.f * SPAN_LOG2E);
+            s[r] = fabsf(u) <= 0.5f ? span_tanh_poly(u, C) : far;
+        }
+    SpanTanh t;
+    t.k = near ? k : 1.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) t.c[x] = near ? C[x] : 0.f;
+    return t;
 }
 
 // dot product of two rows by one lane

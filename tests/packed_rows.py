@@ -55,7 +55,7 @@ def visible(n, j, spans=None, key_mask=None, b=1):
     return seen
 
 
-def attention(q, k, v, seen, scale, cap=0.0, slopes=None, pos_q=None, pos_k=None, dout=None, out=None, lse=None):
+def attention(q, k, v, seen, scale, cap=0.0, slopes=None, pos_q=None, pos_k=None, dout=None, out=None, lse=None, tight_cap=False):
     """float64 results and their bounds: forward {out, lse}, with dout (and the forward's out / lse, taken as they are) {dq, dk, dv, dslopes}; each with a tensor
     of what the kernel's roundings may change.  Hidden keys and rows are taken out of the operands (their values, NaN among them, take no part)."""
     dt, half = q.dtype, HALF[q.dtype]
@@ -87,7 +87,7 @@ def attention(q, k, v, seen, scale, cap=0.0, slopes=None, pos_q=None, pos_k=None
             if cap:
                 t = torch.tanh(raw / cap)
                 s, slope = cap * t, 1 - t * t
-                serr = serr + F32 * 8 * cap      # 1 - 2 / (exp + 1): roundings of 1, times cap
+                serr = serr + F32 * 8 * (s.abs() if tight_cap else cap)      # a few roundings, of the cap's size or (tight_cap) of the score's own
             far = []
             if slopes is not None:
                 pq, pk = (p if p.dim() == 3 else p[None].expand(b, -1, -1) for p in (pos_q, pos_k))

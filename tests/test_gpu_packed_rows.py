@@ -562,6 +562,34 @@ def test_attend_spans_gradients_against_differences():
         assert abs(float((grad * e).sum()) - diff) < 3 * 2.0 ** -8 * float((grad * e).abs().sum()) + 1e-6, ('q', 'k', 'v', 'slopes')[n]
 
 
+@pytest.mark.parametrize('d,hk', [(32, 2), (64, 4), (128, 2)])
+@pytest.mark.parametrize('cap,axes', [(1000.0, 1), (10000.0, 2)])
+@pytest.mark.parametrize('big', [False, True])
+def test_slope_gradients_behind_a_cap_far_above_the_scores(d, hk, cap, axes, big):
+    """the slopes' gradient, which no rounding to 16 bits follows, of scores of a few units under a large cap, and (big) of a few beyond it among them: within fp32 roundings of the
+    scores' own size, not of the cap's"""
+    x = att_inputs(2, 4, hk, 5, 6, d, 'bf16', 'none', cap, axes, seed=99)
+    # one element a head: the products are exact, so that the bound is that of the cap alone; few pairs, whose errors do not cancel
+    keep = x['q'][..., :1].clone()
+    x['q'].zero_()
+    x['q'][..., :1] = keep
+    x['kv'][..., 1:] = 0
+    x['scale'] = 2.0
+    if big:
+        x['q'][:, :, 0, 0], x['kv'][:, 3, :hk, 0] = 1.5, 1.25 * cap
+    f = plain(x)
+    out, lse = f['out'].to(torch.bfloat16), f['lse'].float()
+    args, kw = on_gpu(x)
+    dout = torch.randn(out.shape, generator=gen(100)).to(torch.bfloat16)
+    dout[..., 1:] = 0
+    got = ops.attend_spans_bwd(*args[:3], out.to(DEV), lse.to(DEV), dout.to(DEV), args[3], **kw)
+    want = plain(x, dout=dout, out=out, lse=lse)
+    for name, t in zip(('dq', 'dk', 'dv'), got):
+        R.check(t, want[name], want[name + '_tol'], name)
+    want = plain(x, dout=dout, out=out, lse=lse, tight_cap=True)
+    R.check(got[3], want['dslopes'], want['dslopes_tol'], 'dslopes')
+
+
 def test_packed_training_pass_of_all_operators_together():
     """a layer's attention over a packed row, as a model runs it: projection rows -> l2norm, scales and positions -> attention by document with a distance bias, and
     the way back; against the same chain in 64 bits"""
