@@ -92,12 +92,13 @@ struct Form {
 // The weights' reference m follows the running maximum: it moves only when some row's maximum passes m + TOP, and then to UP below it.  Most tiles rescale nothing.
 // bf16: P stays below 2^8.  fp16 has no exponents to spare: weights below 2^-24 would vanish as operands, though a long cache of them counts (131072 keys of 2^-25 beside one
 // key of 1: 0 for 0.003), and those below 2^-14 lose bits.  There P lies between 2^10 and 2^14 at a row's maximum, so that weights down to 2^-24 of it keep all their bits.
+template <bool F16> constexpr float UP = F16 ? 10.f : 0.f;
+template <bool F16> constexpr float TOP = F16 ? 14.f : 8.f;
 template <int D, bool F16>
 __device__ __forceinline__ void rescale(float tmax, float& m, float& l, f32x16_t (&o)[D / 32]) {
-    constexpr float UP = F16 ? 10.f : 0.f, TOP = F16 ? 14.f : 8.f;
     tmax = both_halves_max(tmax);
-    if (__any(tmax > m + TOP)) {
-        const float mn = fmaxf(m, tmax - UP), f = __builtin_amdgcn_exp2f(m - mn);
+    if (__any(tmax > m + TOP<F16>)) {
+        const float mn = fmaxf(m, tmax - UP<F16>), f = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         l *= f;
 #pragma unroll
@@ -105,6 +106,13 @@ __device__ __forceinline__ void rescale(float tmax, float& m, float& l, f32x16_t
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[c][r] *= f;
     }
+}
+
+// lse of a row from its reference and its sum (the sum back in the maximum's units first: its logarithm is rounded at its own size); nothing seen: -inf
+template <bool F16>
+__device__ __forceinline__ float row_lse(float m, float l) {
+    constexpr float down = F16 ? 1.f / 1024.f : 1.f;      // 2^-UP
+    return l > 0.f ? (m + UP<F16> + __builtin_amdgcn_logf(l * down)) * SPAN_LN2 : (l == 0.f ? -INFINITY : l);
 }
 
 // 8 probabilities of a lane -> an operand.  Rounding of P to 16 bits: the product with V needs it; the sum takes the unrounded values
@@ -317,7 +325,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
 
     l = both_halves_sum(l);
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    if (p.lse && ok && half == 0) p.lse[((long)b * p.Hq + h) * p.nq + i] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * SPAN_LN2 : (l == 0.f ? -INFINITY : l);
+    if (p.lse && ok && half == 0) p.lse[((long)b * p.Hq + h) * p.nq + i] = row_lse<F16>(m, l);
     float bad = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
@@ -501,7 +509,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
 #pragma unroll
             for (int c = 0; c < D / 32; ++c)
                 *reinterpret_cast<uint2*>(op + (c * 8 + (t & 7)) * 4) = make_uint2(pack2<F16>(v[c].x * inv, v[c].y * inv), pack2<F16>(v[c].z * inv, v[c].w * inv));
-        if (p.lse && (t & 7) == 0) p.lse[((long)b * p.Hq + rh) * p.nq + ri] = L > 0.f ? (M + __builtin_amdgcn_logf(L)) * SPAN_LN2 : (L == 0.f ? -INFINITY : L);
+        if (p.lse && (t & 7) == 0) p.lse[((long)b * p.Hq + rh) * p.nq + ri] = row_lse<F16>(M, L);
     } else if (live) {
         float* po = p.part_o + (split * prows + prow) * D;
         if (!redo)
@@ -577,7 +585,7 @@ __global__ __launch_bounds__(256) void span_attn_join(const SpanArgs p) {
     const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
     *reinterpret_cast<uint2*>(p.out + b * p.o_s[0] + h * p.o_s[1] + (long)i * p.o_s[2] + c * 4) =
         make_uint2(pack2<F16>(v.x * inv, v.y * inv), pack2<F16>(v.z * inv, v.w * inv));
-    if (p.lse && c == 0) p.lse[((long)b * p.Hq + h) * p.nq + i] = L > 0.f ? (M + __builtin_amdgcn_logf(L)) * SPAN_LN2 : (L == 0.f ? -INFINITY : L);
+    if (p.lse && c == 0) p.lse[((long)b * p.Hq + h) * p.nq + i] = row_lse<F16>(M, L);
 }
 
 __global__ __launch_bounds__(1024) void span_order(const int32_t* __restrict__ spans, long sb, int B, int n, int nk, int32_t* __restrict__ order) {

@@ -450,6 +450,19 @@ def test_scores_of_1e7(sign, hq, n, dtype):
     R.check(lse, torch.full(lse.shape, top + math.log(63), dtype=torch.float64), torch.full(lse.shape, 4 * R.F32 * abs(top), dtype=torch.float64), 'lse')
 
 
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+@pytest.mark.parametrize('hq,n', [(1, 1), (128, 129)])
+def test_lse_of_few_keys_keeps_its_bits(hq, n, dtype):
+    """rows that see 1 .. 40 keys of score 0: lse is log(keys), whatever the weights are scaled by for their 16 bits"""
+    t, j = DT[dtype], 40
+    q, k = torch.zeros(j, hq, n, 32, dtype=t, device=DEV), torch.zeros(j, 1, j, 32, dtype=t, device=DEV)
+    spans = torch.stack([torch.zeros(j, n), (torch.arange(j) + 1.0)[:, None].expand(j, n)], 2).to(torch.int32)
+    _, lse = ops.attend_spans(q, k, k, spans.to(DEV), scale=1.0, return_lse=True)
+    want = torch.arange(1, j + 1).double().log()[:, None, None].expand(j, hq, n)
+    # the logarithm of a whole number (an ulp of up to 5.4), the reference beside it (0 or a power of two away), ln 2 and its product
+    R.check(lse, want, 5 * R.F32 * want + 1e-30, 'lse')
+
+
 def test_attend_spans_sees_through_strides_and_expanded_operands():
     """keys shared by a batch (batch stride 0), token-major and head-major operands, a slice of a longer cache"""
     g = gen(9)
