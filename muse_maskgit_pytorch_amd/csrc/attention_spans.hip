@@ -16,7 +16,7 @@ namespace {
 constexpr int WQ = SPAN_TILE, KT = 64;
 
 // sum over this row's visible keys in [k0, k1) of exp2(s - m) v, by one wave: lane = key for the scores, lane = element for the sum
-template <int D, bool F16, int AX>
+template <int D, bool F16, int AX, bool TANH>
 __device__ __forceinline__ void row_again(const SpanArgs& p, int b, int h, int i, int k0, int k1, float m, int lane, float (&o)[2]) {
     const uint16_t* q = p.q + b * p.q_s[0] + h * p.q_s[1] + (long)i * p.q_s[2];
     const int hk = h / (p.Hq / p.Hk);
@@ -28,7 +28,7 @@ __device__ __forceinline__ void row_again(const SpanArgs& p, int b, int h, int i
         const int key = t0 + lane;
         const bool sees = key < k1 && (!p.kmask || p.kmask[b * p.km_sb + key]);
         float w = 0.f, unused;
-        if (sees) w = __builtin_amdgcn_exp2f(pair_score<D, F16, AX>(p, q, kb + (long)key * p.k_s[2], b, h, i, key, &unused) - m);
+        if (sees) w = __builtin_amdgcn_exp2f(pair_score<D, F16, AX, TANH>(p, q, kb + (long)key * p.k_s[2], b, h, i, key, &unused) - m);
         rows_add<D, F16>(o, __ballot(sees), w, vb + (long)t0 * p.v_s[2], p.v_s[2], min(64, k1 - t0), lane);
     }
 }
@@ -38,16 +38,18 @@ __device__ __forceinline__ void row_again(const SpanArgs& p, int b, int h, int i
 //     cap, no bias:    r = 1 / (exp(2 raw scale / cap) + 1),     score = ka y + kb,  ka = -2 cap log2 e, kb = cap log2 e   (cap tanh(x) = cap - 2 cap r: smallest r)
 //     cap and bias:    cap tanh(..) - sum slope |distance|,      score = y           (all in units of log2)
 // and p = exp2(ka y + (kb - m)): one fused multiply-add in front of exp2 whatever the form.
-template <bool CAP, int AX>
+// TANH: the tanh itself comes in (span_tanh_block: a score to a few roundings of its own size, not of the cap's, and so the lse of a row of few keys); the cap without a bias
+// is then y = tanh, ka = cap log2 e, kb = 0.
+template <bool CAP, int AX, bool TANH = false>
 struct Form {
-    static constexpr bool falls = CAP && AX == 0;      // the score falls with y
+    static constexpr bool falls = CAP && AX == 0 && !TANH;      // the score falls with y
     float pre, ka, kb, sl[AX ? AX : 1];
     __device__ __forceinline__ void init(const SpanArgs& p, int h) {
         const float c1 = p.scale * SPAN_LOG2E;
         pre = CAP ? 2.f * c1 / p.cap : 1.f;
-        ka = CAP ? (AX ? 1.f : -2.f * p.cap * SPAN_LOG2E) : c1;
-        kb = CAP && !AX ? p.cap * SPAN_LOG2E : 0.f;
         c2 = p.cap * SPAN_LOG2E;
+        ka = CAP ? (AX ? 1.f : (TANH ? c2 : -2.f * c2)) : c1;
+        kb = falls ? c2 : 0.f;
 #pragma unroll
         for (int a = 0; a < AX; ++a) sl[a] = CAP ? p.slopes[h * AX + a] * SPAN_LOG2E : p.slopes[h * AX + a] / p.scale;
     }
@@ -56,7 +58,11 @@ struct Form {
     // apart): a subtraction and a multiply-add with |.| an axis and score
     __device__ __forceinline__ void y4(f32x16_t& s, int r, const float (&pq)[AX ? AX : 1], const f32x4_t (&k)[AX ? AX : 1]) const {
         float v[4] = {s[r], s[r + 1], s[r + 2], s[r + 3]};
-        if constexpr (CAP) {
+        if constexpr (CAP && TANH) {
+            if constexpr (AX > 0)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] *= c2;
+        } else if constexpr (CAP) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 v[e] = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v[e] * pre) + 1.f);
@@ -349,7 +355,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_wide(const SpanArgs p) {
         todo &= todo - 1;
         const int ri = tile * WQ + w * 32 + r;
         float ro[2];
-        row_again<D, F16, AX>(p, b, h, ri, __shfl(lo, r, 64), __shfl(hi, r, 64), __shfl(m, r, 64), lane, ro);
+        row_again<D, F16, AX, false>(p, b, h, ri, __shfl(lo, r, 64), __shfl(hi, r, 64), __shfl(m, r, 64), lane, ro);
         const float rinv = __shfl(inv, r, 64);
         uint16_t* op = p.out + b * p.o_s[0] + h * p.o_s[1] + (long)ri * p.o_s[2];
         if (lane < D) op[lane] = (uint16_t)pack2<F16>(ro[0] * rinv, 0.f);
@@ -399,8 +405,9 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
     float pq[AX ? AX : 1];
 #pragma unroll
     for (int a = 0; a < AX; ++a) pq[a] = (float)p.pos_q[b * p.pq_sb + (long)i * AX + a];
-    Form<CAP, AX> F;
+    Form<CAP, AX, true> F;      // (memory and latency are what bounds this form: tanh to its own size costs nothing here)
     F.init(p, h);
+    const float cap_k = CAP ? p.scale / p.cap : 0.f;
     const uint16_t* kp = p.k + b * p.k_s[0] + hk * p.k_s[1];
     const uint16_t* vp = p.v + b * p.v_s[0] + hk * p.v_s[1];
     const uint8_t* km = p.kmask ? p.kmask + b * p.km_sb : nullptr;
@@ -444,7 +451,12 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) s = mfma32<F16>(T::rows(Ks, c, 0, lane), qf[c], s);
-        if constexpr (CAP || AX > 0)
+        if constexpr (CAP) {
+            const SpanTanh tanh = span_tanh_block(s, cap_k);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = span_tanh_poly(s[r] * tanh.k, tanh.c);
+        }
+        if constexpr (AX > 0)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 f32x4_t pk[AX ? AX : 1];
@@ -453,7 +465,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
                 F.y4(s, g * 4, pq, pk);
             }
         if (keep != 0xFFFFFFFFu || !__all(lo <= t0 && hi >= t0 + 32)) F.hide(s, (uint32_t)((bit_range(lo - t0, hi - t0) & (unsigned long long)keep) >> (4 * half)));
-        rescale<D, F16>(F.score(F.extreme(s, Form<CAP, AX>::worst())), m, l, o);
+        rescale<D, F16>(F.score(F.extreme(s, Form<CAP, AX, true>::worst())), m, l, o);
         const float kbm = F.kb - m;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -529,7 +541,7 @@ __global__ __launch_bounds__(256, 2) void span_attn_narrow(const SpanArgs p) {
             xlo = max(sp.x, 0); xhi = min(sp.y, p.nk);
         }
         float ro[2];
-        row_again<D, F16, AX>(p, b, xh, xi, max(xlo, k0), min(xhi, k1), __shfl(M, src, 64), lane, ro);
+        row_again<D, F16, AX, true>(p, b, xh, xi, max(xlo, k0), min(xhi, k1), __shfl(M, src, 64), lane, ro);
         const float rinv = __shfl(inv, src, 64);
         if (p.splits == 1) {
             uint16_t* op = p.out + b * p.o_s[0] + xh * p.o_s[1] + (long)xi * p.o_s[2];

@@ -116,7 +116,7 @@ __device__ __forceinline__ void query_again(const SpanArgs& p, int b, int h, int
         const bool sees = key < k1 && (!p.kmask || p.kmask[b * p.km_sb + key]);
         float w = 0.f, slope;
         if (sees) {
-            const float s = pair_score<D, false, AX>(p, q, kb + (long)key * p.k_s[2], b, h, i, key, &slope);
+            const float s = pair_score<D, false, AX, false>(p, q, kb + (long)key * p.k_s[2], b, h, i, key, &slope);
             w = __builtin_amdgcn_exp2f(s - lse2) * (row_dot<D, false>(g, vb + (long)key * p.v_s[2]) - delta) * slope;
         }
         rows_add<D, false>(o, __ballot(sees), w, kb + (long)t0 * p.k_s[2], p.k_s[2], min(64, k1 - t0), lane);
@@ -142,7 +142,7 @@ __device__ __forceinline__ void key_again(const SpanArgs& p, int b, int hk, int 
             }
             if (sees) {
                 const long row = ((long)b * p.Hq + h) * p.nq + i;
-                const float s = pair_score<D, false, AX>(p, p.q + b * p.q_s[0] + h * p.q_s[1] + (long)i * p.q_s[2], k, b, h, i, key, &slope);
+                const float s = pair_score<D, false, AX, false>(p, p.q + b * p.q_s[0] + h * p.q_s[1] + (long)i * p.q_s[2], k, b, h, i, key, &slope);
                 w = __builtin_amdgcn_exp2f(s - p.lse[row] * SPAN_LOG2E);
                 ds = w * (row_dot<D, false>(p.dout + b * p.do_s[0] + h * p.do_s[1] + (long)i * p.do_s[2], v) - p.delta[row]) * slope;
             }

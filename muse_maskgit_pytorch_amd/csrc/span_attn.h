@@ -142,11 +142,12 @@ __device__ __forceinline__ float span_tanh(float x, float c1) {
     return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f), 1.f);
 }
 
-// tanh(u) to a few fp32 roundings of its own size, for the slopes' gradient: that is fp32, and a score that is off by a rounding of its cap leaves it 3 - 15 times as far from the
-// 64-bit form as a plain fp32 form is (scores of a few units under caps of 30 and 50).  |u| <= 1/2: u times a polynomial in u^2 (the minimax of the relative error, 1.5e-8, with 1 in
+// tanh(u) to a few fp32 roundings of its own size, for what is fp32 behind it, the slopes' gradients and the lse of few rows: a score that is off by a rounding of its cap leaves
+// them 3 - 15 times as far from the 64-bit form as a plain fp32 form is, a row of few keys 60 times (scores of a few units under caps of 30 and 50).  |u| <= 1/2: u times a polynomial in u^2 (the minimax of the relative error, 1.5e-8, with 1 in
 // front; Remez's exchange); beyond, the exponential.  A wave whose scores are all below takes the polynomial alone; otherwise the scores become their tanh first and the polynomial
 // leaves them as they are (its coefficients are 0): one code for both, and a score's value is the same either way, whatever stands beside it.
 struct SpanTanh { float k, c[4]; };
+constexpr float SPAN_TANH[4] = {-0.333331436f, 0.133258790f, -0.0530454926f, 0.0172414910f};
 __device__ __forceinline__ float span_tanh_poly(float u, const float (&c)[4]) {
     const float v = u * u;
     float t = __builtin_fmaf(c[3], v, c[2]);
@@ -154,23 +155,23 @@ __device__ __forceinline__ float span_tanh_poly(float u, const float (&c)[4]) {
     t = __builtin_fmaf(t, v, c[0]);
     return u * __builtin_fmaf(t, v, 1.f);
 }
+__device__ __forceinline__ float span_tanh_one(float u) {
+    const float far = span_tanh(u, 2.f * SPAN_LOG2E);
+    return fabsf(u) <= 0.5f ? span_tanh_poly(u, SPAN_TANH) : far;
+}
 // a block of raw scores in front of span_tanh_poly(raw * .k, .c) = tanh(raw k)
 __device__ __forceinline__ SpanTanh span_tanh_block(f32x16_t& s, float k) {
-    constexpr float C[4] = {-0.333331436f, 0.133258790f, -0.0530454926f, 0.0172414910f};
     float m[4] = {0.f, 0.f, 0.f, 0.f};      // (a NaN is passed over: the polynomial keeps it)
 #pragma unroll
     for (int r = 0; r < 16; ++r) m[r & 3] = fmaxf(m[r & 3], fabsf(s[r]));
     const bool near = __all(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * k <= 0.5f);
     if (!near)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float u = s[r] * k, far = span_tanh(u, 2.f * SPAN_LOG2E);
-            s[r] = fabsf(u) <= 0.5f ? span_tanh_poly(u, C) : far;
-        }
+        for (int r = 0; r < 16; ++r) s[r] = span_tanh_one(s[r] * k);
     SpanTanh t;
     t.k = near ? k : 1.f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) t.c[x] = near ? C[x] : 0.f;
+    for (int x = 0; x < 4; ++x) t.c[x] = near ? SPAN_TANH[x] : 0.f;
     return t;
 }
 
@@ -215,13 +216,13 @@ __device__ __forceinline__ void rows_add(float (&o)[2], unsigned long long sees,
 template <int D>
 __device__ __forceinline__ bool all_nan(const float (&o)[2], int lane) { return __all((lane >= D || o[0] != o[0]) && (D <= 64 || o[1] != o[1])); }
 
-// score (log2 units) of one visible pair by one lane; *slope: derivative of the cap
-template <int D, bool F16, int AX>
+// score (log2 units) of one visible pair by one lane; *slope: derivative of the cap; TANH: to its own size
+template <int D, bool F16, int AX, bool TANH>
 __device__ __forceinline__ float pair_score(const SpanArgs& p, const uint16_t* q, const uint16_t* k, int b, int h, int i, int key, float* slope) {
     float x = row_dot<D, F16>(q, k);
     *slope = 1.f;
     if (p.cap > 0.f) {
-        const float t = span_tanh(x, 2.f * p.scale * SPAN_LOG2E / p.cap);
+        const float t = TANH ? span_tanh_one(x * (p.scale / p.cap)) : span_tanh(x, 2.f * p.scale * SPAN_LOG2E / p.cap);
         *slope = 1.f - t * t;
         x = t * (p.cap * SPAN_LOG2E);
     } else x *= p.scale * SPAN_LOG2E;

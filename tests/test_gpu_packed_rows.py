@@ -575,6 +575,36 @@ def test_attend_spans_gradients_against_differences():
         assert abs(float((grad * e).sum()) - diff) < 3 * 2.0 ** -8 * float((grad * e).abs().sum()) + 1e-6, ('q', 'k', 'v', 'slopes')[n]
 
 
+CAPS = [(1e-3, 1.0), (1.0, 0.125), (30.0, 1.0), (50.0, 8.0), (1e4, 1.0)]
+
+
+@pytest.mark.parametrize('cap,scale', CAPS)
+@pytest.mark.parametrize('hq,n,d', [(1, 400, 64), (2, 400, 32), (1, 400, 128)])
+@pytest.mark.parametrize('axes', [0, 1])
+def test_a_capped_score_keeps_the_bits_of_its_own_size(axes, hq, n, d, cap, scale):
+    """few rows: a row that sees one key has that score as its lse, within a few fp32 roundings of the score itself, from 1e-6 of the cap to far beyond it, either sign, on tiles of
+    small scores alone and beside large ones"""
+    u = torch.cat([torch.logspace(-6, -0.05, 200), torch.logspace(-6, 1.5, 200)]).double()      # the first tiles stay below the cap, the others do not
+    u = u * torch.where(torch.arange(400) % 3 == 0, -1.0, 1.0)
+    q, k = torch.zeros(1, hq, n, d), torch.zeros(1, 1, n, d)
+    q[..., 5], k[..., 5] = 1.0, (u * cap / scale).float()
+    q, k = q.to(torch.bfloat16), k.to(torch.bfloat16)
+    at = torch.arange(n, dtype=torch.int32)
+    spans = torch.stack([at, at + 1], 1)
+    kw = {}
+    if axes:
+        kw = dict(slopes=torch.full((hq, 1), 0.25 * cap), positions=at[:, None] * 3, key_positions=at[:, None] * 3 - 1)
+    g = lambda t: t.to(DEV) if isinstance(t, torch.Tensor) else t
+    _, lse = ops.attend_spans(g(q), g(k), g(k), g(spans), scale=scale, softcap=cap, return_lse=True, **{a: g(b) for a, b in kw.items()})
+    want = cap * torch.tanh(k[0, 0, :, 5].double() * scale / cap)
+    size = want.abs()
+    if axes:
+        size = size + 0.25 * cap
+        want = want - 0.25 * cap
+    # scale / cap, its product, four roundings in tanh, the cap in units of log2, the product with it, back to natural units; log2 of the sum (exact: 1) -- a dozen at most
+    R.check(lse, want.expand(1, hq, n), (12 * R.F32 * size + 1e-37).expand(1, hq, n), 'lse')
+
+
 @pytest.mark.parametrize('d,hk', [(32, 2), (64, 4), (128, 2)])
 @pytest.mark.parametrize('cap,axes', [(1000.0, 1), (10000.0, 2)])
 @pytest.mark.parametrize('big', [False, True])
