@@ -316,7 +316,8 @@ int mm_rotary_axes_bwd(mm_stream_t stream, const mm_rotary* desc, float* dscales
  * q [B][Hq][nq][dim], k / v [B][Hk][nk][dim], Hk a divisor of Hq (query head h reads key head h / (Hq / Hk)); bf16 or fp16; dim 32, 64 or 128; element strides
  * (batch, head, token), multiples of 8, head elements contiguous, 16-byte aligned; token strides of k and v at least dim.  slopes fp32 [Hq][axes], axes 0 .. 3,
  * positions int32 [B][n][axes] (batch stride 0: one for all rows), |position| < 2^24 (a distance above 2^24 is rounded once to fp32).  lse fp32 [B][Hq][nq] (optional
- * in the forward).  scale 1e-20 .. 1e20; softcap 0 (none) or 1e-3 .. 1e4.  Scores are fp32: up to 1e7 in size, beyond which 32 bits do not tell one from the next.
+ * in the forward).  scale 1e-20 .. 1e20; softcap 0 (none) or 1e-3 .. 1e4; a capped score has the precision of softcap in fp32 (in calls of few rows, and in dslopes, its
+ * own).  Scores are fp32: up to 1e7 in size, beyond which 32 bits do not tell one from the next.
  * Few queries over many keys: the keys are split over workgroups, partial results in ws joined in a fixed order; many queries with spans: ws takes the order of their
  * tiles (mm_span_attention_workspace_bytes, may be 0).
  * What a row does not see never reaches it, infinities and NaN included.

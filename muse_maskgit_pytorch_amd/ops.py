@@ -1089,7 +1089,8 @@ def _span_args(q, k, v, spans, scale, softcap, slopes, positions, key_positions,
 def attend_spans(q, k, v, spans=None, scale=8.0, softcap=0.0, slopes=None, positions=None, key_positions=None, key_mask=None, return_lse=False, out_rows=False):
     """Attention of packed rows: q (b, hq, n, d), k / v (b, hk, j, d), bf16 or fp16, d = 32 / 64 / 128, hk a divisor of hq (shared key heads), strided views
     with 16-byte aligned rows.  A query sees the keys of its span (int32 (n, 2) or (b, n, 2), ops.attention_spans; None: all) that key_mask (b, j) keeps.
-    softcap > 0 (1e-3 .. 1e4; the score keeps the absolute precision of softcap in fp32): scores are softcap * tanh(score / softcap).  slopes fp32 (hq, axes) and positions / key_positions int32 (n, axes) / (j, axes) (or (b, .., axes);
+    softcap > 0 (1e-3 .. 1e4): scores are softcap * tanh(score / softcap), to the precision of softcap in fp32 (few rows, and the slopes' gradient: to the
+    score's own).  slopes fp32 (hq, axes) and positions / key_positions int32 (n, axes) / (j, axes) (or (b, .., axes);
     key_positions default: positions): sum over the axes of slope * |distance| is taken off the score; |position| < 2^24.  Scores are fp32, up to 1e7 in size (beyond,
     32 bits do not tell one from the next).  No autograd graph: attend_spans_bwd has the gradients.  A row that sees nothing gives 0
     (lse -inf); what a row does not see never reaches it, infinities and NaN included.  Returns (b, hq, n, d) (a view of rows), out_rows: [b * n, hq * d], and with
