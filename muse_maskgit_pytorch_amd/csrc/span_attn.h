@@ -142,10 +142,11 @@ __device__ __forceinline__ float span_tanh(float x, float c1) {
     return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c1) + 1.f), 1.f);
 }
 
-// tanh(u) to a few fp32 roundings of its own size, for what is fp32 behind it, the slopes' gradients and the lse of few rows: a score that is off by a rounding of its cap leaves
-// them 3 - 15 times as far from the 64-bit form as a plain fp32 form is, a row of few keys 60 times (scores of a few units under caps of 30 and 50).  |u| <= 1/2: u times a polynomial in u^2 (the minimax of the relative error, 1.5e-8, with 1 in
-// front; Remez's exchange); beyond, the exponential.  A wave whose scores are all below takes the polynomial alone; otherwise the scores become their tanh first and the polynomial
-// leaves them as they are (its coefficients are 0): one code for both, and a score's value is the same either way, whatever stands beside it.
+// tanh(u) to a few fp32 roundings of its own size, for what is fp32 behind it, the slopes' gradients and the lse of few rows: a score that is off by a rounding of its cap
+// leaves them 3 - 15 times as far from the 64-bit form as a plain fp32 form is, a row of few keys 60 times (scores of a few units under caps of 30 and 50).
+// |u| <= 1/2: u times a polynomial in u^2 (the minimax of the relative error, 1.5e-8, with 1 in front; Remez's exchange); beyond, the exponential.  A wave whose scores are all
+// below takes the polynomial alone; otherwise the scores become their tanh first and the polynomial leaves them as they are (its coefficients are 0): one code for both, whose
+// scores stay in their product's registers, and a score's value is the same either way, whatever stands beside it.
 struct SpanTanh { float k, c[4]; };
 constexpr float SPAN_TANH[4] = {-0.333331436f, 0.133258790f, -0.0530454926f, 0.0172414910f};
 __device__ __forceinline__ float span_tanh_poly(float u, const float (&c)[4]) {
